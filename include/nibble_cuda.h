@@ -57,7 +57,9 @@ typedef enum {
   NBL_Q5_1 = 6,
   NBL_Q4_K = 7,
   NBL_Q5_K = 8,
-  NBL_Q6_K = 9
+  NBL_Q6_K = 9,
+  NBL_I8 = 10,   /* K/V pools: 8-bit integer codes -127..127 with one fp32 scale per (16-token page, K/V, KV head) */
+  NBL_E4M3 = 11  /* K/V pools: 8-bit floats (4 exponent, 3 mantissa bits, largest 448) with the same scales */
 } nbl_dtype;
 
 typedef struct nbl_ctx nbl_ctx; /* device, stream, scratch, RoPE tables, allocation registry */
@@ -76,14 +78,43 @@ typedef struct {
  *   pool[page][2 (K then V)][n_kv_heads][page_size][head_dim]  (dtype F16 or BF16)
  * so the K rows of one (page, KV head) are one contiguous page_size*head_dim block. Sequences own pages
  * through page tables (int32 page ids, row-major [rows, pt_stride]); pages need not be contiguous or
- * ordered. Replaces the flat fp32 per-layer cache of src/model/transformer.cpp:74-90. */
+ * ordered. Replaces the flat fp32 per-layer cache of src/model/transformer.cpp:74-90.
+ *
+ * With dtype NBL_I8 or NBL_E4M3 the pool holds 8-bit codes (half the bytes of F16): an element is code * scale, with one
+ * fp32 scale per page, K or V, and KV head, so a scale spans 16 tokens of one head. The order of the codes inside a page
+ * is the library's own (the attention kernels' operand order): such a pool is written by nbl_rotary_kv_append and
+ * nbl_kv_import, read by nbl_attn_decode, nbl_attn_prefill, nbl_kv_read and nbl_kv_export. */
 typedef struct {
   int64_t n_pages;
   int32_t n_kv_heads;
-  int32_t head_dim;  /* 64 on the TMA/tensor-core kernels */
+  int32_t head_dim;  /* 64; 64 or 128 for the 8-bit dtypes */
   int32_t page_size; /* 16 */
-  int32_t dtype;     /* NBL_F16 or NBL_BF16 */
+  int32_t dtype;     /* NBL_F16, NBL_BF16, NBL_I8 or NBL_E4M3 */
 } nbl_kv_config;
+
+/* How rotary positions are stretched for a context longer than the one a model was trained for. */
+typedef enum {
+  NBL_ROTARY_NONE = 0,
+  NBL_ROTARY_LINEAR = 1,     /* every frequency / factor */
+  NBL_ROTARY_NTK = 2,        /* base * factor^(n / (n - 2)), n rotated elements */
+  NBL_ROTARY_YARN = 3,       /* slow pairs interpolated, fast ones kept, a ramp between; cos and sin * attn_factor */
+  NBL_ROTARY_WAVELENGTH = 4  /* the same by wavelength against original_ctx / low_ and high_freq_factor */
+} nbl_rotary_scaling;
+
+/* Rotary positions of part of a head: the first rotary_dim elements rotate, the rest pass unchanged. Pair i of n =
+ * rotary_dim turns by pos * freq_base^(-2i/n), changed by the scaling, divided by freq_factors[i] if given. */
+typedef struct {
+  float freq_base;     /* > 1 */
+  int32_t neox;        /* nonzero: pairs (i, i + n/2); zero: (2i, 2i + 1) */
+  int32_t rotary_dim;  /* even, <= head_dim; 0: head_dim */
+  int32_t scaling;     /* nbl_rotary_scaling */
+  float factor;        /* >= 1; new context / original one */
+  int32_t original_ctx;                     /* yarn, wavelength: tokens of the original context */
+  float beta_fast, beta_slow;               /* yarn: turns over the original context (usually 32 and 1) */
+  float low_freq_factor, high_freq_factor;  /* wavelength (usually 1 and 4) */
+  float attn_factor;   /* factor on cos and sin; 0: 0.1 ln(factor) + 1 for yarn, else 1 */
+  const float* freq_factors;  /* HOST memory, rotary_dim / 2 floats, or NULL */
+} nbl_rotary_params;
 
 /* ABI version the library was built with (NBL_ABI_VERSION). */
 NBL_API int nbl_abi_version(void);
@@ -223,7 +254,10 @@ NBL_API int nbl_rope_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const
  * seq_lens[r] == 0 gives out = 0 and lse = -inf. max_seq_len bounds every seq_lens[r] (it sizes the splits;
  * the kernel also checks each length against pt_stride * page_size). n_splits: KV splits per row (0 = chosen
  * from the sizes); more than one uses context scratch sized by nbl_reserve (grown on demand otherwise).
- * head_dim 64, n_heads / n_kv_heads <= 8. */
+ * head_dim 64, n_heads / n_kv_heads <= 8.
+ * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes any group size; the split count is then an upper bound, each
+ * row's own pages being divided evenly, and its results are the softmax over the values that the codes stand for, to
+ * fp32 accuracy. */
 NBL_API int nbl_attn_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_t* page_table, int32_t pt_stride,
                     const int32_t* seq_lens, int32_t max_seq_len, int32_t n_rows, int32_t n_heads, float* out,
                     float* lse, int32_t n_splits);
@@ -267,11 +301,73 @@ NBL_API int nbl_attn_decode_static(nbl_ctx* ctx, const nbl_kv* kv, const float* 
  * (q_dtype = the pool dtype, already roped) at positions kv_pos0[i] + t, attending keys 0..kv_pos0[i]+t of
  * page-table row i (those keys must already be in the pool). max_q_len bounds every q_len[i]. Writes the
  * items' out rows in out_dtype (F32 or the pool dtype). Tensor-core kernel (tcgen05): bf16/fp16 operands, fp32
- * accumulation in TMEM. */
+ * accumulation in TMEM.
+ * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes q in F32, F16 or BF16 and writes out in F32 or q's dtype;
+ * the scales are applied to scores and weights in fp32, the weights of 16-bit queries are rounded to fp16. */
 NBL_API int nbl_attn_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype, int64_t n_q_rows,
                      const int32_t* q_start, const int32_t* q_len, const int32_t* kv_pos0, const int32_t* page_table,
                      int32_t pt_stride, int32_t n_items, int32_t n_heads, int32_t max_q_len, void* out,
                      int32_t out_dtype);
+
+/* ---- the 8-bit K/V pool: writing and reading it ---- */
+/* New tokens into an 8-bit pool in one launch: bias, rotary positions, quantization and page write, and the rotated
+ * queries. Item i (page-table row i) appends the q_len[i] tokens of activation rows q_start[i].. at positions
+ * kv_pos0[i].. ; its positions before kv_pos0[i] are in the pool already, its later ones are dropped:
+ *   q_out[r] = rotary(q_in[r] + bq),   K <- quantize(rotary(k_in[r] + bk)),   V <- quantize(v_in[r] + bv)
+ * q_in / q_out [n_rows, n_heads, head_dim], k_in / v_in [n_rows, n_kv_heads, head_dim] of in_dtype (F32, F16 or BF16;
+ * q_out of q_out_dtype, which may alias q_in when the dtypes match); biases fp32 device vectors or NULL. max_q_len bounds
+ * every q_len. In a page that already holds tokens, s = max(old scale, largest new magnitude / 127 (I8) or 448 (E4M3)):
+ * when the scale grows the old codes are rounded again to it (at most half a step of the new scale each time).
+ * Magnitudes below 1e-30 in a whole page are stored as 0; an infinity or NaN is stored saturated or as 0 and flagged
+ * (nbl_ctx_check). A page may be written by one item only in a call. */
+NBL_API int nbl_rotary_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const void* k_in, const void* v_in,
+                                 int32_t in_dtype, const float* bq, const float* bk, const float* bv, void* q_out,
+                                 int32_t q_out_dtype, int64_t n_rows, const int32_t* q_start, const int32_t* q_len,
+                                 const int32_t* kv_pos0, const int32_t* page_table, int32_t pt_stride, int32_t n_items,
+                                 int32_t n_heads, int32_t max_q_len, const nbl_rotary_params* rotary);
+/* The values that an 8-bit pool stands for: item i's positions kv_pos0[i] .. + len[i] as rows start[i].. of k_out / v_out
+ * ([n_rows, n_kv_heads, head_dim] of out_dtype; either may be NULL), code * scale rounded once. max_len bounds every
+ * len. */
+NBL_API int nbl_kv_read(nbl_ctx* ctx, const nbl_kv* kv, int64_t n_rows, const int32_t* start, const int32_t* len,
+                        const int32_t* kv_pos0, const int32_t* page_table, int32_t pt_stride, int32_t n_items,
+                        int32_t max_len, void* k_out, void* v_out, int32_t out_dtype);
+/* Whole pages of an 8-bit pool from / to a plain layout: codes [n, 2 (K, V), n_kv_heads, 16, head_dim] (int8, or e4m3
+ * bytes) and scales [n, 2, n_kv_heads] fp32, page page_ids[i] from or to entry i (all device memory). Import stores a
+ * code or scale that is not finite, or a negative scale, as 0 and flags it; code -128 is stored as it is. */
+NBL_API int nbl_kv_import(nbl_ctx* ctx, nbl_kv* kv, const int32_t* page_ids, int64_t n, const void* codes,
+                          const float* scales);
+NBL_API int nbl_kv_export(nbl_ctx* ctx, const nbl_kv* kv, const int32_t* page_ids, int64_t n, void* codes,
+                          float* scales);
+
+/* ---- page bookkeeping on the device, for pools of every dtype ----
+ * page_table [n_rows, pt_stride] (-1: no page), seq_lens [n_rows] tokens and ref_counts [n_pages] (how many table entries
+ * name the page; 0: free) are the caller's device memory, kept consistent by these calls. A forked row shares its source's
+ * full pages and owns a copy of the part-filled last one, so a page that is shared is never appended to. Free pages
+ * are handed out lowest id first in the order of the request list. Row lists are device memory; a bad row, or one named
+ * twice, is skipped and flagged (nbl_ctx_check), as is a request for which the pool has no free page. */
+/* Copies page src_pages[i] to dst_pages[i] (no page may be both a source and a destination, or a destination twice). */
+NBL_API int nbl_kv_copy_pages(nbl_ctx* ctx, nbl_kv* kv, const int32_t* src_pages, const int32_t* dst_pages, int32_t n);
+/* Row dst_rows[i] becomes a branch of src_rows[i], i < n: what it held is released, it shares the source's full pages and
+ * gets a copy of the part-filled one. Destinations are distinct and none is a source. Without a free page the branch
+ * keeps the full pages only. */
+NBL_API int nbl_kv_fork(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride, int32_t n_rows,
+                        int32_t* seq_lens, int32_t* ref_counts, const int32_t* src_rows, const int32_t* dst_rows,
+                        int32_t n);
+/* Rows give their pages back (a page is free once no row names it); their lengths become 0. */
+NBL_API int nbl_kv_release(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride, int32_t n_rows,
+                           int32_t* seq_lens, int32_t* ref_counts, const int32_t* rows, int32_t n);
+/* Row rows[i] grows to new_lens[i] tokens: gets the pages that it lacks, and its length. Every row gets its pages, or (too
+ * few free ones) none does. Rows are distinct. */
+NBL_API int nbl_kv_extend(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride, int32_t n_rows,
+                          int32_t* seq_lens, int32_t* ref_counts, const int32_t* rows, const int32_t* new_lens,
+                          int32_t n);
+/* Moves the pages that the rows hold from pool src into pool dst (of the same shape but for n_pages): pages take ids 0, 1,
+ * ... by their first appearance in the table, row by row, so a row's own pages are adjacent and shared pages are
+ * moved once. Writes table_out [n_rows, pt_stride], ref_counts_out [dst pages] and n_used (the distinct pages); if
+ * they exceed dst the rest is left out of the table and flagged. src and its table stay as they are. */
+NBL_API int nbl_kv_compact(nbl_ctx* ctx, const nbl_kv* src, nbl_kv* dst, const int32_t* page_table, int32_t pt_stride,
+                           int32_t n_rows, const int32_t* seq_lens, int32_t* table_out, int32_t* ref_counts_out,
+                           int32_t* n_used);
 
 /* Log-sum-exp merge of n_parts partial results of the same rows (e.g. per-GPU KV chunks after an
  * all-gather): part_o [n_parts, rows, head_dim] normalised outputs, part_lse [n_parts, rows] natural-log

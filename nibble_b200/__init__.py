@@ -14,9 +14,9 @@ import ctypes as C
 from dataclasses import dataclass
 
 from . import _abi
-from ._abi import BF16, F16, F32, Q4_0, Q4_K, Q5_0, Q5_1, Q5_K, Q6_K, Q8_0, NibbleError, check
+from ._abi import BF16, E4M3, F16, F32, I8, Q4_0, Q4_K, Q5_0, Q5_1, Q5_K, Q6_K, Q8_0, NibbleError, check
 
-__all__ = ["Context", "KVPool", "Weight", "NibbleError", "RopeSpec", "F32", "F16", "BF16", "Q4_0", "Q5_0", "Q8_0", "Q5_1",
+__all__ = ["Context", "KVPool", "Weight", "NibbleError", "RopeSpec", "RotarySpec", "F32", "F16", "BF16", "I8", "E4M3", "Q4_0", "Q5_0", "Q8_0", "Q5_1",
            "Q4_K", "Q5_K", "Q6_K",
            "abi_version"]
 
@@ -39,6 +39,36 @@ class RopeSpec:
             ff = (C.c_float * len(self.freq_factors))(*self.freq_factors)
             ptr = C.cast(ff, C.c_void_p)
         return _abi.RopeParams(self.freq_base, int(self.neox), ptr), ff
+
+
+@dataclass(frozen=True)
+class RotarySpec:
+    """Rotary positions of part of a head, stretched for long contexts (nbl_rotary_params): the first rotary_dim elements
+    (0: all) rotate, as pairs (i, i + n/2) with neox, else (2i, 2i + 1). scaling: "none", "linear", "ntk", "yarn" or
+    "wavelength", for a context `factor` times the original one of original_ctx tokens."""
+    freq_base: float
+    neox: bool
+    rotary_dim: int = 0
+    scaling: str = "none"
+    factor: float = 1.0
+    original_ctx: int = 0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    attn_factor: float = 0.0
+    freq_factors: tuple | None = None
+
+    def _c(self):
+        if self.scaling not in _abi.ROTARY_SCALING:
+            raise ValueError(f"unknown rotary scaling {self.scaling!r} (one of {', '.join(_abi.ROTARY_SCALING)})")
+        ff = ptr = None
+        if self.freq_factors is not None:
+            ff = (C.c_float * len(self.freq_factors))(*self.freq_factors)
+            ptr = C.cast(ff, C.c_void_p)
+        return _abi.RotaryParams(self.freq_base, int(self.neox), self.rotary_dim, _abi.ROTARY_SCALING[self.scaling],
+                                 self.factor, self.original_ctx, self.beta_fast, self.beta_slow, self.low_freq_factor,
+                                 self.high_freq_factor, self.attn_factor, ptr), ff
 
 
 _DT = {"float32": F32, "float16": F16, "bfloat16": BF16}
@@ -68,8 +98,15 @@ def _dtype(t) -> int:
     return _DT[name]
 
 
+def _same_shape(kv, q, k, v):
+    if tuple(q.shape[2:]) != (kv.head_dim,) or tuple(k.shape) != (q.shape[0], kv.n_kv_heads, kv.head_dim) \
+            or v.shape != k.shape:
+        raise ValueError(f"expected q [rows, n_heads, {kv.head_dim}] and k, v [rows, {kv.n_kv_heads}, {kv.head_dim}]")
+
+
 class KVPool:
-    """A paged K/V pool: pool[page][2][n_kv_heads][page_size][head_dim] (fp16 or bf16)."""
+    """A paged K/V pool: pool[page][2][n_kv_heads][page_size][head_dim] (fp16 or bf16), or with dtype I8 / E4M3 8-bit
+    codes with a scale per (page, K/V, head), in an order of the library's own (Context.kv_import / kv_export)."""
 
     def __init__(self, ctx: "Context", n_pages: int, n_kv_heads: int, head_dim: int = 64, page_size: int = 16,
                  dtype: int = F16):
@@ -78,6 +115,7 @@ class KVPool:
         h = C.c_void_p()
         check(_abi.lib.nbl_kv_create(ctx.handle, C.byref(cfg), C.byref(h)))
         self.handle = h
+        self._memory, self._tensor = _PoolMemory(ctx, h), None
         self.n_pages, self.n_kv_heads, self.head_dim, self.page_size, self.dtype = (n_pages, n_kv_heads, head_dim,
                                                                                     page_size, dtype)
         base, nbytes = C.c_void_p(), C.c_int64()
@@ -88,13 +126,45 @@ class KVPool:
         """The pool's raw 16-bit elements as a torch int16 view [n_pages, 2, n_kv_heads, page_size, head_dim]
         (aliases the pool; no copy). Reinterpret with .view(torch.float16 / torch.bfloat16)."""
         import torch
-        t = _wrap_device_memory(self.base, self.nbytes // 2, torch.int16, self.ctx.device)
-        return t.view(self.n_pages, 2, self.n_kv_heads, self.page_size, self.head_dim)
+        if self.dtype in (I8, E4M3):
+            raise ValueError("an 8-bit pool has no plain view: use Context.kv_read, kv_export and kv_import")
+        if self._tensor is None:
+            t = _wrap_device_memory(self.base, self.nbytes // 2, torch.int16, self.ctx.device, self._memory)
+            self._tensor = t.view(self.n_pages, 2, self.n_kv_heads, self.page_size, self.head_dim)
+        return self._tensor.view(self._tensor.shape)
 
     def close(self):
-        if self.handle:
-            check(_abi.lib.nbl_kv_destroy(self.handle))
-            self.handle = None
+        """Frees the pool; while tensors from tensor() are alive, once the last of them is gone."""
+        self.handle = self._tensor = None
+        self._memory.close()
+
+
+class _PoolMemory:
+    """A pool's device memory: freed when the pool is closed and no tensor views it any more."""
+
+    def __init__(self, ctx: "Context", handle):
+        self.ctx, self.handle, self.views, self.closing = ctx, handle, 0, False
+
+    def close(self):
+        self.closing = True
+        if self.handle and not self.views:
+            handle, self.handle = self.handle, None
+            if self.ctx.handle:  # a closed context has freed its pools
+                check(_abi.lib.nbl_kv_destroy(handle))
+
+
+class _View:
+    """What a tensor over a pool's memory holds on to."""
+
+    def __init__(self, memory: _PoolMemory, interface: dict):
+        self.__cuda_array_interface__ = interface
+        self.memory = memory
+        memory.views += 1
+
+    def __del__(self):
+        self.memory.views -= 1
+        if self.memory.closing:
+            self.memory.close()
 
 
 class Weight:
@@ -127,19 +197,14 @@ class Weight:
             self.handle = None
 
 
-def _wrap_device_memory(ptr: int, numel: int, dtype, device: int):
-    """A torch tensor aliasing `numel` elements of device memory at `ptr` (owned elsewhere)."""
+def _wrap_device_memory(ptr: int, numel: int, dtype, device: int, memory: _PoolMemory):
+    """A torch tensor aliasing `numel` elements of the pool's device memory at `ptr`."""
     import torch
-
-    class _Holder:
-        def __init__(self):
-            elsize = torch.empty((), dtype=dtype).element_size()
-            self.__cuda_array_interface__ = {
-                "shape": (numel,), "typestr": {torch.int16: "<i2", torch.float32: "<f4"}[dtype],
-                "data": (ptr, False), "version": 3, "strides": (elsize,)}
-
+    elsize = torch.empty((), dtype=dtype).element_size()
+    view = _View(memory, {"shape": (numel,), "typestr": {torch.int16: "<i2", torch.float32: "<f4"}[dtype],
+                          "data": (ptr, False), "version": 3, "strides": (elsize,)})
     with torch.cuda.device(device):
-        return torch.as_tensor(_Holder(), device=f"cuda:{device}")
+        return torch.as_tensor(view, device=f"cuda:{device}")
 
 
 class Context:
@@ -289,6 +354,70 @@ class Context:
         check(_abi.lib.nbl_attn_prefill(self.handle, kv.handle, _ptr(q), _dtype(q), q.shape[0], _ptr(q_start),
                                         _ptr(q_len), _ptr(kv_pos0), _ptr(page_table), page_table.shape[-1],
                                         q_start.shape[0], q.shape[1], max_q_len, _ptr(out), _dtype(out)))
+
+    # ---- the 8-bit cache (kv_pool with dtype I8 or E4M3)
+    def rotary_kv_append(self, kv: KVPool, q_in, k_in, v_in, q_out, q_start, q_len, kv_pos0, page_table, max_q_len: int,
+                         rotary: RotarySpec, bq=None, bk=None, bv=None):
+        """Fused bias -> rotary -> quantization -> page write of item i's q_len[i] tokens (rows q_start[i].. of q_in
+        [rows, n_heads, D], k_in and v_in [rows, n_kv_heads, D]) at positions kv_pos0[i].. of page-table row i, and the
+        rotated queries into q_out (see nbl_rotary_kv_append)."""
+        p, keep = rotary._c()
+        in_dt = _dtype(q_in)
+        if _dtype(k_in) != in_dt or _dtype(v_in) != in_dt:
+            raise ValueError("q_in, k_in, v_in must share a dtype")
+        _same_shape(kv, q_in, k_in, v_in)
+        if rotary.freq_factors is not None and len(rotary.freq_factors) != (rotary.rotary_dim or kv.head_dim) // 2:
+            raise ValueError("freq_factors must hold rotary_dim / 2 factors")
+        check(_abi.lib.nbl_rotary_kv_append(
+            self.handle, kv.handle, _ptr(q_in), _ptr(k_in), _ptr(v_in), in_dt, _ptr(bq), _ptr(bk), _ptr(bv),
+            _ptr(q_out), _dtype(q_out), q_in.shape[0], _ptr(q_start), _ptr(q_len), _ptr(kv_pos0), _ptr(page_table),
+            page_table.shape[-1], q_start.shape[0], q_in.shape[1], max_q_len, C.byref(p)))
+
+    def kv_read(self, kv: KVPool, start, length, kv_pos0, page_table, max_len: int, k_out=None, v_out=None):
+        """Item i's positions kv_pos0[i].. as rows start[i].. of k_out / v_out [rows, n_kv_heads, D] (see nbl_kv_read)."""
+        like = k_out if k_out is not None else v_out
+        check(_abi.lib.nbl_kv_read(self.handle, kv.handle, like.shape[0], _ptr(start), _ptr(length), _ptr(kv_pos0),
+                                   _ptr(page_table), page_table.shape[-1], start.shape[0], max_len, _ptr(k_out),
+                                   _ptr(v_out), _dtype(like)))
+
+    def kv_import(self, kv: KVPool, page_ids, codes, scales):
+        """codes [n, 2, n_kv_heads, 16, D] (int8 / float8_e4m3fn) and scales [n, 2, n_kv_heads] fp32 into pages page_ids."""
+        check(_abi.lib.nbl_kv_import(self.handle, kv.handle, _ptr(page_ids), page_ids.shape[0], _ptr(codes),
+                                     _ptr(scales)))
+
+    def kv_export(self, kv: KVPool, page_ids, codes, scales):
+        check(_abi.lib.nbl_kv_export(self.handle, kv.handle, _ptr(page_ids), page_ids.shape[0], _ptr(codes),
+                                     _ptr(scales)))
+
+    # ---- page bookkeeping on the device (int32 CUDA tensors: page_table [rows, stride], seq_lens [rows],
+    # ref_counts [n_pages])
+    def kv_copy_pages(self, kv: KVPool, src_pages, dst_pages):
+        check(_abi.lib.nbl_kv_copy_pages(self.handle, kv.handle, _ptr(src_pages), _ptr(dst_pages), src_pages.shape[0]))
+
+    def kv_fork(self, kv: KVPool, page_table, seq_lens, ref_counts, src_rows, dst_rows):
+        """Row dst_rows[i] becomes a branch of src_rows[i]: full pages shared, the part-filled one copied."""
+        check(_abi.lib.nbl_kv_fork(self.handle, kv.handle, _ptr(page_table), page_table.shape[-1], page_table.shape[0],
+                                   _ptr(seq_lens), _ptr(ref_counts), _ptr(src_rows), _ptr(dst_rows),
+                                   src_rows.shape[0]))
+
+    def kv_release(self, kv: KVPool, page_table, seq_lens, ref_counts, rows):
+        check(_abi.lib.nbl_kv_release(self.handle, kv.handle, _ptr(page_table), page_table.shape[-1],
+                                      page_table.shape[0], _ptr(seq_lens), _ptr(ref_counts), _ptr(rows),
+                                      rows.shape[0]))
+
+    def kv_extend(self, kv: KVPool, page_table, seq_lens, ref_counts, rows, new_lens):
+        """Row rows[i] gets the pages that new_lens[i] tokens need, lowest free ids first, and that length."""
+        check(_abi.lib.nbl_kv_extend(self.handle, kv.handle, _ptr(page_table), page_table.shape[-1],
+                                     page_table.shape[0], _ptr(seq_lens), _ptr(ref_counts), _ptr(rows),
+                                     _ptr(new_lens), rows.shape[0]))
+
+    def kv_compact(self, src: KVPool, dst: KVPool, page_table, seq_lens, table_out, ref_counts_out, n_used):
+        """The rows' pages move from pool src into pool dst, numbered by first appearance; src stays as it is."""
+        if table_out.shape != page_table.shape or ref_counts_out.shape[0] < dst.n_pages:
+            raise ValueError("table_out must have page_table's shape and ref_counts_out one count per page of dst")
+        check(_abi.lib.nbl_kv_compact(self.handle, src.handle, dst.handle, _ptr(page_table), page_table.shape[-1],
+                                      page_table.shape[0], _ptr(seq_lens), _ptr(table_out), _ptr(ref_counts_out),
+                                      _ptr(n_used)))
 
     def lse_merge_packed(self, packed, n_parts: int, rows: int, head_dim: int, out, lse=None):
         """packed [n_parts, rows * (head_dim + 1)] fp32 (per part: outputs then lse) -> out [rows, head_dim]."""

@@ -14,6 +14,8 @@ LIB_PATH = os.path.join(_HERE, "libnibble_cuda.so")
 
 NBL_OK, NBL_E_INVALID, NBL_E_CUDA, NBL_E_NOMEM, NBL_E_UNSUPPORTED, NBL_E_DEVICE = range(6)
 F32, F16, BF16, Q4_0, Q5_0, Q8_0, Q5_1, Q4_K, Q5_K, Q6_K = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9
+I8, E4M3 = 10, 11  # K/V pools only
+ROTARY_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "wavelength": 4}
 STATUS_NAMES = {0: "NBL_OK", 1: "NBL_E_INVALID", 2: "NBL_E_CUDA", 3: "NBL_E_NOMEM", 4: "NBL_E_UNSUPPORTED",
                 5: "NBL_E_DEVICE"}
 
@@ -28,6 +30,13 @@ class NibbleError(RuntimeError):
 
 class RopeParams(C.Structure):
     _fields_ = [("freq_base", C.c_float), ("neox", C.c_int32), ("freq_factors", C.c_void_p)]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [("freq_base", C.c_float), ("neox", C.c_int32), ("rotary_dim", C.c_int32), ("scaling", C.c_int32),
+                ("factor", C.c_float), ("original_ctx", C.c_int32), ("beta_fast", C.c_float), ("beta_slow", C.c_float),
+                ("low_freq_factor", C.c_float), ("high_freq_factor", C.c_float), ("attn_factor", C.c_float),
+                ("freq_factors", C.c_void_p)]
 
 
 class KvConfig(C.Structure):
@@ -69,6 +78,16 @@ SIGNATURES = {
     "nbl_decode_step_host": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _I32, _I32, _I32, C.POINTER(RopeParams),
                              _P, _I32],
     "nbl_attn_prefill": [_P, _P, _P, _I32, _I64, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _P, _I32],
+    "nbl_rotary_kv_append": [_P, _P, _P, _P, _P, _I32, _P, _P, _P, _P, _I32, _I64, _P, _P, _P, _P, _I32, _I32, _I32, _I32,
+                             C.POINTER(RotaryParams)],
+    "nbl_kv_read": [_P, _P, _I64, _P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _I32],
+    "nbl_kv_import": [_P, _P, _P, _I64, _P, _P],
+    "nbl_kv_export": [_P, _P, _P, _I64, _P, _P],
+    "nbl_kv_copy_pages": [_P, _P, _P, _P, _I32],
+    "nbl_kv_fork": [_P, _P, _P, _I32, _I32, _P, _P, _P, _P, _I32],
+    "nbl_kv_release": [_P, _P, _P, _I32, _I32, _P, _P, _P, _I32],
+    "nbl_kv_extend": [_P, _P, _P, _I32, _I32, _P, _P, _P, _P, _I32],
+    "nbl_kv_compact": [_P, _P, _P, _P, _I32, _I32, _P, _P, _P, _P],
     "nbl_lse_merge": [_P, _P, _P, _I32, _I64, _I32, _P, _P],
     "nbl_lse_merge_packed": [_P, _P, _I32, _I64, _I32, _P, _P],
     "nbl_weight_create": [_P, _P, _I32, _I64, _I64, C.POINTER(_P)],

@@ -12,6 +12,8 @@
 #include <new>
 #include <string>
 
+#include "kv8.cuh"
+#include "kv_pages.h"
 #include "model_ops.h"
 #include "nbl_internal.h"
 
@@ -288,6 +290,62 @@ void qblock_matmul(nbl_ctx* ctx, const nbl_weight* w, float* y, const float* x, 
   nbl::launch_qblock_matmul(ctx->stream, w->w, y, x, n, ctx->qblock_act, ctx->num_sms);
 }
 
+// Attention over an 8-bit pool: plans the splits, grows the scratch and launches.
+void kv8_attention(nbl_ctx* ctx, const nbl_kv* kv, const nbl::Kv8Items& it, const void* q, int q_dtype, int n_heads,
+                   void* out, int out_dtype, float* lse, int max_kv, int n_splits) {
+  use_device(ctx);
+  const auto plan = nbl::plan_kv8_attn(kv, it.n_items, it.max_len, it.n_rows, n_heads, max_kv, q_dtype, ctx->num_sms,
+                                       n_splits);
+  unsigned* counts = nullptr;
+  if (plan.n_splits > 1) {
+    ensure_scratch(ctx, plan.scratch_bytes);
+    counts = nbl::split_counts(ctx, plan.units);
+  }
+  nbl::launch_kv8_attn(ctx->stream, kv, it, q, q_dtype, n_heads, out, out_dtype, lse, plan, ctx->scratch, counts,
+                       ctx->d_err);
+}
+
+// nbl_attn_decode on an 8-bit pool (pointers and context checked).
+void kv8_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_t* page_table, int32_t pt_stride,
+                const int32_t* seq_lens, int32_t max_seq_len, int32_t n_rows, int32_t n_heads, float* out, float* lse,
+                int32_t n_splits) {
+  require(n_rows >= 0 && pt_stride > 0 && max_seq_len >= 0 && n_splits >= 0, "attn_decode: negative size");
+  require(n_heads > 0 && n_heads % kv->cfg.n_kv_heads == 0, "attn_decode: n_heads must be a multiple of n_kv_heads");
+  require(int64_t(pt_stride) * kv->cfg.page_size <= INT32_MAX && int64_t(max_seq_len) <= int64_t(pt_stride) * kv->cfg.page_size,
+          "attn_decode: max_seq_len exceeds pt_stride * page_size");
+  if (n_rows == 0) return;
+  nbl::Kv8Items it;
+  it.pos0 = seq_lens;
+  it.page_table = page_table;
+  it.pt_stride = pt_stride;
+  it.n_items = n_rows;
+  it.max_len = 1;
+  it.n_rows = n_rows;
+  kv8_attention(ctx, kv, it, q, NBL_F32, n_heads, out, NBL_F32, lse, max_seq_len, n_splits);
+}
+
+// nbl_attn_prefill on an 8-bit pool (pointers and context checked).
+void kv8_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype, int64_t n_q_rows,
+                 const int32_t* q_start, const int32_t* q_len, const int32_t* kv_pos0, const int32_t* page_table,
+                 int32_t pt_stride, int32_t n_items, int32_t n_heads, int32_t max_q_len, void* out, int32_t out_dtype) {
+  require(is_dtype(q_dtype) && (out_dtype == NBL_F32 || out_dtype == q_dtype),
+          "attn_prefill: q must be F32, F16 or BF16, and out F32 or of q's dtype");
+  require(n_items >= 0 && pt_stride > 0 && max_q_len >= 0 && n_q_rows >= 0, "attn_prefill: negative size");
+  require(int64_t(pt_stride) * kv->cfg.page_size <= INT32_MAX, "attn_prefill: pt_stride too large");
+  require(n_heads > 0 && n_heads % kv->cfg.n_kv_heads == 0, "attn_prefill: n_heads must be a multiple of n_kv_heads");
+  if (n_items == 0 || max_q_len == 0 || n_q_rows == 0) return;
+  nbl::Kv8Items it;
+  it.start = q_start;
+  it.len = q_len;
+  it.pos0 = kv_pos0;
+  it.page_table = page_table;
+  it.pt_stride = pt_stride;
+  it.n_items = n_items;
+  it.max_len = max_q_len;
+  it.n_rows = n_q_rows;
+  kv8_attention(ctx, kv, it, q, q_dtype, n_heads, out, out_dtype, nullptr, pt_stride * kv->cfg.page_size, 0);
+}
+
 void require_weight(const nbl_ctx* ctx, const nbl_weight* w, const char* what) {
   require(w != nullptr && w->ctx == ctx, std::string(what) + ": weight is NULL or belongs to another context");
 }
@@ -359,6 +417,7 @@ int nbl_ctx_destroy(nbl_ctx* ctx) {
     if (ctx->qblock_act) cudaFree(ctx->qblock_act);
     for (auto& a : ctx->allocs) cudaFree(a.first);
     for (auto& t : ctx->rope_tables) cudaFree(t.dev);
+    for (auto& t : ctx->rotary_tables) cudaFree(t.dev);
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->split_counts) cudaFree(ctx->split_counts);
     if (ctx->io) cudaFree(ctx->io);
@@ -413,6 +472,9 @@ int nbl_ctx_check(nbl_ctx* ctx) {
       if (host & nbl::kErrTimeout) what += " a bounded wait on a copy or MMA completion gave up;";
       if (host & nbl::kErrTmemAlloc) what += " tensor-memory allocation failed;";
       if (host & nbl::kErrSmemAlign) what += " shared memory was not 1024-byte aligned;";
+      if (host & nbl::kErrNoPage) what += " no free page left in the pool;";
+      if (host & nbl::kErrNonFinite) what += " an infinity or NaN was given to the 8-bit cache;";
+      if (host & nbl::kErrRow) what += " page-table row outside the table, or named twice;";
       nbl::fail(NBL_E_DEVICE, "device-side check failed (flags " + std::to_string(host) + "):" + what);
     }
   });
@@ -559,23 +621,43 @@ int nbl_kv_create(nbl_ctx* ctx, const nbl_kv_config* cfg, nbl_kv** out) {
     const nbl_kv_config c = *cfg;
     require(c.n_pages > 0 && c.n_kv_heads > 0 && c.head_dim > 0 && c.page_size > 0,
             "kv_create: n_pages, n_kv_heads, head_dim and page_size must be positive");
-    require(c.dtype == NBL_F16 || c.dtype == NBL_BF16, "kv_create: dtype must be NBL_F16 or NBL_BF16");
-    if (c.head_dim != 64 || c.page_size != 16)
+    const bool kv8 = nbl::is_kv8(c.dtype);
+    require(c.dtype == NBL_F16 || c.dtype == NBL_BF16 || kv8,
+            "kv_create: dtype must be NBL_F16, NBL_BF16, NBL_I8 or NBL_E4M3");
+    if (kv8) {
+      if ((c.head_dim != 64 && c.head_dim != 128) || c.page_size != 16)
+        nbl::fail(NBL_E_UNSUPPORTED, "kv_create: the 8-bit kernels take head_dim 64 or 128 and page_size 16 (got " +
+                                         std::to_string(c.head_dim) + ", " + std::to_string(c.page_size) + ")");
+      require(c.n_pages <= INT32_MAX && c.n_kv_heads <= 65535, "kv_create: too many pages or KV heads");
+    } else if (c.head_dim != 64 || c.page_size != 16)
       nbl::fail(NBL_E_UNSUPPORTED, "kv_create: the paged kernels take head_dim 64 and page_size 16 (got " +
                                        std::to_string(c.head_dim) + ", " + std::to_string(c.page_size) + ")");
     const uint64_t rows = static_cast<uint64_t>(c.n_pages) * 2u * static_cast<uint64_t>(c.n_kv_heads) *
                           static_cast<uint64_t>(c.page_size);
-    if (rows >= (1ull << 31))
+    if (!kv8 && rows >= (1ull << 31))
       nbl::fail(NBL_E_INVALID, "kv_create: pool of " + std::to_string(c.n_pages) +
                                    " pages exceeds 2^31 rows (tensor-map coordinate range)");
     use_device(ctx);
     auto* kv = new nbl_kv();
     kv->ctx = ctx;
     kv->cfg = c;
-    kv->bytes = rows * static_cast<uint64_t>(c.head_dim) * 2u;
+    kv->bytes = kv8 ? static_cast<uint64_t>(c.n_pages) * static_cast<uint64_t>(nbl::kv8::page_bytes(c.head_dim, c.n_kv_heads))
+                    : rows * static_cast<uint64_t>(c.head_dim) * 2u;
     try {
       kv->pool = device_alloc(kv->bytes, "kv pool");
       nbl::check_cuda(cudaMemsetAsync(kv->pool, 0, kv->bytes, ctx->stream), "kv pool zero-fill");
+      if (kv8) {  // read with bulk copies: no tensor map
+        if (c.dtype == NBL_I8) {  // code 0 is the byte 128; the scales behind a page's blocks stay 0
+          const size_t page = static_cast<size_t>(nbl::kv8::page_bytes(c.head_dim, c.n_kv_heads));
+          const size_t codes = static_cast<size_t>(c.n_kv_heads) * nbl::kv8::block_bytes(c.head_dim);
+          nbl::check_cuda(cudaMemset2DAsync(kv->pool, page, 0x80, codes, static_cast<size_t>(c.n_pages), ctx->stream),
+                          "kv pool zero-fill");
+        }
+        nbl::check_cuda(cudaStreamSynchronize(ctx->stream), "kv pool zero-fill");
+        ctx->kvs.push_back(kv);
+        *out = kv;
+        return;
+      }
       const cuuint64_t dims[2] = {static_cast<cuuint64_t>(c.head_dim), rows};
       const cuuint64_t strides[1] = {static_cast<cuuint64_t>(c.head_dim) * 2u};
       const cuuint32_t box[2] = {static_cast<cuuint32_t>(c.head_dim), static_cast<cuuint32_t>(c.page_size)};
@@ -623,6 +705,7 @@ int nbl_rope_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const void* k
             "rope_kv_append: NULL argument");
     nbl::route_flush_queries(ctx);
     require(kv->ctx == ctx, "rope_kv_append: pool belongs to another context");
+    require(!nbl::is_kv8(kv->cfg.dtype), "rope_kv_append: an 8-bit pool takes nbl_rotary_kv_append");
     require(is_dtype(in_dtype) && is_dtype(q_out_dtype), "rope_kv_append: bad dtype");
     require(n_tok >= 0 && n_tok <= INT32_MAX && pt_stride > 0, "rope_kv_append: n_tok or pt_stride out of range");
     require(n_heads > 0 && n_heads % kv->cfg.n_kv_heads == 0, "rope_kv_append: n_heads must be a multiple of n_kv_heads");
@@ -643,7 +726,11 @@ int nbl_attn_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_
     require(ctx && kv && q && page_table && seq_lens && out, "attn_decode: NULL argument");
     nbl::route_flush_queries(ctx);
     require(kv->ctx == ctx, "attn_decode: pool belongs to another context");
-    require(kv->cfg.dtype == NBL_F16, "attn_decode: the decode kernel reads an NBL_F16 pool");
+    if (nbl::is_kv8(kv->cfg.dtype)) {
+      kv8_decode(ctx, kv, q, page_table, pt_stride, seq_lens, max_seq_len, n_rows, n_heads, out, lse, n_splits);
+      return;
+    }
+    require(kv->cfg.dtype == NBL_F16, "attn_decode: the decode kernel reads an NBL_F16, NBL_I8 or NBL_E4M3 pool");
     require(n_rows >= 0 && pt_stride > 0 && max_seq_len >= 0 && n_splits >= 0, "attn_decode: negative size");
     require(n_heads > 0 && n_heads % kv->cfg.n_kv_heads == 0 && n_heads / kv->cfg.n_kv_heads <= 8,
             "attn_decode: n_heads must be a multiple of n_kv_heads with at most 8 query heads per KV head");
@@ -776,6 +863,11 @@ int nbl_attn_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dt
     require(ctx && kv && q && q_start && q_len && kv_pos0 && page_table && out, "attn_prefill: NULL argument");
     nbl::route_flush_queries(ctx);
     require(kv->ctx == ctx, "attn_prefill: pool belongs to another context");
+    if (nbl::is_kv8(kv->cfg.dtype)) {
+      kv8_prefill(ctx, kv, q, q_dtype, n_q_rows, q_start, q_len, kv_pos0, page_table, pt_stride, n_items, n_heads,
+                  max_q_len, out, out_dtype);
+      return;
+    }
     require(q_dtype == kv->cfg.dtype, "attn_prefill: q must have the pool's dtype");
     require(out_dtype == NBL_F32 || out_dtype == kv->cfg.dtype, "attn_prefill: out must be F32 or the pool dtype");
     require(n_items >= 0 && pt_stride > 0 && max_q_len >= 0 && n_q_rows >= 0, "attn_prefill: negative size");

@@ -1,0 +1,172 @@
+// The 8-bit paged K/V pool (dtype NBL_I8 or NBL_E4M3): where a code lies, and the conversions of codes.
+//
+// A page holds 16 token positions of every KV head. Each (page, KV head) is one block of 32 * D bytes -- its keys,
+// then its values -- so attention fetches it with one bulk copy, and the scales of a page (one fp32 for the keys and
+// one for the values of each head) follow its blocks as 16 bytes per head:
+//   page = [n_kv_heads][ keys 16 * D | values 16 * D ] [n_kv_heads][ key scale, value scale, 0, 0 ]  (rounded to 128)
+// A key element is code * key scale, a value element code * value scale.
+//
+// The codes lie in the order in which the m16n8k16 tensor-core instruction wants them, so a lane (g = lane / 4,
+// t = lane % 4) of a warp fetches its operands with 16-byte loads that meet no bank twice:
+//   keys    [D / 64][16 tokens][64 dims]: lane (g, t) reads the 16 dims 16t.. of token g (and of g + 8). The order of
+//           the dims inside the contraction is free as long as the query has the same one.
+//   values  [D / 32][32 lanes][4 tiles j][4 tokens i]: lane (g, t) holds dim 8j + g of tokens 2t, 2t+1, 2t+8, 2t+9.
+// NBL_I8 codes are stored with 128 added (an unsigned byte), which makes the widening to fp16 a byte permute and a
+// subtraction; NBL_E4M3 codes are stored as they are. Every code and scale in a pool is finite: the append saturates
+// and the import refuses, so a masked token's weight of 0 always gives 0.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "nbl_device.cuh"
+#include "nbl_internal.h"
+
+namespace nbl {
+namespace kv8 {
+
+constexpr int kPage = 16;
+
+__host__ __device__ constexpr int block_bytes(int d) { return 2 * kPage * d; }
+__host__ __device__ inline int64_t page_bytes(int d, int n_kv_heads) {
+  return (int64_t(n_kv_heads) * (block_bytes(d) + 16) + 127) / 128 * 128;
+}
+// Offset of a head's scales (two floats) inside its page.
+__host__ __device__ inline int64_t scale_off(int d, int n_kv_heads, int h) {
+  return int64_t(n_kv_heads) * block_bytes(d) + h * 16;
+}
+// Offset of a code inside its (page, head) block.
+__device__ __forceinline__ int key_off(int tok, int dim) { return (dim >> 6) * 1024 + tok * 64 + (dim & 63); }
+__device__ __forceinline__ int value_off(int d, int tok, int dim) {
+  const int lane = (dim & 7) * 4 + ((tok & 7) >> 1);
+  return kPage * d + (dim >> 5) * 512 + lane * 16 + ((dim >> 3) & 3) * 4 + (tok & 1) + 2 * (tok >> 3);
+}
+
+// KIND: NBL_I8 or NBL_E4M3.
+template <int KIND>
+__host__ __device__ constexpr float code_max() {
+  return KIND == NBL_I8 ? 127.0f : 448.0f;
+}
+// Magnitudes below this are stored as 0 with scale 0: the reciprocal of a smaller scale would not be finite.
+constexpr float kTiny = 1e-30f;
+// Non-finite inputs are stored as 0 (NaN) or saturated at this (and flagged): its scale and products stay finite.
+constexpr float kHuge = 3e38f;
+
+// The stored byte of a value already divided by its scale. The scale makes |x| <= code_max up to rounding; the clamp
+// covers that rounding.
+template <int KIND>
+__device__ __forceinline__ uint32_t encode(float x) {
+  if constexpr (KIND == NBL_I8) {
+    return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.f), 127.f)) + 128);
+  } else {
+    return static_cast<uint32_t>(__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3));
+  }
+}
+template <int KIND>
+__device__ __forceinline__ float decode(uint32_t byte) {
+  if constexpr (KIND == NBL_I8) {
+    return static_cast<float>(static_cast<int>(byte & 0xffu) - 128);
+  } else {
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte & 0xffu), __NV_E4M3);
+    return __half2float(__half(h));
+  }
+}
+// Four codes to two fp16 pairs: (byte 0, byte 1) and (byte 2, byte 3). Exact for both kinds. For I8 the byte becomes
+// the low mantissa bits of 1024 (0x6400 | byte = 1024 + byte), from which 1024 + 128 is subtracted.
+template <int KIND>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (KIND == NBL_I8) {
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
+    const __half2_raw y = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
+    lo = static_cast<uint32_t>(x.x) | (static_cast<uint32_t>(x.y) << 16);
+    hi = static_cast<uint32_t>(y.x) | (static_cast<uint32_t>(y.y) << 16);
+  }
+}
+
+// Bulk copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) into shared memory, completing on `bar`.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(smem_dst)),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+// The same with an L2 eviction-priority hint.
+__device__ __forceinline__ void bulk_load_hint(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar,
+                                               uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
+// An element of a float type as fp32, and back (one rounding).
+__device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
+  if (dtype == NBL_F32) return static_cast<const float*>(p)[i];
+  if (dtype == NBL_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_as(void* p, int64_t i, float v, int dtype) {
+  if (dtype == NBL_F32) static_cast<float*>(p)[i] = v;
+  else if (dtype == NBL_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+}  // namespace kv8
+
+inline bool is_kv8(int dtype) { return dtype == NBL_I8 || dtype == NBL_E4M3; }
+
+// Launches (kv8_append.cu, kv8_attn.cu); all asynchronous on `st`.
+// A sequence's stretch of tokens: item i has rows start[i] .. start[i] + len[i] of the packed activations, at
+// positions pos0[i].. of page-table row i.
+struct Kv8Items {
+  const int32_t* start = nullptr;
+  const int32_t* len = nullptr;
+  const int32_t* pos0 = nullptr;
+  const int32_t* page_table = nullptr;
+  int32_t pt_stride = 0;
+  int n_items = 0, max_len = 0;
+  int64_t n_rows = 0;  // rows of the packed activations
+};
+struct Kv8Append {
+  const void *q_in = nullptr, *k_in = nullptr, *v_in = nullptr;
+  const float *bq = nullptr, *bk = nullptr, *bv = nullptr;
+  void* q_out = nullptr;
+  int in_dtype = 0, q_out_dtype = 0, n_heads = 0;
+  bool neox = false;
+  int rotary_dim = 0;
+  const float2* tab = nullptr;  // (cos, sin) [tab_pos][rotary_dim / 2]
+  int64_t tab_pos = 0;
+};
+void launch_kv8_append(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, const Kv8Append& a, int* err);
+void launch_kv8_read(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, void* k_out, void* v_out, int out_dtype,
+                     int* err);
+void launch_kv8_import(cudaStream_t st, const nbl_kv* kv, const int32_t* page_ids, int64_t n, const void* codes,
+                       const float* scales, int* err);
+void launch_kv8_export(cudaStream_t st, const nbl_kv* kv, const int32_t* page_ids, int64_t n, void* codes,
+                       float* scales, int* err);
+// tab[pos][i] = (cos, sin)(pos * freq[i]) * mul in double, rounded to float; freq: n_pairs doubles on the device.
+void launch_rotary_table(cudaStream_t st, float2* tab, int64_t n_pos, const double* freq, int n_pairs, double mul);
+
+struct Kv8AttnPlan {
+  int n_splits = 1;
+  int min_pages = 8;  // fewest pages of a split
+  int tiles = 1;  // row tiles of one (item, KV head)
+  size_t scratch_bytes = 0;
+  int64_t units = 0;  // (item, KV head, tile) triples, one arrival counter each when split
+};
+// n_rows: rows of q (tokens); max_kv: longest key range. q_dtype decides the row tile (8 rows of fp32 queries, whose
+// two fp16 terms fill the 16 rows of the instruction, or 16 rows of 16-bit queries).
+Kv8AttnPlan plan_kv8_attn(const nbl_kv* kv, int n_items, int max_len, int64_t n_rows, int n_heads, int max_kv,
+                          int q_dtype, int num_sms, int requested_splits);
+// items.len == NULL: one query row per item at position pos0[i] - 1 (pos0 = sequence lengths, 0 = no keys).
+void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, const void* q, int q_dtype, int n_heads,
+                     void* out, int out_dtype, float* lse, const Kv8AttnPlan& plan, void* scratch, unsigned* counts,
+                     int* err);
+
+}  // namespace nbl

@@ -36,6 +36,16 @@ struct RopeTable {
   float2* dev = nullptr;
 };
 
+// Cached cos/sin table of one nbl_rotary_params with n rotated elements: tab[pos * n / 2 + i] = (cos, sin)(pos *
+// freq[i]) * mul, freq and mul being what the scaling makes of the base; evaluated in double.
+struct RotaryTable {
+  nbl_rotary_params params{};   // freq_factors NULL
+  std::vector<float> factors;   // empty when none
+  int n = 0;
+  int64_t n_pos = 0;
+  float2* dev = nullptr;
+};
+
 }  // namespace nbl
 
 struct nbl_ctx {
@@ -56,6 +66,7 @@ struct nbl_ctx {
   int64_t split_counts_n = 0;
   int64_t reserved_ctx = 0, reserved_heads = 0;
   std::vector<nbl::RopeTable> rope_tables;
+  std::vector<nbl::RotaryTable> rotary_tables;
   std::vector<nbl_kv*> kvs;
   // nbl_decode_step_host: staging for the step's inputs/outputs and the two copy streams with their events
   void* io = nullptr;
