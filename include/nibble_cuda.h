@@ -255,9 +255,9 @@ NBL_API int nbl_rope_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const
  * the kernel also checks each length against pt_stride * page_size). n_splits: KV splits per row (0 = chosen
  * from the sizes); more than one uses context scratch sized by nbl_reserve (grown on demand otherwise).
  * head_dim 64, n_heads / n_kv_heads <= 8.
- * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes any group size; the split count is then an upper bound, each
- * row's own pages being divided evenly, and its results are the softmax over the values that the codes stand for, to
- * fp32 accuracy. */
+ * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes any group size; n_splits is then not used, the pages of all
+ * rows being divided evenly over the GPU whatever their lengths. The results are the softmax over the values that the
+ * codes stand for, to fp32 accuracy. */
 NBL_API int nbl_attn_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_t* page_table, int32_t pt_stride,
                     const int32_t* seq_lens, int32_t max_seq_len, int32_t n_rows, int32_t n_heads, float* out,
                     float* lse, int32_t n_splits);

@@ -290,19 +290,14 @@ void qblock_matmul(nbl_ctx* ctx, const nbl_weight* w, float* y, const float* x, 
   nbl::launch_qblock_matmul(ctx->stream, w->w, y, x, n, ctx->qblock_act, ctx->num_sms);
 }
 
-// Attention over an 8-bit pool: plans the splits, grows the scratch and launches.
+// Attention over an 8-bit pool: plans the grid, grows the scratch and launches.
 void kv8_attention(nbl_ctx* ctx, const nbl_kv* kv, const nbl::Kv8Items& it, const void* q, int q_dtype, int n_heads,
-                   void* out, int out_dtype, float* lse, int max_kv, int n_splits) {
+                   void* out, int out_dtype, float* lse, int max_kv) {
   use_device(ctx);
-  const auto plan = nbl::plan_kv8_attn(kv, it.n_items, it.max_len, it.n_rows, n_heads, max_kv, q_dtype, ctx->num_sms,
-                                       n_splits);
-  unsigned* counts = nullptr;
-  if (plan.n_splits > 1) {
-    ensure_scratch(ctx, plan.scratch_bytes);
-    counts = nbl::split_counts(ctx, plan.units);
-  }
-  nbl::launch_kv8_attn(ctx->stream, kv, it, q, q_dtype, n_heads, out, out_dtype, lse, plan, ctx->scratch, counts,
-                       ctx->d_err);
+  const auto plan = nbl::plan_kv8_attn(kv, it.n_items, it.max_len, n_heads, max_kv, q_dtype, ctx->num_sms);
+  ensure_scratch(ctx, plan.scratch_bytes);
+  nbl::launch_kv8_attn(ctx->stream, kv, it, q, q_dtype, n_heads, out, out_dtype, lse, plan, ctx->scratch,
+                       nbl::split_counts(ctx, plan.grid), ctx->d_err);
 }
 
 // nbl_attn_decode on an 8-bit pool (pointers and context checked).
@@ -321,7 +316,7 @@ void kv8_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_t* p
   it.n_items = n_rows;
   it.max_len = 1;
   it.n_rows = n_rows;
-  kv8_attention(ctx, kv, it, q, NBL_F32, n_heads, out, NBL_F32, lse, max_seq_len, n_splits);
+  kv8_attention(ctx, kv, it, q, NBL_F32, n_heads, out, NBL_F32, lse, max_seq_len);
 }
 
 // nbl_attn_prefill on an 8-bit pool (pointers and context checked).
@@ -343,7 +338,7 @@ void kv8_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype,
   it.n_items = n_items;
   it.max_len = max_q_len;
   it.n_rows = n_q_rows;
-  kv8_attention(ctx, kv, it, q, q_dtype, n_heads, out, out_dtype, nullptr, pt_stride * kv->cfg.page_size, 0);
+  kv8_attention(ctx, kv, it, q, q_dtype, n_heads, out, out_dtype, nullptr, pt_stride * kv->cfg.page_size);
 }
 
 void require_weight(const nbl_ctx* ctx, const nbl_weight* w, const char* what) {

@@ -11,9 +11,16 @@
 //   keys    [D / 64][16 tokens][64 dims]: lane (g, t) reads the 16 dims 16t.. of token g (and of g + 8). The order of
 //           the dims inside the contraction is free as long as the query has the same one.
 //   values  [D / 32][32 lanes][4 tiles j][4 tokens i]: lane (g, t) holds dim 8j + g of tokens 2t, 2t+1, 2t+8, 2t+9.
-// NBL_I8 codes are stored with 128 added (an unsigned byte), which makes the widening to fp16 a byte permute and a
-// subtraction; NBL_E4M3 codes are stored as they are. Every code and scale in a pool is finite: the append saturates
-// and the import refuses, so a masked token's weight of 0 always gives 0.
+// A word is four codes (four dims of a token, or four tokens of a dim), stored so that they widen to two fp16 pairs with
+// few instructions:
+//   NBL_I8    byte i = code i + 128: the widening is a byte permute and a subtraction.
+//   NBL_E4M3  an fp16 whose sign is a code's and whose next bits are 0, eeee, mmm, 0... is the code times 2^-8 (also for
+//             the subnormal codes), so codes 0 and 1 stand at those bits of the word's two halves, and codes 2 and 3 at the
+//             bits between (sign at bit 14, the rest at 6..0): one mask gives the first pair, two shifts and two
+//             masks the second. (The conversion instruction runs at a quarter of that rate: decode of 256 rows of 4097
+//             tokens took 262 us with it, as against 207 us for NBL_I8.)
+// Every code and scale in a pool is finite: the append saturates and the import refuses, so a masked token's weight
+// of 0 always gives 0.
 #pragma once
 #include <cuda_fp8.h>
 
@@ -34,11 +41,15 @@ __host__ __device__ inline int64_t scale_off(int d, int n_kv_heads, int h) {
   return int64_t(n_kv_heads) * block_bytes(d) + h * 16;
 }
 // Offset of a code inside its (page, head) block.
+// Offset of the word with a token's dims dim .. dim + 3 (dim a multiple of 4).
 __device__ __forceinline__ int key_off(int tok, int dim) { return (dim >> 6) * 1024 + tok * 64 + (dim & 63); }
-__device__ __forceinline__ int value_off(int d, int tok, int dim) {
-  const int lane = (dim & 7) * 4 + ((tok & 7) >> 1);
-  return kPage * d + (dim >> 5) * 512 + lane * 16 + ((dim >> 3) & 3) * 4 + (tok & 1) + 2 * (tok >> 3);
+// Offset of the word with a dim's tokens 2t, 2t + 1, 2t + 8, 2t + 9.
+__device__ __forceinline__ int value_off(int d, int t, int dim) {
+  return kPage * d + (dim >> 5) * 512 + ((dim & 7) * 4 + t) * 16 + ((dim >> 3) & 3) * 4;
 }
+// Where a token's code stands: t of its word, and its place there.
+__device__ __forceinline__ int value_t(int tok) { return (tok & 7) >> 1; }
+__device__ __forceinline__ int value_i(int tok) { return (tok & 1) + 2 * (tok >> 3); }
 
 // KIND: NBL_I8 or NBL_E4M3.
 template <int KIND>
@@ -50,27 +61,45 @@ constexpr float kTiny = 1e-30f;
 // Non-finite inputs are stored as 0 (NaN) or saturated at this (and flagged): its scale and products stay finite.
 constexpr float kHuge = 3e38f;
 
-// The stored byte of a value already divided by its scale. The scale makes |x| <= code_max up to rounding; the clamp
-// covers that rounding.
+// The code (as a byte: int8 or e4m3) of a value already divided by its scale. The scale makes |x| <= code_max up to
+// rounding; the clamp covers that rounding.
 template <int KIND>
 __device__ __forceinline__ uint32_t encode(float x) {
   if constexpr (KIND == NBL_I8) {
-    return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.f), 127.f)) + 128);
+    return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.f), 127.f))) & 0xffu;
   } else {
     return static_cast<uint32_t>(__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3));
   }
 }
 template <int KIND>
-__device__ __forceinline__ float decode(uint32_t byte) {
+__device__ __forceinline__ float decode(uint32_t code) {
   if constexpr (KIND == NBL_I8) {
-    return static_cast<float>(static_cast<int>(byte & 0xffu) - 128);
+    return static_cast<float>(static_cast<int8_t>(code & 0xffu));
   } else {
-    const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte & 0xffu), __NV_E4M3);
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code & 0xffu), __NV_E4M3);
     return __half2float(__half(h));
   }
 }
-// Four codes to two fp16 pairs: (byte 0, byte 1) and (byte 2, byte 3). Exact for both kinds. For I8 the byte becomes
-// the low mantissa bits of 1024 (0x6400 | byte = 1024 + byte), from which 1024 + 128 is subtracted.
+// Four codes (byte i of `codes`) as the word that is stored, and back.
+template <int KIND>
+__host__ __device__ __forceinline__ uint32_t to_word(uint32_t codes) {
+  if constexpr (KIND == NBL_I8) return codes ^ 0x80808080u;
+  const uint32_t a = (codes & 0xffu) | ((codes & 0xff00u) << 8), b = ((codes >> 16) & 0xffu) | ((codes >> 8) & 0xff0000u);
+  return ((a & 0x00800080u) << 8) | ((a & 0x007f007fu) << 7) | ((b & 0x00800080u) << 7) | (b & 0x007f007fu);
+}
+template <int KIND>
+__host__ __device__ __forceinline__ uint32_t from_word(uint32_t w) {
+  if constexpr (KIND == NBL_I8) return w ^ 0x80808080u;
+  const uint32_t a = ((w >> 8) & 0x00800080u) | ((w >> 7) & 0x007f007fu);
+  const uint32_t b = ((w >> 7) & 0x00800080u) | (w & 0x007f007fu);
+  return (a & 0xffu) | ((a >> 8) & 0xff00u) | ((b & 0xffu) << 16) | ((b & 0xff0000u) << 8);
+}
+// A word as two fp16 pairs (codes 0, 1 and 2, 3), each the code divided by unit<KIND>(). Exact for both kinds. For I8 the
+// byte becomes the low mantissa bits of 1024 (0x6400 | byte = 1024 + byte), from which 1024 + 128 is subtracted.
+template <int KIND>
+__host__ __device__ constexpr float unit() {
+  return KIND == NBL_I8 ? 1.f : 256.f;
+}
 template <int KIND>
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (KIND == NBL_I8) {
@@ -81,10 +110,8 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
     lo = *reinterpret_cast<const uint32_t*>(&x);
     hi = *reinterpret_cast<const uint32_t*>(&y);
   } else {
-    const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3);
-    const __half2_raw y = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
-    lo = static_cast<uint32_t>(x.x) | (static_cast<uint32_t>(x.y) << 16);
-    hi = static_cast<uint32_t>(y.x) | (static_cast<uint32_t>(y.y) << 16);
+    lo = w & 0xbf80bf80u;
+    hi = ((w << 7) & 0x3f803f80u) | ((w << 1) & 0x80008000u);
   }
 }
 
@@ -154,16 +181,13 @@ void launch_kv8_export(cudaStream_t st, const nbl_kv* kv, const int32_t* page_id
 void launch_rotary_table(cudaStream_t st, float2* tab, int64_t n_pos, const double* freq, int n_pairs, double mul);
 
 struct Kv8AttnPlan {
-  int n_splits = 1;
-  int min_pages = 8;  // fewest pages of a split
-  int tiles = 1;  // row tiles of one (item, KV head)
-  size_t scratch_bytes = 0;
-  int64_t units = 0;  // (item, KV head, tile) triples, one arrival counter each when split
+  int grid = 1;              // CTAs, and arrival counters
+  size_t scratch_bytes = 0;  // parts of units that span CTAs
 };
-// n_rows: rows of q (tokens); max_kv: longest key range. q_dtype decides the row tile (8 rows of fp32 queries, whose
-// two fp16 terms fill the 16 rows of the instruction, or 16 rows of 16-bit queries).
-Kv8AttnPlan plan_kv8_attn(const nbl_kv* kv, int n_items, int max_len, int64_t n_rows, int n_heads, int max_kv,
-                          int q_dtype, int num_sms, int requested_splits);
+// max_kv: longest key range. q_dtype decides the row tile (8 rows of fp32 queries, whose two fp16 terms fill the 16 rows
+// of the instruction, or 16 rows of 16-bit queries).
+Kv8AttnPlan plan_kv8_attn(const nbl_kv* kv, int n_items, int max_len, int n_heads, int max_kv, int q_dtype,
+                          int num_sms);
 // items.len == NULL: one query row per item at position pos0[i] - 1 (pos0 = sequence lengths, 0 = no keys).
 void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, const void* q, int q_dtype, int n_heads,
                      void* out, int out_dtype, float* lse, const Kv8AttnPlan& plan, void* scratch, unsigned* counts,

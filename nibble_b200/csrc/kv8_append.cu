@@ -3,7 +3,7 @@
 //
 // Quantization. A block is the 16 places of one (page, KV head), keys and values apart. With amax the largest
 // magnitude among the tokens that a call adds to the block and s_old the scale of the tokens that were there,
-//   s = max(s_old, amax / code_max),   new code = round(x / s),   old code = round(code * s_old / s),
+//   s = max(s_old, amax * (1 / code_max)),   new code = round(x / s),   old code = round(code * s_old / s),
 // so a block's scale only grows while it fills, and each growth adds at most half a step to an old token's error. The
 // places after the last token are set to 0. Products use the fp32 reciprocal of s; all of it is IEEE fp32, each step
 // rounded once, so the codes do not depend on how the work is spread over threads.
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const Kv8Items it,
 #pragma unroll
     for (int i = 0; i < kThreads / 32; ++i) m = fmaxf(m, red[w][i]);
     const float old = s[w];
-    s[w] = fmaxf(old, m >= kTiny ? __fdiv_rn(m, code_max<KIND>()) : 0.f);
+    s[w] = fmaxf(old, m >= kTiny ? __fmul_rn(m, 1.f / code_max<KIND>()) : 0.f);
     inv[w] = s[w] > 0.f ? __fdiv_rn(1.f, s[w]) : 0.f;
     ratio[w] = __fmul_rn(old, inv[w]);
   }
@@ -118,24 +118,20 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const Kv8Items it,
   for (int u = threadIdx.x; u < kPage * D / 16; u += kThreads) {
     const int tok = u / (D / 16), d0 = (u % (D / 16)) * 16;
     uint4* dst = reinterpret_cast<uint4*>(blk + key_off(tok, d0));
+    const uint4 was = tok < slot0 ? *dst : uint4{};
+    const uint32_t o[4] = {was.x, was.y, was.z, was.w};
     uint32_t w4[4];
-    if (tok < slot0) {
-      const uint4 was = *dst;
-      const uint32_t o[4] = {was.x, was.y, was.z, was.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        w4[k] = 0;
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t old = from_word<KIND>(o[k]);
+      w4[k] = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) w4[k] |= encode<KIND>(__fmul_rn(decode<KIND>(o[k] >> (8 * b)), ratio[0])) << (8 * b);
+      for (int b = 0; b < 4; ++b) {
+        const float x = tok < slot0 ? __fmul_rn(decode<KIND>(old >> (8 * b)), ratio[0])
+                                    : (tok < slot1 ? __fmul_rn(xs[0][tok][d0 + 4 * k + b], inv[0]) : 0.f);
+        w4[k] |= encode<KIND>(x) << (8 * b);
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        w4[k] = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-          w4[k] |= encode<KIND>(tok < slot1 ? __fmul_rn(xs[0][tok][d0 + 4 * k + b], inv[0]) : 0.f) << (8 * b);
-      }
+      w4[k] = to_word<KIND>(w4[k]);
     }
     *dst = make_uint4(w4[0], w4[1], w4[2], w4[3]);
   }
@@ -148,14 +144,16 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const Kv8Items it,
     uint32_t w4[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      const uint32_t old = from_word<KIND>(o[j]);
       w4[j] = 0;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int tok = 2 * t + (b & 1) + 8 * (b >> 1), dim = 32 * c + 8 * j + g;
-        const float x = tok < slot0 ? __fmul_rn(decode<KIND>(o[j] >> (8 * b)), ratio[1])
+        const float x = tok < slot0 ? __fmul_rn(decode<KIND>(old >> (8 * b)), ratio[1])
                                     : (tok < slot1 ? __fmul_rn(xs[1][tok][dim], inv[1]) : 0.f);
         w4[j] |= encode<KIND>(x) << (8 * b);
       }
+      w4[j] = to_word<KIND>(w4[j]);
     }
     *dst = make_uint4(w4[0], w4[1], w4[2], w4[3]);
   }
@@ -192,8 +190,14 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const Kv8Items it, c
   for (int u = threadIdx.x; u < n * D; u += kThreads) {
     const int i = u / D, dim = u % D, tok = slot0 + i;
     const int64_t at = (int64_t(start) + (first - pos0) + i) * n_kv_heads * D + int64_t(kvh) * D + dim;
-    if (k_out) store_as(k_out, at, __fmul_rn(decode<KIND>(blk[key_off(tok, dim)]), ks), out_dtype);
-    if (v_out) store_as(v_out, at, __fmul_rn(decode<KIND>(blk[value_off(D, tok, dim)]), vs), out_dtype);
+    if (k_out) {
+      const uint32_t w = from_word<KIND>(*reinterpret_cast<const uint32_t*>(blk + key_off(tok, dim & ~3)));
+      store_as(k_out, at, __fmul_rn(decode<KIND>(w >> (8 * (dim & 3))), ks), out_dtype);
+    }
+    if (v_out) {
+      const uint32_t w = from_word<KIND>(*reinterpret_cast<const uint32_t*>(blk + value_off(D, value_t(tok), dim)));
+      store_as(v_out, at, __fmul_rn(decode<KIND>(w >> (8 * value_i(tok))), vs), out_dtype);
+    }
   }
 }
 
@@ -214,20 +218,36 @@ __global__ void __launch_bounds__(kThreads) kv8_pages_kernel(uint8_t* pool, int6
   float* sc = reinterpret_cast<float*>(pg + scale_off(D, n_kv_heads, kvh));
   for (int w = 0; w < 2; ++w) {
     uint8_t* src = codes + ((i * 2 + w) * n_kv_heads + kvh) * (kPage * D);
-    for (int u = threadIdx.x; u < kPage * D; u += kThreads) {
-      const int tok = u / D, dim = u % D;
-      uint8_t* at = blk + (w ? value_off(D, tok, dim) : key_off(tok, dim));
-      if constexpr (IMPORT) {
-        uint8_t b = src[u];
-        if constexpr (KIND == NBL_I8) {
-          b = static_cast<uint8_t>(b + 128);
-        } else if ((b & 0x7f) == 0x7f) {  // e4m3's NaN
-          flag_error(err, kErrNonFinite);
-          b = 0;
-        }
-        *at = b;
+    for (int u = threadIdx.x; u < kPage * D / 4; u += kThreads) {  // words
+      int at, tok[4], dim[4];
+      if (w == 0) {
+        const int d0 = (u % (D / 4)) * 4;
+        at = key_off(u / (D / 4), d0);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) tok[b] = u / (D / 4), dim[b] = d0 + b;
       } else {
-        src[u] = KIND == NBL_I8 ? static_cast<uint8_t>(*at - 128) : *at;
+        const int t = u / D;
+        at = value_off(D, t, u % D);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) tok[b] = 2 * t + (b & 1) + 8 * (b >> 1), dim[b] = u % D;
+      }
+      uint32_t* word = reinterpret_cast<uint32_t*>(blk + at);
+      if constexpr (IMPORT) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t x = src[tok[b] * D + dim[b]];
+          if (KIND == NBL_E4M3 && (x & 0x7f) == 0x7f) {  // e4m3's NaN
+            flag_error(err, kErrNonFinite);
+            x = 0;
+          }
+          c |= x << (8 * b);
+        }
+        *word = to_word<KIND>(c);
+      } else {
+        const uint32_t c = from_word<KIND>(*word);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) src[tok[b] * D + dim[b]] = static_cast<uint8_t>(c >> (8 * b));
       }
     }
     if (threadIdx.x == 0) {

@@ -156,7 +156,7 @@ class PlainCache:
             for w, x in enumerate((k, v)):
                 new = x[lo - pos0:hi - pos0].transpose(1, 0, 2)  # [KV, tokens, D]
                 amax = np.abs(new).max((1, 2)).astype(np.float32)
-                want = np.where(amax >= np.float32(1e-30), amax / np.float32(QMAX[self.kind]), 0).astype(np.float32)
+                want = np.where(amax >= np.float32(1e-30), amax * (np.float32(1) / np.float32(QMAX[self.kind])), 0).astype(np.float32)
                 old = self.scales[page, w] if s0 else np.zeros_like(want)
                 s = np.maximum(old, want)
                 inv = np.divide(one, s, out=np.zeros_like(s), where=s > 0)
