@@ -642,12 +642,7 @@ int nbl_kv_create(nbl_ctx* ctx, const nbl_kv_config* cfg, nbl_kv** out) {
       kv->pool = device_alloc(kv->bytes, "kv pool");
       nbl::check_cuda(cudaMemsetAsync(kv->pool, 0, kv->bytes, ctx->stream), "kv pool zero-fill");
       if (kv8) {  // read with bulk copies: no tensor map
-        if (c.dtype == NBL_I8) {  // code 0 is the byte 128; the scales behind a page's blocks stay 0
-          const size_t page = static_cast<size_t>(nbl::kv8::page_bytes(c.head_dim, c.n_kv_heads));
-          const size_t codes = static_cast<size_t>(c.n_kv_heads) * nbl::kv8::block_bytes(c.head_dim);
-          nbl::check_cuda(cudaMemset2DAsync(kv->pool, page, 0x80, codes, static_cast<size_t>(c.n_pages), ctx->stream),
-                          "kv pool zero-fill");
-        }
+        nbl::launch_kv8_clear(ctx->stream, kv);
         nbl::check_cuda(cudaStreamSynchronize(ctx->stream), "kv pool zero-fill");
         ctx->kvs.push_back(kv);
         *out = kv;

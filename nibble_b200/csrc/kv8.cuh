@@ -1,9 +1,8 @@
 // The 8-bit paged K/V pool (dtype NBL_I8 or NBL_E4M3): where a code lies, and the conversions of codes.
 //
-// A page holds 16 token positions of every KV head. Each (page, KV head) is one block of 32 * D bytes -- its keys,
-// then its values -- so attention fetches it with one bulk copy, and the scales of a page (one fp32 for the keys and
-// one for the values of each head) follow its blocks as 16 bytes per head:
-//   page = [n_kv_heads][ keys 16 * D | values 16 * D ] [n_kv_heads][ key scale, value scale, 0, 0 ]  (rounded to 128)
+// A page holds 16 token positions of every KV head. Each (page, KV head) is one block of 32 * D + 16 bytes -- its keys,
+// its values, then their two scales -- so attention fetches it with one bulk copy:
+//   page = [n_kv_heads][ keys 16 * D | values 16 * D | key scale, value scale, 0, 0 (fp32) ]  (rounded to 128)
 // A key element is code * key scale, a value element code * value scale.
 //
 // The codes lie in the order in which the m16n8k16 tensor-core instruction wants them, so a lane (g = lane / 4,
@@ -32,15 +31,12 @@ namespace kv8 {
 
 constexpr int kPage = 16;
 
-__host__ __device__ constexpr int block_bytes(int d) { return 2 * kPage * d; }
+__host__ __device__ constexpr int block_bytes(int d) { return 2 * kPage * d + 16; }
 __host__ __device__ inline int64_t page_bytes(int d, int n_kv_heads) {
-  return (int64_t(n_kv_heads) * (block_bytes(d) + 16) + 127) / 128 * 128;
+  return (int64_t(n_kv_heads) * block_bytes(d) + 127) / 128 * 128;
 }
-// Offset of a head's scales (two floats) inside its page.
-__host__ __device__ inline int64_t scale_off(int d, int n_kv_heads, int h) {
-  return int64_t(n_kv_heads) * block_bytes(d) + h * 16;
-}
-// Offset of a code inside its (page, head) block.
+// Offset of the two scales inside their block.
+__host__ __device__ constexpr int scale_off(int d) { return 2 * kPage * d; }
 // Offset of the word with a token's dims dim .. dim + 3 (dim a multiple of 4).
 __device__ __forceinline__ int key_off(int tok, int dim) { return (dim >> 6) * 1024 + tok * 64 + (dim & 63); }
 // Offset of the word with a dim's tokens 2t, 2t + 1, 2t + 8, 2t + 9.
@@ -170,6 +166,8 @@ struct Kv8Append {
   const float2* tab = nullptr;  // (cos, sin) [tab_pos][rotary_dim / 2]
   int64_t tab_pos = 0;
 };
+// A new pool's codes and scales: all 0.
+void launch_kv8_clear(cudaStream_t st, const nbl_kv* kv);
 void launch_kv8_append(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, const Kv8Append& a, int* err);
 void launch_kv8_read(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, void* k_out, void* v_out, int out_dtype,
                      int* err);

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const Kv8Items it,
   }
   uint8_t* pg = pool + int64_t(page) * page_bytes(D, n_kv_heads);
   uint8_t* blk = pg + int64_t(kvh) * block_bytes(D);
-  float* sc = reinterpret_cast<float*>(pg + scale_off(D, n_kv_heads, kvh));
+  float* sc = reinterpret_cast<float*>(blk + scale_off(D));
   float s[2], inv[2], ratio[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) s[w] = slot0 > 0 ? sc[w] : 0.f;  // the scale of the tokens already there
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const Kv8Items it, c
   const int slot0 = first - static_cast<int>(block) * kPage;
   const uint8_t* pg = pool + int64_t(page) * page_bytes(D, n_kv_heads);
   const uint8_t* blk = pg + int64_t(kvh) * block_bytes(D);
-  const float* sc = reinterpret_cast<const float*>(pg + scale_off(D, n_kv_heads, kvh));
+  const float* sc = reinterpret_cast<const float*>(blk + scale_off(D));
   const float ks = sc[0], vs = sc[1];
   for (int u = threadIdx.x; u < n * D; u += kThreads) {
     const int i = u / D, dim = u % D, tok = slot0 + i;
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kThreads) kv8_pages_kernel(uint8_t* pool, int6
   }
   uint8_t* pg = pool + int64_t(page) * page_bytes(D, n_kv_heads);
   uint8_t* blk = pg + int64_t(kvh) * block_bytes(D);
-  float* sc = reinterpret_cast<float*>(pg + scale_off(D, n_kv_heads, kvh));
+  float* sc = reinterpret_cast<float*>(blk + scale_off(D));
   for (int w = 0; w < 2; ++w) {
     uint8_t* src = codes + ((i * 2 + w) * n_kv_heads + kvh) * (kPage * D);
     for (int u = threadIdx.x; u < kPage * D / 4; u += kThreads) {  // words
@@ -267,6 +267,14 @@ __global__ void __launch_bounds__(kThreads) kv8_pages_kernel(uint8_t* pool, int6
   }
 }
 
+__global__ void kv8_clear_kernel(uint8_t* pool, int64_t n_pages, int n_kv_heads, int d) {
+  for (int64_t u = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; u < n_pages * n_kv_heads;
+       u += int64_t(gridDim.x) * blockDim.x) {
+    uint8_t* blk = pool + u / n_kv_heads * page_bytes(d, n_kv_heads) + u % n_kv_heads * block_bytes(d);
+    *reinterpret_cast<uint4*>(blk + scale_off(d)) = uint4{};
+  }
+}
+
 __global__ void rotary_table_kernel(float2* __restrict__ tab, int64_t n, const double* __restrict__ freq, int n_pairs,
                                     double mul) {
   for (int64_t u = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; u < n; u += int64_t(gridDim.x) * blockDim.x) {
@@ -297,6 +305,14 @@ void grid_check(int64_t ctas, const char* what) {
 }
 
 }  // namespace
+
+void launch_kv8_clear(cudaStream_t st, const nbl_kv* kv) {
+  // code 0 is the byte 128 for I8, 0 for E4M3
+  check_cuda(cudaMemsetAsync(kv->pool, kv->cfg.dtype == NBL_I8 ? 0x80 : 0, kv->bytes, st), "kv pool zero-fill");
+  kv8_clear_kernel<<<1184, 256, 0, st>>>(static_cast<uint8_t*>(kv->pool), kv->cfg.n_pages, kv->cfg.n_kv_heads,
+                                         kv->cfg.head_dim);
+  check_cuda(cudaGetLastError(), "kv pool zero-fill");
+}
 
 void launch_kv8_append(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, const Kv8Append& a, int* err) {
   const int blocks = touched_pages(items.max_len);

@@ -8,9 +8,9 @@
 // Work. A unit is one (item, KV head, tile of query rows); row r of an (item, KV head) is token r / G, head r % G, and a
 // tile is 8 or 16 rows. The units' pages, end to end, are cut into gridDim.x equal stretches, one per CTA, whatever the
 // rows' lengths (each CTA finds its stretch from the lengths). A CTA walks the segments of its stretch (pages of one
-// unit); its 4 warps take a segment's chunks round-robin, each with a private ring in shared memory that bulk copies
-// keep filled across segments, and a softmax state of its own. At a segment's end the warps merge through shared
-// memory; a unit that spans CTAs leaves partials in scratch, and the last of its CTAs to arrive merges them.
+// unit). Its last warp fills a ring of chunks with bulk copies, running ahead across segments; the others take the
+// chunks round-robin, each with a softmax state of its own, and merge through shared memory at a segment's end. A unit
+// that spans CTAs leaves partials in scratch, and the last of its CTAs to arrive merges them.
 //
 // m16n8k16: S[16 rows x 8 tokens] = Q (A) K^T (B), O[16 rows x 8 dims] = P (A) V (B). The C fragment of S is the A
 // fragment of P, so P never leaves its lane. HILO (fp32 queries): a tile is 8 rows; rows 0-7 of the instruction carry
@@ -31,6 +31,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "kv8.cuh"
 
@@ -39,26 +40,36 @@ namespace {
 
 using namespace kv8;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kPScale = 16384.f;  // 2^14
 
 template <int D, bool HILO>
 struct Cfg {
-  static constexpr int kRows = HILO ? 8 : 16;           // query rows of a tile
-  static constexpr int kPages = D == 64 ? 4 : 2;        // pages of a chunk
-  static constexpr int kStages = D == 64 || !HILO ? 2 : 3;
-  static constexpr int kCtasPerSm = D == 64 && HILO ? 3 : 2;
+  static constexpr int kCtas = D == 64 ? 3 : 2;             // per SM
+  static constexpr int kConsumers = D == 64 ? 4 : 5;        // attending warps; one more issues the loads
+  static constexpr int kThreads = (kConsumers + 1) * 32;
+  static constexpr int kRows = HILO ? 8 : 16;        // query rows of a tile
+  static constexpr int kPages = 2;                   // pages of a chunk (the loads below are written for 2)
   static constexpr int kBlock = block_bytes(D);
-  static constexpr int kStageBytes = kPages * (kBlock + 16);
-  static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kStageBytes = kPages * kBlock;
   static constexpr int kMergeFloats = kRows * (D + 2);  // per warp: outputs, maxima, sums
-  static constexpr int kOffMerge = kRingBytes;
-  static constexpr int kOffBar = kOffMerge + kWarps * kMergeFloats * 4;
-  static constexpr int kSmemBytes = kOffBar + kWarps * kStages * 8;
-  static constexpr int kMinPages = kWarps * kPages;     // fewest pages of a CTA's stretch
-  static constexpr int kSnapPages = 3 * kMinPages;      // units up to this long are not cut
+  static constexpr int kQBytes = (D / 16) * 32 * 16;    // a tile's queries in operand order
+  static constexpr int kRowFloats = 2 * kRows;          // per row: factor and offset of its scores
+  static constexpr int kFixed = kConsumers * kMergeFloats * 4 + kQBytes + kRowFloats * 4;
+  // A whole number of stages for each attending warp: chunk k is warp k % kConsumers's, and so are all the chunks
+  // of its stage, so a warp never waits on a barrier that is two phases behind.
+  static constexpr int kStages = ((227 * 1024 / kCtas - 1152) - kFixed) / (kStageBytes + 32) / kConsumers * kConsumers;
+  static constexpr int kOffMerge = (kStages * kStageBytes + 15) / 16 * 16;
+  static constexpr int kOffQ = kOffMerge + kConsumers * kMergeFloats * 4;
+  static constexpr int kOffRow = kOffQ + kQBytes;
+  static constexpr int kOffBar = kOffRow + kRowFloats * 4;   // full[kStages], empty[kStages]
+  static constexpr int kOffMask = kOffBar + kStages * 16;    // pages of the stage that were loaded
+  static constexpr int kSmemBytes = kOffMask + kStages * 4;
+  static constexpr int kBatch = D == 64 ? 8 : 4;  // pages that the loading warp issues at once
+  // What a segment costs besides its pages, in pages (a CTA attends 4-7 pages a microsecond; a segment's start, merge and
+  // store take 2-4 us). Units up to kSnapPages long are not cut.
+  static constexpr int kSegCost = 16, kSnapPages = 48;
+  static_assert(kOffQ % 16 == 0 && kOffBar % 8 == 0 && kStages >= kConsumers, "layout");
 };
 
 // n / d for 0 <= n < 2^31 by a multiplication (the divisors are a call's constants): with 2^l >= d, the quotient is
@@ -187,14 +198,16 @@ __device__ __forceinline__ Item load_item(const AttnArgs& a, int i) {
   return x;
 }
 
-// Where a stretch stands: unit (item, sub) and the segment [page, page + seg) of it; rem pages after the segment.
+// Where a stretch stands: unit (item, sub), the unit'th of all, and the segment [page, page + seg) of it; rem pages after
+// the segment.
 struct Cursor {
-  int item, sub, page, seg, rem;
+  int item, sub, unit, page, seg, rem;
   Item x;
 };
 template <int ROWS>
 __device__ __forceinline__ void next_segment(const AttnArgs& a, Cursor& c) {
   ++c.sub;
+  ++c.unit;
   c.page = 0;
   if (c.sub >= c.x.subs) {
     c.sub = 0;
@@ -207,62 +220,79 @@ __device__ __forceinline__ void next_segment(const AttnArgs& a, Cursor& c) {
 }
 
 template <int D, int KIND, bool HILO>
-__global__ void __launch_bounds__(kThreads, Cfg<D, HILO>::kCtasPerSm) kv8_attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) kv8_attn_kernel(const AttnArgs a) {
   using C = Cfg<D, HILO>;
+  constexpr int kConsumers = C::kConsumers, kThreads = C::kThreads;
   constexpr int ROWS = C::kRows, NP = C::kPages;
-  constexpr int NR = HILO ? 1 : 2;  // query rows whose scores a lane holds: g (and g + 8)
+  constexpr int NR = HILO ? 1 : 2;        // query rows whose scores a lane holds: g (and g + 8)
   constexpr int kSb = D / 64;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int s_item, s_sub, s_page, s_begin, s_end, s_flag, s_sum[kWarps];
+  __shared__ int s_item, s_sub, s_unit, s_page, s_begin, s_end, s_pages[kThreads / 32], s_units[kThreads / 32];
+  __shared__ int s_last, s_due[2][6];  // a unit whose parts this CTA may have to merge
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n_items = a.it.n_items;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* empty = full + C::kStages;
+  uint32_t* mask = reinterpret_cast<uint32_t*>(smem + C::kOffMask);
+  if (threadIdx.x < C::kStages) {
+    mbar_init(&full[threadIdx.x], 1);
+    mbar_init(&empty[threadIdx.x], 1);
+    fence_barrier_init();
+  }
 
-  // ---- this CTA's stretch [s_begin, s_end) of the units' pages end to end: `per` pages from blockIdx.x * per on, but a
-  // cut inside a unit of at most kSnapPages moves to the unit's start
-  int total, per;
+  // ---- this CTA's stretch: pages [s_begin, s_end) of the units' pages end to end. The cuts are at multiples of `per`
+  // on a line where a unit takes kSegCost + its pages; a cut in the kSegCost, or inside a unit of at most kSnapPages, is
+  // at the unit's start.
+  int per;
   {
     const int each = (n_items + kThreads - 1) / kThreads;
     const int i0 = min(int(threadIdx.x) * each, n_items), i1 = min(i0 + each, n_items);
-    int mine = 0;
+    int my_pages = 0, my_units = 0;
     for (int i = i0; i < i1; ++i) {
       const Item x = load_item<ROWS>(a, i);
-      mine += x.pages * x.subs;
+      my_pages += x.pages * x.subs;
+      my_units += x.pages ? x.subs : 0;
     }
-    int inc = mine;
+    int pages = my_pages, units = my_units;  // up to and with this thread's items
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
+      const int y = __shfl_up_sync(0xffffffffu, pages, o), z = __shfl_up_sync(0xffffffffu, units, o);
+      if (lane >= o) pages += y, units += z;
     }
-    if (lane == 31) s_sum[warp] = inc;
+    if (lane == 31) s_pages[warp] = pages, s_units[warp] = units;
     __syncthreads();
-    total = 0;
+    int all_pages = 0, all_units = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) inc += s_sum[w];
-      total += s_sum[w];
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) pages += s_pages[w], units += s_units[w];
+      all_pages += s_pages[w], all_units += s_units[w];
     }
-    per = max((total + int(gridDim.x) - 1) / int(gridDim.x), C::kMinPages);
+    const int total = all_pages + all_units * C::kSegCost;
+    per = max((total + int(gridDim.x) - 1) / int(gridDim.x), C::kSegCost + 1);
+    const int hi = pages + units * C::kSegCost, lo = hi - my_pages - my_units * C::kSegCost;
     // the cuts before and after this CTA, found by the threads in whose items they fall
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < 2; ++k) {
       const int64_t cut64 = (int64_t(blockIdx.x) + k) * per;
       const int cut = cut64 < total ? static_cast<int>(cut64) : total;
       if (cut == total) {
-        if (threadIdx.x == 0) (k ? s_end : s_begin) = total;
-      } else if (cut >= inc - mine && cut < inc) {
-        int at = inc - mine, i = i0;
+        if (threadIdx.x == 0) (k ? s_end : s_begin) = all_pages;
+      } else if (cut >= lo && cut < hi) {
+        int at = lo, pg = pages - my_pages, un = units - my_units, i = i0;
         Item x = load_item<ROWS>(a, i);
-        while (cut - at >= x.pages * x.subs) {
-          at += x.pages * x.subs;
+        for (;;) {
+          const int cost = x.pages ? (x.pages + C::kSegCost) * x.subs : 0;
+          if (cut - at < cost) break;
+          at += cost, pg += x.pages * x.subs, un += x.pages ? x.subs : 0;
           x = load_item<ROWS>(a, ++i);
         }
-        const int sub = (cut - at) / x.pages, page = x.pages <= C::kSnapPages ? 0 : (cut - at) - sub * x.pages;
+        const int sub = (cut - at) / (x.pages + C::kSegCost), in = (cut - at) - sub * (x.pages + C::kSegCost);
+        const int page = x.pages <= C::kSnapPages ? 0 : max(0, in - C::kSegCost);
         if (k) {
-          s_end = at + sub * x.pages + page;
+          s_end = pg + sub * x.pages + page;
         } else {
-          s_begin = at + sub * x.pages + page;
-          s_item = i, s_sub = sub, s_page = page;
+          s_begin = pg + sub * x.pages + page;
+          s_item = i, s_sub = sub, s_unit = un + sub, s_page = page;
         }
       }
     }
@@ -280,140 +310,189 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, HILO>::kCtasPerSm) kv8_attn_k
   }
   if (begin >= end) return;
 
-  Cursor cc;  // the segment being attended
-  cc.item = s_item, cc.sub = s_sub, cc.page = s_page;
+  Cursor cc;  // the segment at hand
+  cc.item = s_item, cc.sub = s_sub, cc.unit = s_unit, cc.page = s_page;
   cc.x = load_item<ROWS>(a, cc.item);
   cc.seg = min(cc.x.pages - cc.page, end - begin);
   cc.rem = end - begin - cc.seg;
-  Cursor ic = cc;                // the segment of the next load
-  int ipos = warp * NP;          // and this warp's next chunk in it
-  const int64_t pg_bytes = page_bytes(D, a.n_kv_heads);
 
-  uint8_t* ring = smem + warp * C::kStages * C::kStageBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar) + warp * C::kStages;
-  if (lane == 0) {
-    for (int s = 0; s < C::kStages; ++s) mbar_init(&bars[s], 1);
-    fence_barrier_init();
+  if (warp == kConsumers) {
+    // ================= loads: every chunk of every segment in order, as the stages become free
+    const int64_t pg_bytes = page_bytes(D, a.n_kv_heads);
+    int k = 0;  // chunks so far
+    bool ok = true;
+    for (;;) {
+      const int kvh = cc.sub - a.by_kv_heads.div(cc.sub) * a.n_kv_heads;
+      const int32_t* pt = a.it.page_table + int64_t(cc.item) * a.it.pt_stride + cc.page;
+      const uint8_t* head = a.pool + int64_t(kvh) * C::kBlock;
+      int32_t pid = lane < cc.seg ? pt[lane] : -1;  // 32 pages at a time, the next ones read ahead
+      for (int p0 = 0; p0 < cc.seg && ok; p0 += 32) {
+        const int32_t ahead = p0 + 32 + lane < cc.seg ? pt[p0 + 32 + lane] : -1;
+        const int n = min(32, cc.seg - p0);
+        for (int c0 = 0; c0 < n && ok; c0 += C::kBatch) {  // some chunks at a time, a lane for each page
+          const int32_t mine = __shfl_sync(0xffffffffu, pid, c0 + (lane & (C::kBatch - 1)));
+          const bool in = lane < C::kBatch && c0 + lane < n, there = in && mine >= 0 && mine < a.n_pages;
+          if (in && !there) flag_error(a.err, kErrPageId);
+          const int kk = k + (lane >> 1), s = kk % C::kStages;
+          ok = __all_sync(0xffffffffu, !in || kk < C::kStages ||
+                                           mbar_wait(&empty[s], ((kk / C::kStages) & 1) ^ 1, a.err));
+          if (!ok) break;
+          const uint32_t m = (__ballot_sync(0xffffffffu, there) >> (lane & ~1)) & 3u;
+          if (in && (lane & 1) == 0) {
+            mask[s] = m;
+            mbar_arrive_expect_tx(&full[s], __popc(m) * uint32_t(C::kBlock));
+          }
+          __syncwarp();
+          if (there)
+            bulk_load(smem + s * C::kStageBytes + (lane & 1) * C::kBlock, head + int64_t(mine) * pg_bytes, C::kBlock,
+                      &full[s]);
+          k += (min(C::kBatch, n - c0) + 1) / 2;
+        }
+        pid = ahead;
+      }
+      if (!ok || cc.rem == 0) break;
+      next_segment<ROWS>(a, cc);
+    }
+    // No load outlives the CTA: the last ones are waited for (bounded) whether or not a consumer attends them.
+    for (int i = max(0, k - C::kStages); i < k; ++i) mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, a.err);
+    return;
   }
-  __syncwarp();
 
-  // The next chunk to load: lane j < NP gets its page j's id (-1: past the segment, -2: no such page); ikvh its head.
-  // False when the stretch holds no further chunk for this warp.
-  int ikvh = 0;
-  auto next_chunk = [&](int32_t& pid) -> bool {
-    while (ipos >= ic.seg) {
-      if (ic.rem == 0) return false;
-      next_segment<ROWS>(a, ic);
-      ipos = warp * NP;
-    }
-    pid = -1;
-    if (lane < NP && ipos + lane < ic.seg) {
-      pid = a.it.page_table[int64_t(ic.item) * a.it.pt_stride + ic.page + ipos + lane];
-      if (pid < 0 || pid >= a.n_pages) pid = -2;
-    }
-    ikvh = ic.sub - a.by_kv_heads.div(ic.sub) * a.n_kv_heads;
-    ipos += kWarps * NP;
-    return true;
-  };
-  // loaded: NP bits per ring stage, the pages that were loaded (the same in every lane).
-  uint32_t loaded = 0;
-  auto issue = [&](int stage, int32_t pid, int kvh) {
-    const uint32_t there = __ballot_sync(0xffffffffu, pid >= 0);
-    loaded = (loaded & ~(((1u << NP) - 1u) << (NP * stage))) | (there << (NP * stage));
-    uint8_t* st = ring + stage * C::kStageBytes;
-    if (lane == 0) {
-      fence_proxy_async_smem();  // this warp's reads of the stage come before its next write
-      mbar_arrive_expect_tx(&bars[stage], __popc(there) * (C::kBlock + 16u));
-    }
-    __syncwarp();
-    if (pid >= 0) {
-      const uint8_t* pg = a.pool + int64_t(pid) * pg_bytes;
-      bulk_load(st + lane * C::kBlock, pg + int64_t(kvh) * C::kBlock, C::kBlock, &bars[stage]);
-      bulk_load(st + NP * C::kBlock + lane * 16, pg + scale_off(D, a.n_kv_heads, kvh), 16, &bars[stage]);
-    } else if (pid == -2) {
-      flag_error(a.err, kErrPageId);
+  // ================= the attending warps
+  // The queries of a segment's tile into shared memory in operand order -- 16 bytes for each k-step (4 dims of
+  // every lane t) and lane -- each row over its largest power of two, so fp16 holds it whatever its magnitude; and
+  // per row the factor and offset that make a raw product a score: raw * factor * s_k - offset * s_k (log2 units).
+  uint4* s_q = reinterpret_cast<uint4*>(smem + C::kOffQ);
+  float* s_row = reinterpret_cast<float*>(smem + C::kOffRow);
+  constexpr int kLanes = D / 4;                                               // threads of a row, 4 dims each
+  constexpr int kQSteps = (ROWS * kLanes + kConsumers * 32 - 1) / (kConsumers * 32);
+  auto read_queries = [&](const Cursor& c, float (&x)[kQSteps][4]) {
+    const int tile = a.by_kv_heads.div(c.sub), kvh = c.sub - tile * a.n_kv_heads, n_rows_item = c.x.q_len * a.group;
+#pragma unroll
+    for (int i = 0; i < kQSteps; ++i) {
+      const int u = i * kConsumers * 32 + threadIdx.x;
+      const int row = u / kLanes, d = (u % kLanes) * 4, r = tile * ROWS + row;
+      x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+      if (row < ROWS && r < n_rows_item) {
+        const int tok = a.by_group.div(r), hd = kvh * a.group + r - tok * a.group;
+        load4q(a, ((int64_t(c.x.q_start) + tok) * a.n_heads + hd) * D + d, x[i]);
+      }
     }
   };
-  int n_issued = 0;  // chunks whose loads were issued, and attended (ring stage = count % kStages)
-  {
-    int32_t pid[C::kStages];
-    int kvh[C::kStages];
-    bool go = true;
+  auto write_queries = [&](const float (&xs)[kQSteps][4]) {
 #pragma unroll
-    for (int s = 0; s < C::kStages; ++s) {  // the page-table reads of all stages before the first copy
-      pid[s] = -1;
-      go = go && next_chunk(pid[s]);
-      kvh[s] = ikvh;
-      if (go) n_issued = s + 1;
+    for (int i = 0; i < kQSteps; ++i) {
+      const int u = i * kConsumers * 32 + threadIdx.x;
+      if (u >= ROWS * kLanes) break;  // whole warps
+      const int row = u / kLanes, d = (u % kLanes) * 4;
+      const float(&x)[4] = xs[i];
+      float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const uint32_t e = min(max(__float_as_uint(mx) >> 23, 1u), 253u);
+      const float inv = __uint_as_float((254u - e) << 23);
+      // dim d = 64 sb + 16 t + 4 ks: k-step 4 sb + ks, lane (row % 8, t)
+      const int at = ((d >> 6) * 4 + ((d >> 2) & 3)) * 32 + (row & 7) * 4 + ((d >> 4) & 3);
+      uint32_t hi0, hi1, lo0 = 0, lo1 = 0;
+      if constexpr (HILO) {
+        split_half2(make_float2(x[0] * inv, x[1] * inv), hi0, lo0);
+        split_half2(make_float2(x[2] * inv, x[3] * inv), hi1, lo1);
+        s_q[at] = make_uint4(hi0, lo0, hi1, lo1);
+      } else {
+        hi0 = pack(x[0] * inv, x[1] * inv);
+        hi1 = pack(x[2] * inv, x[3] * inv);
+        uint32_t* w = reinterpret_cast<uint32_t*>(&s_q[at]) + (row >> 3);
+        w[0] = hi0;
+        w[2] = hi1;
+      }
+      float sum = 0.f;
+      if constexpr (KIND == NBL_I8) {
+        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&hi0));
+        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi1));
+        const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&lo0));
+        const float2 l1 = __half22float2(*reinterpret_cast<const __half2*>(&lo1));
+        sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((l0.x + l0.y) + (l1.x + l1.y));
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      }
+      if (d == 0) {
+        const float scale = __uint_as_float(e << 23) * a.scale_log2;
+        s_row[row] = scale * key_unit<KIND>();
+        s_row[ROWS + row] = 128.f * sum * scale;
+      }
     }
-#pragma unroll
-    for (int s = 0; s < C::kStages; ++s)
-      if (s < n_issued) issue(s, pid[s], kvh[s]);
-  }
-  int n_done = 0;
+  };
+  // A barrier of the attending warps.
+  auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); };
+  float xq[kQSteps][4];
+  read_queries(cc, xq);
+  write_queries(xq);
+  sync();
+  // Four outputs of row rr of (item, KV head): dims d.. of its head.
+  auto store4 = [&](int q_start, int kvh, int rr, int d, float4 v, float L, float m) {
+    const int tok = a.by_group.div(rr);
+    const int64_t row = (int64_t(q_start) + tok) * a.n_heads + kvh * a.group + rr - tok * a.group;
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    if (a.out_dtype == NBL_F32 && a.q_vec) {
+      *reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * D + d) =
+          make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    } else {
+      store_as(a.out, row * D + d, v.x * inv, a.out_dtype);
+      store_as(a.out, row * D + d + 1, v.y * inv, a.out_dtype);
+      store_as(a.out, row * D + d + 2, v.z * inv, a.out_dtype);
+      store_as(a.out, row * D + d + 3, v.w * inv, a.out_dtype);
+    }
+    if (d == 0 && a.lse) a.lse[row] = L > 0.f ? (m + log2f(L)) * kLn2 : -INFINITY;
+  };
+  // The unit in s_due, whose parts are all in scratch, if this CTA was the last to arrive.
+  int seg_parity = 0;
+  auto merge_parts = [&] {
+    if (!s_last) return;
+    __threadfence();
+    const int* w = s_due[seg_parity];
+    const int q_start = w[0], kvh = w[1], row0 = w[2], n_here = w[3], first = w[4], last = w[5];
+    // CTA k's part of the unit
+    auto part = [&](int k) -> const float* {
+      return a.part + (int64_t(k) * 2 + (k == first ? 1 : 0)) * C::kMergeFloats;
+    };
+    for (int u = threadIdx.x; u < n_here * (D / 4); u += kConsumers * 32) {
+      const int r = u / (D / 4), d = (u % (D / 4)) * 4;
+      float mx = -INFINITY;
+#pragma unroll 8
+      for (int k = first; k <= last; ++k) mx = fmaxf(mx, __ldcg(part(k) + ROWS * D + r));
+      float L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (mx != -INFINITY) {
+#pragma unroll 4
+        for (int k = first; k <= last; ++k) {
+          const float* pb = part(k);
+          const float e = ex2(__ldcg(pb + ROWS * D + r) - mx);
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(pb + r * D + d));
+          L = fmaf(e, __ldcg(pb + ROWS * D + ROWS + r), L);
+          O.x = fmaf(e, x.x, O.x), O.y = fmaf(e, x.y, O.y), O.z = fmaf(e, x.z, O.z), O.w = fmaf(e, x.w, O.w);
+        }
+      }
+      store4(q_start, kvh, row0 + r, d, O, L, mx);
+    }
+  };
+  bool due = false;  // whether the segment before was part of a unit
+  int k0 = 0;  // chunks before this segment
   bool alive = true;  // false after a wait that gave up
+  float* mrg = reinterpret_cast<float*>(smem + C::kOffMerge);
 
   for (;;) {  // segments
     const int tile = a.by_kv_heads.div(cc.sub), kvh = cc.sub - tile * a.n_kv_heads;
     const int row0 = tile * ROWS, n_rows_item = cc.x.q_len * a.group;
     const int n_here = min(ROWS, n_rows_item - row0);
     const int kv_min = cc.x.pos0 + a.by_group.div(row0) + 1;  // keys that every row of the tile sees
-
-    // ---- Q as the A operand: row g's (and row g + 8's) dims 64 sb + 16 t + 4 ks ..+3 for k-step (sb, ks)
-    uint32_t qa[kSb * 4][4];
-    float row_scale[NR], row_off[NR];  // score = raw * row_scale * s_k - row_off * s_k (log2 units)
-    int lim[NR];                       // keys the row sees
+    float row_scale[NR], row_off[NR];
+    int lim[NR];  // keys the row sees
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      const int r = row0 + g + 8 * n;
-      const bool valid = r < n_rows_item;
-      const int tok = valid ? a.by_group.div(r) : 0, head = kvh * a.group + (valid ? r - tok * a.group : 0);
-      const int64_t base = ((int64_t(cc.x.q_start) + tok) * a.n_heads + head) * D;
-      lim[n] = valid ? cc.x.pos0 + tok + 1 : 0;
-      float x[kSb * 4][4];
-      float mx = 0.f;
-#pragma unroll
-      for (int k = 0; k < kSb * 4; ++k) {
-        if (valid) load4q(a, base + 64 * (k >> 2) + 16 * t + 4 * (k & 3), x[k]);
-        else x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fabsf(x[k][j]));
-      }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      // the row over its largest power of two: fp16 then holds it whatever its magnitude
-      const uint32_t e = min(max(__float_as_uint(mx) >> 23, 1u), 253u);
-      const float inv = __uint_as_float((254u - e) << 23);
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < kSb * 4; ++k) {
-        uint32_t hi0, hi1, lo0 = 0, lo1 = 0;
-        if constexpr (HILO) {
-          split_half2(make_float2(x[k][0] * inv, x[k][1] * inv), hi0, lo0);
-          split_half2(make_float2(x[k][2] * inv, x[k][3] * inv), hi1, lo1);
-          qa[k][0] = hi0, qa[k][1] = lo0, qa[k][2] = hi1, qa[k][3] = lo1;
-        } else {
-          qa[k][n] = hi0 = pack(x[k][0] * inv, x[k][1] * inv);
-          qa[k][2 + n] = hi1 = pack(x[k][2] * inv, x[k][3] * inv);
-        }
-        if constexpr (KIND == NBL_I8) {
-          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&hi0));
-          const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi1));
-          const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&lo0));
-          const float2 l1 = __half22float2(*reinterpret_cast<const __half2*>(&lo1));
-          sum += ((f0.x + f0.y) + (f1.x + f1.y)) + ((l0.x + l0.y) + (l1.x + l1.y));
-        }
-      }
-      const float scale = __uint_as_float(e << 23) * a.scale_log2;
-      row_scale[n] = scale * key_unit<KIND>();
-      row_off[n] = 0.f;
-      if constexpr (KIND == NBL_I8) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        row_off[n] = 128.f * sum * scale;
-      }
+      row_scale[n] = s_row[g + 8 * n];
+      row_off[n] = s_row[ROWS + g + 8 * n];
+      lim[n] = row0 + g + 8 * n < n_rows_item ? cc.x.pos0 + a.by_group.div(row0 + g + 8 * n) + 1 : 0;
     }
-
     float2 o[D / 8][2];  // dims (8j + 2t, 8j + 2t + 1) of row g; of row g + 8, or of row g's remainder terms
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = make_float2(0.f, 0.f);
@@ -422,56 +501,60 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, HILO>::kCtasPerSm) kv8_attn_k
     for (int n = 0; n < NR; ++n) m_run[n] = -INFINITY, l_run[n] = 0.f;
     float vref = 0.f, vinv = 0.f;  // largest value scale so far, and 2^14 / it
 
-    // One chunk: FULL when all its pages are loaded and every row sees all their tokens.
-    auto attend = [&](auto full, const uint8_t* st, uint32_t there, int tok0) {
-      constexpr bool FULL = decltype(full)::value;
+    // Two pages at st; FULL when both are loaded and every row sees all their tokens (else `there` has a bit for each
+    // loaded one, and the rows see the tokens below lim).
+    auto attend = [&](auto whole, const uint8_t* st, uint32_t there, int tok0) {
+      constexpr bool FULL = decltype(whole)::value;
       float2 s[NR][NP][2];  // lane's tokens (2t, 2t+1) and (8+2t, 9+2t) of each page
       float2 sc[NP];
+      float c0[NP][4], c1[NP][4];
+#pragma unroll
+      for (int sb = 0; sb < kSb; ++sb) {
+        uint4 ka[NP], kb[NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          const uint8_t* kp = st + j * C::kBlock + sb * 1024 + lane * 16;
+          ka[j] = *reinterpret_cast<const uint4*>(kp);
+          kb[j] = *reinterpret_cast<const uint4*>(kp + 512);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const uint4 q = s_q[(sb * 4 + ks) * 32 + lane];
+          const uint32_t q4[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            const uint32_t wa = ks == 0 ? ka[j].x : ks == 1 ? ka[j].y : ks == 2 ? ka[j].z : ka[j].w;
+            const uint32_t wb = ks == 0 ? kb[j].x : ks == 1 ? kb[j].y : ks == 2 ? kb[j].z : kb[j].w;
+            uint32_t b0, b1;
+            widen4_key<KIND>(wa, b0, b1);
+            if (sb == 0 && ks == 0) mma_first(c0[j], q4, b0, b1);
+            else mma(c0[j], q4, b0, b1);
+            widen4_key<KIND>(wb, b0, b1);
+            if (sb == 0 && ks == 0) mma_first(c1[j], q4, b0, b1);
+            else mma(c1[j], q4, b0, b1);
+          }
+        }
+      }
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
-        sc[j] = *reinterpret_cast<const float2*>(st + NP * C::kBlock + j * 16);
-        if constexpr (!FULL) {
-          if (!((there >> j) & 1u)) {
-            sc[j] = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int n = 0; n < NR; ++n) s[n][j][0] = s[n][j][1] = make_float2(-INFINITY, -INFINITY);
-            continue;
-          }
-        }
-        float c0[4], c1[4];
-#pragma unroll
-        for (int sb = 0; sb < kSb; ++sb) {
-          const uint8_t* kp = st + j * C::kBlock + sb * 1024 + lane * 16;
-          const uint4 ka = *reinterpret_cast<const uint4*>(kp);
-          const uint4 kb = *reinterpret_cast<const uint4*>(kp + 512);
-          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint32_t(&q4)[4] = qa[sb * 4 + ks];
-            uint32_t b0, b1;
-            widen4_key<KIND>(wa[ks], b0, b1);
-            if (sb == 0 && ks == 0) mma_first(c0, q4, b0, b1);
-            else mma(c0, q4, b0, b1);
-            widen4_key<KIND>(wb[ks], b0, b1);
-            if (sb == 0 && ks == 0) mma_first(c1, q4, b0, b1);
-            else mma(c1, q4, b0, b1);
-          }
-        }
+        sc[j] = *reinterpret_cast<const float2*>(st + j * C::kBlock + scale_off(D));
+        const bool got = FULL || ((there >> j) & 1u);
+        if (!got) sc[j] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
           if constexpr (HILO) {
-            s[n][j][0] = __fadd2_rn(make_float2(c0[0], c0[1]), make_float2(c0[2], c0[3]));
-            s[n][j][1] = __fadd2_rn(make_float2(c1[0], c1[1]), make_float2(c1[2], c1[3]));
+            s[n][j][0] = __fadd2_rn(make_float2(c0[j][0], c0[j][1]), make_float2(c0[j][2], c0[j][3]));
+            s[n][j][1] = __fadd2_rn(make_float2(c1[j][0], c1[j][1]), make_float2(c1[j][2], c1[j][3]));
           } else {
-            s[n][j][0] = make_float2(c0[2 * n], c0[2 * n + 1]);
-            s[n][j][1] = make_float2(c1[2 * n], c1[2 * n + 1]);
+            s[n][j][0] = make_float2(c0[j][2 * n], c0[j][2 * n + 1]);
+            s[n][j][1] = make_float2(c1[j][2 * n], c1[j][2 * n + 1]);
           }
           if constexpr (!FULL) {
-            const int tok = tok0 + j * kPage + 2 * t;
-            if (tok >= lim[n]) s[n][j][0].x = -INFINITY;
-            if (tok + 1 >= lim[n]) s[n][j][0].y = -INFINITY;
-            if (tok + 8 >= lim[n]) s[n][j][1].x = -INFINITY;
-            if (tok + 9 >= lim[n]) s[n][j][1].y = -INFINITY;
+            const int tok = tok0 + j * kPage + 2 * t, see = got ? lim[n] : 0;
+            if (tok >= see) s[n][j][0].x = -INFINITY;
+            if (tok + 1 >= see) s[n][j][0].y = -INFINITY;
+            if (tok + 8 >= see) s[n][j][1].x = -INFINITY;
+            if (tok + 9 >= see) s[n][j][1].y = -INFINITY;
           }
         }
       }
@@ -541,22 +624,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, HILO>::kCtasPerSm) kv8_attn_k
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         float acc[4][4];
-        if constexpr (!FULL) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc[k][0] = acc[k][1] = acc[k][2] = acc[k][3] = 0.f;
-        }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
+          uint4 v4 = *reinterpret_cast<const uint4*>(st + j * C::kBlock + kPage * D + c * 512 + lane * 16);
           if constexpr (!FULL) {
-            if (!((there >> j) & 1u)) continue;
+            if (!((there >> j) & 1u)) v4 = uint4{};  // nothing was loaded: any finite codes will do
           }
-          const uint4 v4 = *reinterpret_cast<const uint4*>(st + j * C::kBlock + kPage * D + c * 512 + lane * 16);
           const uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             uint32_t b0, b1;
             widen4<KIND>(w[k], b0, b1);
-            if (FULL && j == 0) mma_first(acc[k], pa[j], b0, b1);
+            if (j == 0) mma_first(acc[k], pa[j], b0, b1);
             else mma(acc[k], pa[j], b0, b1);
           }
         }
@@ -569,35 +648,34 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, HILO>::kCtasPerSm) kv8_attn_k
       }
     };
 
-    for (int pos = warp * NP; pos < cc.seg && alive; pos += kWarps * NP) {
-      const int stage = n_done % C::kStages;
-      alive = warp_wait_all(&bars[stage], (n_done / C::kStages) & 1, a.err);
+    const int n_chunks = (cc.seg + C::kPages - 1) / C::kPages;
+    for (int i = (warp + kConsumers - k0 % kConsumers) % kConsumers; i < n_chunks && alive; i += kConsumers) {
+      const int stage = (k0 + i) % C::kStages;
+      alive = warp_wait_all(&full[stage], ((k0 + i) / C::kStages) & 1, a.err);
       if (!alive) break;
-      ++n_done;
-      // the ids of the chunk this stage takes next, read now and used below
-      int32_t pid = -1;
-      const bool more = next_chunk(pid);
-      const int kvh_next = ikvh;
-      const uint8_t* st = ring + stage * C::kStageBytes;
-      const uint32_t there = (loaded >> (NP * stage)) & ((1u << NP) - 1u);
-      const int tok0 = (cc.page + pos) * kPage;
+      const uint32_t there = mask[stage];
+      const uint8_t* st = smem + stage * C::kStageBytes;
+      const int tok0 = (cc.page + i * NP) * kPage;
       if (there == (1u << NP) - 1u && tok0 + NP * kPage <= kv_min) attend(std::true_type{}, st, there, tok0);
-      else attend(std::false_type{}, st, there, tok0);
+      else if (there) attend(std::false_type{}, st, there, tok0);
       __syncwarp();
-      if (more) {
-        issue(stage, pid, kvh_next);
-        ++n_issued;
-      }
+      if (lane == 0) mbar_arrive(&empty[stage]);
     }
+    k0 += n_chunks;
 
-    // ---- merge the 4 warps through shared memory
+    // ---- merge the warps through shared memory; the next segment's queries are on their way meanwhile
+    const Cursor done = cc;
+    const bool more = cc.rem > 0;
+    if (more) {
+      next_segment<ROWS>(a, cc);
+      read_queries(cc, xq);
+    }
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       l_run[n] += __shfl_xor_sync(0xffffffffu, l_run[n], 1);
       l_run[n] += __shfl_xor_sync(0xffffffffu, l_run[n], 2);
     }
-    __syncthreads();  // the merge area is free: every warp is past the segment before
-    float* mrg = reinterpret_cast<float*>(smem + C::kOffMerge);
+    sync();  // every warp is done with the segment's queries, and with the merge of the segment before
     {
       float* w_o = mrg + warp * C::kMergeFloats;
       float* w_m = w_o + ROWS * D;
@@ -619,39 +697,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, HILO>::kCtasPerSm) kv8_attn_k
         }
       }
     }
-    __syncthreads();
-    // Row r of the tile as a row of the packed (token, head) outputs.
-    auto out_row = [&](int r) -> int64_t {
-      const int rr = row0 + r, tok = a.by_group.div(rr);
-      return (int64_t(cc.x.q_start) + tok) * a.n_heads + kvh * a.group + rr - tok * a.group;
-    };
-    auto store4 = [&](int r, int d, float4 v, float L, float m) {
-      const float inv = L > 0.f ? 1.f / L : 0.f;
-      const int64_t row = out_row(r);
-      if (a.out_dtype == NBL_F32 && a.q_vec) {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * D + d) =
-            make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-      } else {
-        store_as(a.out, row * D + d, v.x * inv, a.out_dtype);
-        store_as(a.out, row * D + d + 1, v.y * inv, a.out_dtype);
-        store_as(a.out, row * D + d + 2, v.z * inv, a.out_dtype);
-        store_as(a.out, row * D + d + 3, v.w * inv, a.out_dtype);
-      }
-      if (d == 0 && a.lse) a.lse[row] = L > 0.f ? (m + log2f(L)) * kLn2 : -INFINITY;
-    };
-    const bool whole = cc.page == 0 && cc.seg == cc.x.pages;
+    if (more) write_queries(xq);
+    sync();
+    if (due) merge_parts();
+    const bool whole = done.page == 0 && done.seg == done.x.pages;
     // a part of a unit: slot 1 where the unit starts in this CTA's stretch, else slot 0
-    float* mine = a.part + (int64_t(blockIdx.x) * 2 + (cc.page == 0 ? 1 : 0)) * C::kMergeFloats;
-    for (int u = threadIdx.x; u < ROWS * (D / 4); u += kThreads) {
+    float* mine = a.part + (int64_t(blockIdx.x) * 2 + (done.page == 0 ? 1 : 0)) * C::kMergeFloats;
+    for (int u = threadIdx.x; u < n_here * (D / 4); u += kConsumers * 32) {
       const int r = u / (D / 4), d = (u % (D / 4)) * 4;
       float mx = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, mrg[w * C::kMergeFloats + ROWS * D + r]);
+      for (int w = 0; w < kConsumers; ++w) mx = fmaxf(mx, mrg[w * C::kMergeFloats + ROWS * D + r]);
       float L = 0.f;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
       if (mx != -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < kConsumers; ++w) {
           const float* wb = mrg + w * C::kMergeFloats;
           const float k = ex2(wb[ROWS * D + r] - mx);  // 0 for warps that saw no key
           const float4 x = *reinterpret_cast<const float4*>(wb + r * D + d);
@@ -660,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, HILO>::kCtasPerSm) kv8_attn_k
         }
       }
       if (whole) {
-        if (r < n_here) store4(r, d, O, L, mx);
+        store4(done.x.q_start, kvh, row0 + r, d, O, L, mx);
       } else {
         *reinterpret_cast<float4*>(mine + r * D + d) = O;
         if (d == 0) {
@@ -669,49 +730,32 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, HILO>::kCtasPerSm) kv8_attn_k
         }
       }
     }
-    if (!whole) {
-      // The CTAs whose stretches hold the unit: first .. last. The last of them to arrive merges; the counter (of the
-      // first) wraps back to 0 for the next launch.
-      // (Cuts inside a unit long enough to be cut are exact multiples of `per`.)
-      const int u0 = end - cc.rem - cc.seg - cc.page, u1 = u0 + cc.x.pages;  // the unit's place, pages end to end
-      const int first = u0 / per, last = (u1 - 1) / per;
+    due = !whole;
+    if (due) {
+      // The CTAs whose stretches hold the unit: first .. last (page p of a unit that starts at `at` on the cuts' line is
+      // behind the cuts up to at + kSegCost + p). The last of them to arrive merges; the counter (of the first) wraps
+      // back to 0 for the next launch. Only warp 0 waits for the arrival; the merge is done at the next barrier.
+      const int at = end - done.rem - done.seg - done.page + done.unit * C::kSegCost + C::kSegCost;
+      const int first = at / per, last = (at + done.x.pages - 1) / per;
+      seg_parity ^= 1;
       __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0)
-        s_flag = atomicInc(&a.counts[first], static_cast<unsigned>(last - first)) == static_cast<unsigned>(last - first);
-      __syncthreads();
-      if (s_flag) {
-        __threadfence();
-        for (int u = threadIdx.x; u < n_here * (D / 4); u += kThreads) {
-          const int r = u / (D / 4), d = (u % (D / 4)) * 4;
-          // CTA k's part of the unit
-          auto part = [&](int k) -> const float* {
-            return a.part + (int64_t(k) * 2 + (k == first ? 1 : 0)) * C::kMergeFloats;
-          };
-          float mx = -INFINITY;
-#pragma unroll 8
-          for (int k = first; k <= last; ++k) mx = fmaxf(mx, __ldcg(part(k) + ROWS * D + r));
-          float L = 0.f;
-          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (mx != -INFINITY) {
-#pragma unroll 4
-            for (int k = first; k <= last; ++k) {
-              const float* pb = part(k);
-              const float w = ex2(__ldcg(pb + ROWS * D + r) - mx);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(pb + r * D + d));
-              L = fmaf(w, __ldcg(pb + ROWS * D + ROWS + r), L);
-              O.x = fmaf(w, x.x, O.x), O.y = fmaf(w, x.y, O.y), O.z = fmaf(w, x.z, O.z), O.w = fmaf(w, x.w, O.w);
-            }
-          }
-          store4(r, d, O, L, mx);
+      if (warp == 0) {
+        asm volatile("bar.sync 2, %0;" ::"n"(kConsumers * 32) : "memory");
+        if (lane == 0) {
+          s_last = atomicInc(&a.counts[first], static_cast<unsigned>(last - first)) == static_cast<unsigned>(last - first);
+          int* d = s_due[seg_parity];
+          d[0] = done.x.q_start, d[1] = kvh, d[2] = row0, d[3] = n_here, d[4] = first, d[5] = last;
         }
+      } else {
+        asm volatile("bar.arrive 2, %0;" ::"n"(kConsumers * 32) : "memory");
       }
     }
-    if (cc.rem == 0) break;
-    next_segment<ROWS>(a, cc);
+    if (!more) break;
   }
-  // After a wait that gave up, the loads still in flight are drained (bounded) before the CTA ends.
-  for (int i = n_done; i < n_issued; ++i) mbar_wait(&bars[i % C::kStages], (i / C::kStages) & 1, a.err);
+  if (due) {
+    sync();
+    merge_parts();
+  }
 }
 
 template <int D, int KIND, bool HILO>
@@ -727,7 +771,7 @@ void launch_t(cudaStream_t st, const AttnArgs& a, int grid) {
                "kv8 attention smem attribute");
     configured.fetch_or(bit);
   }
-  kv8_attn_kernel<D, KIND, HILO><<<grid, kThreads, C::kSmemBytes, st>>>(a);
+  kv8_attn_kernel<D, KIND, HILO><<<grid, C::kThreads, C::kSmemBytes, st>>>(a);
 }
 
 template <int D, int KIND>
@@ -752,11 +796,11 @@ Kv8AttnPlan plan_kv8_attn(const nbl_kv* kv, int n_items, int max_len, int n_head
     Kv8AttnPlan p;
     const int64_t tiles = (int64_t(max_len) * (n_heads / kv->cfg.n_kv_heads) + C::kRows - 1) / C::kRows;
     const int64_t max_pages = std::max(1, (max_kv + kPage - 1) / kPage);
-    // the most pages that the call can have, in stretches of at least kMinPages: at most one wave of CTAs
-    if (double(n_items) * kv->cfg.n_kv_heads * double(tiles) * (double(kv->cfg.page_size) * double(max_pages)) > 3.0e10)
+    if (double(n_items) * kv->cfg.n_kv_heads * double(tiles) * (double(max_pages) + C::kSegCost) > 2.0e9)
       fail(NBL_E_INVALID, "attention: over 2^31 pages of all rows, heads and query tiles in one call");
-    const double bound = double(n_items) * kv->cfg.n_kv_heads * double(tiles) * double(max_pages) / C::kMinPages;
-    const int slots = num_sms * C::kCtasPerSm;
+    // one wave of CTAs, or one for each kSegCost + 1 of the most that the call can cost
+    const double bound = double(n_items) * kv->cfg.n_kv_heads * double(tiles) * (double(max_pages) + C::kSegCost) / (C::kSegCost + 1);
+    const int slots = num_sms * C::kCtas;
     p.grid = bound >= slots ? slots : std::max(1, static_cast<int>(std::ceil(bound)));
     p.scratch_bytes = size_t(p.grid) * 2 * C::kMergeFloats * sizeof(float);
     return p;
