@@ -20,8 +20,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libnibble_cuda.so")
 STAMP = LIB + ".stamp"
 SOURCES = ["api.cu", "rope.cu", "attn_f32.cu", "decode.cu", "decode_static.cu", "prefill.cu", "model_ops.cu", "quant_ops.cu", "quant_gemm.cu", "quant_blocks.cu", "f32_gemm.cu", "selftest.cu", "backend_route.cu",
-           "kv8_append.cu", "kv8_attn.cu", "kv_pages.cu", "kv8_api.cu"]
-HEADERS = ["qkv_epilogue.cuh", "kv8.cuh", "kv_pages.h", "nbl_device.cuh", "nbl_internal.h", "nbl_errors.h", "model_ops.h", "quant_common.cuh"]
+           "kv8_append.cu", "kv8_attn.cu", "kv8_prefill.cu", "kv_pages.cu", "kv8_api.cu"]
+HEADERS = ["qkv_epilogue.cuh", "kv8.cuh", "kv_pages.h", "softmax_tile.cuh", "nbl_device.cuh", "nbl_internal.h", "nbl_errors.h", "model_ops.h", "quant_common.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
          "--expt-relaxed-constexpr", "-I" + os.path.join(ROOT, "include")]

@@ -338,7 +338,17 @@ void kv8_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype,
   it.n_items = n_items;
   it.max_len = max_q_len;
   it.n_rows = n_q_rows;
-  kv8_attention(ctx, kv, it, q, q_dtype, n_heads, out, out_dtype, nullptr, pt_stride * kv->cfg.page_size);
+  const int max_kv = pt_stride * kv->cfg.page_size;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  if (q_dtype == NBL_F32 || !aligned || max_q_len <= nbl::kKv8FewTokens || n_items > 65535 ||
+      n_q_rows * n_heads >= (int64_t(1) << 31)) {
+    kv8_attention(ctx, kv, it, q, q_dtype, n_heads, out, out_dtype, nullptr, max_kv);
+    return;
+  }
+  use_device(ctx);
+  const auto plan = nbl::plan_kv8_prefill(kv, n_items, max_q_len, n_q_rows, n_heads, max_kv, ctx->num_sms);
+  ensure_scratch(ctx, plan.scratch_bytes);
+  nbl::launch_kv8_prefill(ctx->stream, kv, it, q, q_dtype, n_heads, out, out_dtype, plan, ctx->scratch, ctx->d_err);
 }
 
 void require_weight(const nbl_ctx* ctx, const nbl_weight* w, const char* what) {

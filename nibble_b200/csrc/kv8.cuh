@@ -191,4 +191,17 @@ void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, c
                      void* out, int out_dtype, float* lse, const Kv8AttnPlan& plan, void* scratch, unsigned* counts,
                      int* err);
 
+// Longest query stretch that the warp-level kernel takes; longer ones go to the tcgen05 one.
+constexpr int kKv8FewTokens = 24;
+// kv8_prefill.cu: the same for many query tokens of 16-bit type (q and out 16-byte aligned) on the tensor cores. n_rows:
+// rows of q; split keys leave partial results in scratch.
+struct Kv8PrefillPlan {
+  int n_splits = 1, n_works = 0, grid = 1;
+  size_t scratch_bytes = 0;
+};
+Kv8PrefillPlan plan_kv8_prefill(const nbl_kv* kv, int n_items, int max_len, int64_t n_rows, int n_heads, int max_kv,
+                                int num_sms);
+void launch_kv8_prefill(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, const void* q, int q_dtype, int n_heads,
+                        void* out, int out_dtype, const Kv8PrefillPlan& plan, void* scratch, int* err);
+
 }  // namespace nbl

@@ -217,6 +217,15 @@ __global__ void __launch_bounds__(kThreads) kv8_pages_kernel(uint8_t* pool, int6
   uint8_t* blk = pg + int64_t(kvh) * block_bytes(D);
   float* sc = reinterpret_cast<float*>(blk + scale_off(D));
   for (int w = 0; w < 2; ++w) {
+    float v = 0.f;
+    if constexpr (IMPORT) {
+      v = scales[(i * 2 + w) * n_kv_heads + kvh];
+      if (!(v >= 0.f && v <= kHuge)) {
+        if (threadIdx.x == 0) flag_error(err, kErrNonFinite);
+        v = 0.f;
+      }
+      if (v < kTiny / 448.f) v = 0.f;  // as the append: no scale whose reciprocal is not finite
+    }
     uint8_t* src = codes + ((i * 2 + w) * n_kv_heads + kvh) * (kPage * D);
     for (int u = threadIdx.x; u < kPage * D / 4; u += kThreads) {  // words
       int at, tok[4], dim[4];
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(kThreads) kv8_pages_kernel(uint8_t* pool, int6
           }
           c |= x << (8 * b);
         }
-        *word = to_word<KIND>(c);
+        *word = to_word<KIND>(v > 0.f ? c : 0u);  // a scale of 0 has codes of 0
       } else {
         const uint32_t c = from_word<KIND>(*word);
 #pragma unroll
@@ -253,12 +262,6 @@ __global__ void __launch_bounds__(kThreads) kv8_pages_kernel(uint8_t* pool, int6
     if (threadIdx.x == 0) {
       float* s = scales + (i * 2 + w) * n_kv_heads + kvh;
       if constexpr (IMPORT) {
-        float v = *s;
-        if (!(v >= 0.f && v <= kHuge)) {
-          flag_error(err, kErrNonFinite);
-          v = 0.f;
-        }
-        if (v < kTiny / 448.f) v = 0.f;  // as the append: no scale whose reciprocal is not finite
         sc[w] = v;
       } else {
         *s = sc[w];
