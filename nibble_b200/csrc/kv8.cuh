@@ -78,7 +78,7 @@ __device__ __forceinline__ float decode(uint32_t code) {
 }
 // Four codes (byte i of `codes`) as the word that is stored, and back.
 template <int KIND>
-__host__ __device__ __forceinline__ uint32_t to_word(uint32_t codes) {
+__host__ __device__ constexpr uint32_t to_word(uint32_t codes) {
   if constexpr (KIND == NBL_I8) return codes ^ 0x80808080u;
   const uint32_t a = (codes & 0xffu) | ((codes & 0xff00u) << 8), b = ((codes >> 16) & 0xffu) | ((codes >> 8) & 0xff0000u);
   return ((a & 0x00800080u) << 8) | ((a & 0x007f007fu) << 7) | ((b & 0x00800080u) << 7) | (b & 0x007f007fu);

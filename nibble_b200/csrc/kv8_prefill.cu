@@ -43,16 +43,16 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: p may reach 2^8 before
 constexpr float kPShift = 6.0f;            // p' carries 2^6
 constexpr float kMinLv = -24.0f;           // smallest log2(s_v / vref) kept: below it a block adds nothing to fp16 weights
 
-template <int D, int HEADS>
+template <int D>
 struct PCfg {
-  static constexpr int NH = HEADS;                      // heads of a CTA
-  static constexpr int kCtas = D == 64 && NH == 2 ? 2 : 1;  // per SM
+  static constexpr int NH = 2;                          // heads of a CTA
+  static constexpr int kCtas = D == 64 ? 2 : 1;         // per SM
   static constexpr int SB = D == 64 ? 1 : 2;            // S buffers of a head
-  static constexpr bool kOwnConv = kCtas == 1;          // converting warps of their own
   static constexpr int ST = 3;                          // tiles of K and V operands
-  static constexpr int kConv = !kOwnConv ? 8 : D == 64 ? 2 : 4;  // converting warps
-  static constexpr int kConvPages = kOwnConv ? kTilePages / kConv : 1, kConvHalves = kOwnConv ? 2 : 1;  // of each, a tile
-  static constexpr int kWarpConv = kOwnConv ? 4 * NH : 0, kWarpMma = kWarpConv + kConv;
+  static constexpr int kConv = D == 64 ? 1 : 4;         // converting warps
+  static constexpr int kConvPages = kTilePages / kConv; // pages of a tile that one of them converts
+  static constexpr int kAhead = D == 64 ? 2 : 1;        // pages whose codes are on their way
+  static constexpr int kWarpConv = 4 * NH, kWarpMma = kWarpConv + kConv;
   static constexpr int kThreads = (kWarpMma + 1) * 32;
   static constexpr int kQBytes = kBM * D * 2;           // one head's Q tile: D / 64 parts of [128][64]
   static constexpr int kTileBytes = kBN * D * 2;        // K (or V) operand tile
@@ -65,8 +65,7 @@ struct PCfg {
                        kBarP = kBarS + NH * SB, kBarODone = kBarP + NH * SB, kBarODrained = kBarODone + NH,
                        kBarPV = kBarODrained + NH, kNumBars = kBarPV + NH;
   static constexpr int kOffTmemSlot = kOffBar + ((kNumBars * 8 + 15) & ~15);
-  static constexpr int kOffConv = kOffTmemSlot + 16;    // converters' cursors
-  static constexpr int kSmemBytes = kOffConv + (kOwnConv ? 0 : kConv * 48);
+  static constexpr int kSmemBytes = kOffTmemSlot + 16;
   static constexpr uint32_t kTmemCols = kCtas == 2 ? 256 : 512;
   __host__ __device__ static constexpr uint32_t col_s(int g, int buf) { return (g * SB + buf) * kBN; }
   __host__ __device__ static constexpr uint32_t col_o(int g) { return NH * SB * kBN + g * D; }
@@ -94,7 +93,6 @@ struct Work {
 // Work w (-1: none); the same in every warp. Works are numbered with the query tile (latest, so heaviest, first) slowest,
 // then the split, the item, the KV head and the head pair: the works of a round are about equally long, whatever the
 // number of items (with the item slowest, 4 prompts of 2048 tokens left the busiest CTA with 1.6 times the mean).
-template <int NH>
 __device__ __forceinline__ Work decode_work(const PrefillArgs& a, int w) {
   Work k{};
   k.valid = false;
@@ -107,8 +105,8 @@ __device__ __forceinline__ Work decode_work(const PrefillArgs& a, int w) {
   w /= a.it.n_items;
   k.split = w % a.n_splits;
   const int mt = a.m_tiles - 1 - w / a.n_splits;
-  k.n_g = min(NH, a.group - NH * hg);  // the last heads of a group may be fewer
-  k.head0 = k.kvh * a.group + NH * hg;
+  k.n_g = min(2, a.group - 2 * hg);  // an odd group leaves the last pair with one head
+  k.head0 = k.kvh * a.group + 2 * hg;
   k.qlen = a.it.len[item];
   k.pos0 = a.it.pos0[item];
   k.qs = a.it.start[item];
@@ -154,10 +152,10 @@ __device__ __forceinline__ void widen4_key(uint32_t w, uint32_t& lo, uint32_t& h
   }
 }
 
-template <int D, int HEADS, int KIND, bool BF16>
-__global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCtas)
+template <int D, int KIND, bool BF16>
+__global__ void __launch_bounds__(PCfg<D>::kThreads, PCfg<D>::kCtas)
     kv8_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const PrefillArgs a) {
-  using C = PCfg<D, HEADS>;
+  using C = PCfg<D>;
   constexpr int NH = C::NH, SB = C::SB, ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -213,127 +211,117 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
                             : static_cast<int>(blockIdx.x));
     return w < n_works ? w : -1;
   };
-  // ---- conversion of the tiles, in order across works: a warp has kPages pages of each tile, their keys (half 0), values
-  // (half 1) or both
-  constexpr int kRaw = D / 32;  // 16-byte pieces of half a block per lane
-  constexpr int kPages = C::kConvPages, kHalves = C::kConvHalves, kParts = kPages * kHalves;
-  struct Conv {
-    int w0, j, n, kt, kvh, page, last;  // round, tile of the work and their number, tile of the CTA, first page, end
-    const int32_t* pt_row;
-    int32_t id[kPages];  // the next tile's pages of this warp (-1: none)
-  };
-  const int cw = warp - C::kWarpConv, conv_page = C::kOwnConv ? cw * kPages : cw >> 1, conv_half = C::kOwnConv ? 0 : cw & 1;
-  const int64_t pg_bytes = page_bytes(D, a.n_kv_heads);
-  auto conv_id = [&](const Conv& c, int i) -> int32_t {
-    const int pg = c.page + c.j * kTilePages + conv_page + i;
-    if (pg >= c.last) return -1;
-    const int32_t id = c.pt_row[pg];
-    if (id >= 0 && id < a.n_pages) return id;
-    if (lane == 0) flag_error(a.err, kErrPageId);
-    return -1;
-  };
-  // The next tile (of the next work that has one); n = 0 when there is none.
-  auto conv_next = [&](Conv& c) {
-    if (++c.j >= c.n) {
-      c.j = c.n = 0;
-      while (c.n == 0) {
-        c.w0 += gridDim.x;
-        if (c.w0 >= a.n_works) return;
-        const Work wk = decode_work<NH>(a, work_of(c.w0, a.n_works));
-        if (!wk.valid) continue;
-        c.n = wk.t1 - wk.t0, c.kvh = wk.kvh, c.pt_row = wk.pt_row;
-        c.page = wk.t0 * kTilePages, c.last = min(wk.n_item_pages, wk.t1 * kTilePages);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kPages; ++i) c.id[i] = conv_id(c, i);
-  };
-  auto conv_read = [&](const Conv& c, uint4 (&raw)[kParts * kRaw], float (&scale)[kParts]) {
-#pragma unroll
-    for (int i = 0; i < kPages; ++i) {
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) scale[i * kHalves + h] = 0.f;
-      if (c.id[i] < 0) continue;
-      const uint8_t* blk = a.pool + int64_t(c.id[i]) * pg_bytes + int64_t(c.kvh) * C::kBlock;
-      const uint4* src = reinterpret_cast<const uint4*>(blk + conv_half * kPage * D) + lane;
-#pragma unroll
-      for (int k = 0; k < kHalves * kRaw; ++k) raw[i * kHalves * kRaw + k] = __ldg(src + 32 * k);
-      if (lane == 0) {
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-          scale[i * kHalves + h] = __ldg(reinterpret_cast<const float*>(blk + scale_off(D)) + conv_half + h);
-      }
-    }
-  };
-  // The tile's part of this warp into its stage, which has to be free; false after a wait that gave up.
-  auto conv_write = [&](const Conv& c, const uint4 (&raw)[kParts * kRaw], const float (&scale)[kParts]) -> bool {
-    const int s = c.kt % ST;
-    if (c.kt >= ST && !warp_wait(&bars[C::kBarKVEmpty + s], ((c.kt / ST) & 1) ^ 1, a.err)) return false;
-#pragma unroll
-    for (int part = 0; part < kParts; ++part) {
-      const int h = part % kHalves, b = conv_page + part / kHalves;
-      const bool there = c.id[part / kHalves] >= 0;
-      if (conv_half + h == 0) {  // keys: 16 dims of a token a step, to its row's chunks 2c and 2c + 1
-#pragma unroll
-        for (int i = 0; i < kRaw; ++i) {
-          const int u = i * 32 + lane, sb = u >> 6, tok = (u >> 2) & 15, ch = u & 3, row = b * kPage + tok;
-          const uint4 x = raw[part * kRaw + i];
-          uint4 y0 = uint4{}, y1 = uint4{};
-          if (there) {
-            widen4_key<KIND, BF16>(x.x, y0.x, y0.y);
-            widen4_key<KIND, BF16>(x.y, y0.z, y0.w);
-            widen4_key<KIND, BF16>(x.z, y1.x, y1.y);
-            widen4_key<KIND, BF16>(x.w, y1.z, y1.w);
-          }
-          uint8_t* dst = sK(s) + sb * (kBN * 128);
-          *reinterpret_cast<uint4*>(dst + swz128(row, 2 * ch)) = y0;
-          *reinterpret_cast<uint4*>(dst + swz128(row, 2 * ch + 1)) = y1;
+  if (warp >= C::kWarpConv && warp < C::kWarpMma) {
+    // ================= converters: a page at a time, in order across works; the codes of the next kAhead pages are on
+    // their way while one is widened and stored
+    constexpr int kRaw = D / 16;  // 16-byte pieces of a page's block per lane: its keys, then its values
+    constexpr int kA = C::kAhead, NB = kA + 1;
+    const int cw = warp - C::kWarpConv;
+    const int64_t pg_bytes = page_bytes(D, a.n_kv_heads);
+    uint4 raw[NB][kRaw];
+    float2 scale[NB];
+    int meta[NB];  // tile of the CTA * 4 + page of this warp in it; -1: no more
+    // The page that is read next: round, place among the work's pages of this warp and their number, tile of the CTA; the
+    // work's first page and its end, the page table row, the KV head's place in a page, and the ids of 32 of the
+    // work's pages of this warp (lane = place % 32) and the next 32.
+    int w0 = -static_cast<int>(gridDim.x), at = 0, n = 1, kt = -1, page0 = 0, last = 0;
+    int32_t ids = -1, ids2 = -1;
+    const int32_t* pt_row = nullptr;
+    const uint8_t* head = nullptr;
+    auto read_ids = [&](int place) -> int32_t {
+      const int pg = page0 + place / C::kConvPages * kTilePages + place % C::kConvPages;
+      if (place >= n || pg >= last) return -1;
+      const int32_t id = pt_row[pg];
+      if (id >= 0 && id < a.n_pages) return id;
+      flag_error(a.err, kErrPageId);
+      return -1;
+    };
+    auto read_next = [&](uint4 (&x)[kRaw], float2& sc, int& m) {
+      m = -1;
+      if (n == 0) return;
+      if (++at >= n) {
+        at = n = 0;
+        while (n == 0) {
+          w0 += gridDim.x;
+          if (w0 >= a.n_works) return;
+          const Work wk = decode_work(a, work_of(w0, a.n_works));
+          if (!wk.valid) continue;
+          n = (wk.t1 - wk.t0) * C::kConvPages, pt_row = wk.pt_row;
+          head = a.pool + int64_t(wk.kvh) * C::kBlock;
+          page0 = wk.t0 * kTilePages + cw * C::kConvPages, last = min(wk.n_item_pages, wk.t1 * kTilePages);
         }
-      } else {  // values: dims 8j + g (j = 0..3) of tokens 2t, 2t+1, 2t+8, 2t+9 a step, 8 bytes to each dim's row
+        ids = read_ids(lane);
+        ids2 = read_ids(32 + lane);
+      } else if ((at & 31) == 0) {
+        ids = ids2;
+        ids2 = read_ids(at + 32 + lane);
+      }
+      const int step = at % C::kConvPages;
+      if (step == 0) ++kt;
+      m = kt * 4 + step;
+      const int32_t id = __shfl_sync(0xffffffffu, ids, at & 31);
+      sc = make_float2(0.f, 0.f);
+      if (id < 0) {  // no such page: codes of 0
+        constexpr uint32_t zero = to_word<KIND>(0u);
 #pragma unroll
-        for (int i = 0; i < kRaw; ++i) {
-          const int g = lane >> 2, t = lane & 3;
-          const uint4 x = raw[part * kRaw + i];
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        for (int k = 0; k < kRaw; ++k) x[k] = make_uint4(zero, zero, zero, zero);
+        return;
+      }
+      const uint8_t* blk = head + int64_t(id) * pg_bytes;
+      const uint4* src = reinterpret_cast<const uint4*>(blk) + lane;
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj) {
-            uint2 y = make_uint2(0u, 0u);
-            if (there) widen4<KIND>(w[jj], y.x, y.y);
-            *reinterpret_cast<uint2*>(sV(s) + swz128(32 * i + 8 * jj + g, 2 * b + (t >> 1)) + 8 * (t & 1)) = y;
-          }
+      for (int k = 0; k < kRaw; ++k) x[k] = __ldg(src + 32 * k);
+      sc = __ldg(reinterpret_cast<const float2*>(blk + scale_off(D)));
+    };
+    // A page's codes as operands; false after a wait that gave up.
+    auto write = [&](const uint4 (&x)[kRaw], float2 sc, int m) -> bool {
+      const int tile = m >> 2, st = m & 3, s = tile % ST, b = cw * C::kConvPages + st;  // b: page of the tile
+      if (st == 0 && tile >= ST && !warp_wait(&bars[C::kBarKVEmpty + s], ((tile / ST) & 1) ^ 1, a.err)) return false;
+      // keys: 16 dims of a token a piece, to its row's chunks 2c and 2c + 1
+#pragma unroll
+      for (int k = 0; k < kRaw / 2; ++k) {
+        const int u = k * 32 + lane, sb = u >> 6, tok = (u >> 2) & 15, ch = u & 3, row = b * kPage + tok;
+        uint4 y0, y1;
+        widen4_key<KIND, BF16>(x[k].x, y0.x, y0.y);
+        widen4_key<KIND, BF16>(x[k].y, y0.z, y0.w);
+        widen4_key<KIND, BF16>(x[k].z, y1.x, y1.y);
+        widen4_key<KIND, BF16>(x[k].w, y1.z, y1.w);
+        uint8_t* dst = sK(s) + sb * (kBN * 128);
+        *reinterpret_cast<uint4*>(dst + swz128(row, 2 * ch)) = y0;
+        *reinterpret_cast<uint4*>(dst + swz128(row, 2 * ch + 1)) = y1;
+      }
+      // values: dims 8j + g (j = 0..3) of tokens 2t, 2t+1, 2t+8, 2t+9 a piece, 8 bytes to each dim's row
+#pragma unroll
+      for (int k = 0; k < kRaw / 2; ++k) {
+        const int g = lane >> 2, t = lane & 3;
+        const uint32_t w[4] = {x[kRaw / 2 + k].x, x[kRaw / 2 + k].y, x[kRaw / 2 + k].z, x[kRaw / 2 + k].w};
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          uint2 y;
+          widen4<KIND>(w[jj], y.x, y.y);
+          *reinterpret_cast<uint2*>(sV(s) + swz128(32 * k + 8 * jj + g, 2 * b + (t >> 1)) + 8 * (t & 1)) = y;
         }
       }
-      if (lane == 0) {
-        // a scale of 0 comes with codes of 0: any other scale gives the same
-        const float x = fmaxf(scale[part], 1e-34f);
-        float* sc = reinterpret_cast<float*>(&scales[s * kTilePages + b]);
-        if (conv_half + h == 0) sc[0] = x * (unit<KIND>() * a.scale_log2);
-        else sc[1] = log2f(x), sc[2] = 1.f / x;
+      // a scale of 0 comes with codes of 0: any other scale gives the same
+      const float ks = fmaxf(sc.x, 1e-34f), vs = fmaxf(sc.y, 1e-34f);
+      const float4 out = make_float4(ks * (unit<KIND>() * a.scale_log2), __log2f(vs), __fdividef(1.f, vs), 0.f);
+      if (lane == 0) scales[s * kTilePages + b] = out;
+      if (st == C::kConvPages - 1) {
+        fence_proxy_async_smem();  // the operands, for the tensor core
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[C::kBarKVFull + s]);
       }
-    }
-    fence_proxy_async_smem();  // the operands, for the tensor core
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars[C::kBarKVFull + s]);
-    return true;
-  };
-  Conv cv{};
-  cv.w0 = -static_cast<int>(gridDim.x);
-
-  if (C::kOwnConv && warp >= C::kWarpConv && warp < C::kWarpMma) {
-    // ================= converters: a tile's codes are read while the one before is stored
-    uint4 raw[2][kParts * kRaw];
-    float scale[2][kParts];
-    conv_next(cv);
-    Conv cur = cv;
-    if (cv.n) conv_read(cur, raw[0], scale[0]);
-    for (bool ok = true; ok && cur.n;) {
+      return true;
+    };
 #pragma unroll
-      for (int h = 0; h < 2 && ok && cur.n; ++h) {
-        conv_next(cv);
-        ++cv.kt;
-        if (cv.n) conv_read(cv, raw[h ^ 1], scale[h ^ 1]);
-        ok = conv_write(cur, raw[h], scale[h]);
-        cur = cv;
+    for (int i = 0; i < kA; ++i) read_next(raw[i], scale[i], meta[i]);
+    for (bool run = true; run;) {
+#pragma unroll
+      for (int h = 0; h < NB; ++h) {
+        if (meta[h] < 0) run = false;
+        if (!run) break;
+        read_next(raw[(h + kA) % NB], scale[(h + kA) % NB], meta[(h + kA) % NB]);
+        run = write(raw[h], scale[h], meta[h]);
       }
     }
   } else if (warp == C::kWarpMma) {
@@ -353,7 +341,7 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       auto next_work = [&](int& w0) -> Work {  // the next work of this CTA that has tiles
         Work wk{};
         for (wk.valid = false; w0 < a.n_works; w0 += gridDim.x) {
-          wk = decode_work<NH>(a, work_of(w0, a.n_works));
+          wk = decode_work(a, work_of(w0, a.n_works));
           if (wk.valid && wk.t0 < wk.t1) break;
           wk.valid = false;
         }
@@ -442,40 +430,12 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
     const uint32_t tO = tmem + C::col_o(g) + lane_off;
     int h_tiles = 0, h_works = 0, kt = 0;
     bool ok = true;
-    // D = 64: converts the tile two ahead of the one whose P was just handed over (its page id was read a tile before).
-    // The cursor is kept in shared memory: its registers are the softmax's between two calls.
-    Conv* my_cv = reinterpret_cast<Conv*>(smem + C::kOffConv + cw * 48);
-    static_assert(sizeof(Conv) <= 48, "a converter's cursor");
-    auto convert_ahead = [&]() -> bool {
-      if constexpr (C::kOwnConv) return true;
-      Conv c = *my_cv;
-      if (c.n == 0) return true;
-      uint4 raw[kParts * kRaw];
-      float scale[kParts];
-      conv_read(c, raw, scale);
-      Conv nx = c;
-      conv_next(nx);  // (its page id is on its way while the codes are)
-      ++nx.kt;
-      const bool fine = conv_write(c, raw, scale);
-      if (lane == 0) *my_cv = nx;
-      __syncwarp();
-      return fine;
-    };
-    if constexpr (!C::kOwnConv) {
-      conv_next(cv);
-      if (lane == 0) *my_cv = cv;
-      __syncwarp();
-      ok = convert_ahead() && convert_ahead();
-    }
     for (int w0 = 0; w0 < a.n_works && ok; w0 += gridDim.x) {
-      const Work wk = decode_work<NH>(a, work_of(w0, a.n_works));
+      const Work wk = decode_work(a, work_of(w0, a.n_works));
       if (!wk.valid) continue;
       const int n = wk.t1 - wk.t0, kt0 = kt;
       kt += n;
-      if (g >= wk.n_g) {  // no second head in this work: its warps still convert
-        for (int j = 0; j < n && ok; ++j) ok = convert_ahead();
-        continue;
-      }
+      if (g >= wk.n_g) continue;
       const int qpos = wk.pos0 + wk.m0 + r;
       const int64_t orow = (int64_t(wk.qs) + wk.m0 + r) * a.n_heads + wk.head0 + g;
       const bool live = wk.m0 + r < wk.qlen;
@@ -566,8 +526,6 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
         tc_wait_st();
         tc_fence_before();
         mbar_arrive(bar_p(g, buf));
-        ok = convert_ahead();
-        if (!ok) break;
       }
       if (!ok) break;
       // ---- epilogue: O_g out of TMEM, normalised and stored; then the next work's first PV may overwrite it
@@ -655,49 +613,42 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const float* __r
   }
 }
 
-template <int D, int HEADS, int KIND, bool BF16>
+template <int D, int KIND, bool BF16>
 void launch_t(cudaStream_t st, const CUtensorMap& qmap, const PrefillArgs& a, int grid) {
-  using C = PCfg<D, HEADS>;
+  using C = PCfg<D>;
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   const uint64_t bit = uint64_t(1) << (dev & 63);
   if (!(configured.load() & bit)) {
-    check_cuda(cudaFuncSetAttribute(kv8_prefill_kernel<D, HEADS, KIND, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    check_cuda(cudaFuncSetAttribute(kv8_prefill_kernel<D, KIND, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     C::kSmemBytes),
                "kv8 prefill smem attribute");
     configured.fetch_or(bit);
   }
-  kv8_prefill_kernel<D, HEADS, KIND, BF16><<<grid, C::kThreads, C::kSmemBytes, st>>>(qmap, a);
+  kv8_prefill_kernel<D, KIND, BF16><<<grid, C::kThreads, C::kSmemBytes, st>>>(qmap, a);
 }
 
-template <int D, int HEADS>
+template <int D>
 void launch_d(cudaStream_t st, int kind, bool bf16, const CUtensorMap& qmap, const PrefillArgs& a, int grid) {
   if (kind == NBL_I8) {
-    if (bf16) launch_t<D, HEADS, NBL_I8, true>(st, qmap, a, grid);
-    else launch_t<D, HEADS, NBL_I8, false>(st, qmap, a, grid);
+    if (bf16) launch_t<D, NBL_I8, true>(st, qmap, a, grid);
+    else launch_t<D, NBL_I8, false>(st, qmap, a, grid);
   } else {
-    if (bf16) launch_t<D, HEADS, NBL_E4M3, true>(st, qmap, a, grid);
-    else launch_t<D, HEADS, NBL_E4M3, false>(st, qmap, a, grid);
+    if (bf16) launch_t<D, NBL_E4M3, true>(st, qmap, a, grid);
+    else launch_t<D, NBL_E4M3, false>(st, qmap, a, grid);
   }
 }
 
-}  // namespace
-
-namespace {
-// Heads of a CTA: four at D = 64 (one CTA per SM, each converted tile serves four heads), but two where a group has no more
-// (two CTAs per SM; with four, MHA would leave three of the softmax chains idle). D = 128: two fill TMEM.
-int heads_of(int d, int group) { return d == 64 && group > 2 ? 4 : 2; }
 }  // namespace
 
 Kv8PrefillPlan plan_kv8_prefill(const nbl_kv* kv, int n_items, int max_len, int64_t n_rows, int n_heads, int max_kv,
                                 int num_sms) {
   Kv8PrefillPlan p;
   const int group = n_heads / kv->cfg.n_kv_heads;
-  const int heads = heads_of(kv->cfg.head_dim, group);
   const int64_t m_tiles = (max_len + kBM - 1) / kBM;
-  const int64_t pairs = int64_t(n_items) * kv->cfg.n_kv_heads * ((group + heads - 1) / heads) * m_tiles;
-  const int64_t slots = int64_t(num_sms) * (kv->cfg.head_dim == 64 && heads == 2 ? PCfg<64, 2>::kCtas : 1);
+  const int64_t pairs = int64_t(n_items) * kv->cfg.n_kv_heads * ((group + 1) / 2) * m_tiles;
+  const int64_t slots = int64_t(num_sms) * (kv->cfg.head_dim == 64 ? PCfg<64>::kCtas : PCfg<128>::kCtas);
   // Fewer works than CTAs: split the keys, each stretch at least 8 tiles.
   int64_t splits = 1;
   if (pairs < slots) splits = std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(pairs, 1), max_kv / (8 * kBN)));
@@ -733,15 +684,13 @@ void launch_kv8_prefill(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items
   a.n_heads = n_heads;
   a.n_kv_heads = c.n_kv_heads;
   a.group = n_heads / c.n_kv_heads;
-  const int heads = heads_of(d, a.group);
-  a.n_hgroups = (a.group + heads - 1) / heads;
+  a.n_hgroups = (a.group + 1) / 2;
   a.m_tiles = (items.max_len + kBM - 1) / kBM;
   a.n_splits = plan.n_splits;
   a.n_works = plan.n_works;
   a.scale_log2 = 1.4426950408889634f / std::sqrt(static_cast<float>(d));
-  if (d == 128) launch_d<128, 2>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
-  else if (heads == 4) launch_d<64, 4>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
-  else launch_d<64, 2>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
+  if (d == 64) launch_d<64>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
+  else launch_d<128>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
   check_cuda(cudaGetLastError(), "kv8 prefill launch");
   if (plan.n_splits > 1) {
     const int64_t units = int64_t(items.max_len) * n_heads * (d / 4);
