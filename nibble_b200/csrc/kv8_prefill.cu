@@ -43,17 +43,18 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: p may reach 2^8 before
 constexpr float kPShift = 6.0f;            // p' carries 2^6
 constexpr float kMinLv = -24.0f;           // smallest log2(s_v / vref) kept: below it a block adds nothing to fp16 weights
 
-template <int D>
+template <int D, int HEADS>
 struct PCfg {
-  static constexpr int NH = 2;                          // heads of a CTA
-  static constexpr int kCtas = D == 64 ? 2 : 1;         // per SM
+  static constexpr int NH = HEADS;                      // heads of a CTA
+  static constexpr int kCtas = D == 64 && NH == 2 ? 2 : 1;  // per SM
   static constexpr int SB = D == 64 ? 1 : 2;            // S buffers of a head
   static constexpr int ST = 3;                          // tiles of K and V operands
-  static constexpr int kConv = D == 64 ? 1 : 4;         // converting warps
+  static constexpr int kConv = D == 128 ? 4 : NH / 2;   // converting warps
   static constexpr int kConvPages = kTilePages / kConv; // pages of a tile that one of them converts
   static constexpr int kAhead = D == 64 ? 2 : 1;        // pages whose codes are on their way
+  static constexpr int kMma = NH / 2;                   // issuing warps, two heads each
   static constexpr int kWarpConv = 4 * NH, kWarpMma = kWarpConv + kConv;
-  static constexpr int kThreads = (kWarpMma + 1) * 32;
+  static constexpr int kThreads = (kWarpMma + kMma) * 32;
   static constexpr int kQBytes = kBM * D * 2;           // one head's Q tile: D / 64 parts of [128][64]
   static constexpr int kTileBytes = kBN * D * 2;        // K (or V) operand tile
   static constexpr int kBlock = block_bytes(D);
@@ -93,6 +94,7 @@ struct Work {
 // Work w (-1: none); the same in every warp. Works are numbered with the query tile (latest, so heaviest, first) slowest,
 // then the split, the item, the KV head and the head pair: the works of a round are about equally long, whatever the
 // number of items (with the item slowest, 4 prompts of 2048 tokens left the busiest CTA with 1.6 times the mean).
+template <int NH>
 __device__ __forceinline__ Work decode_work(const PrefillArgs& a, int w) {
   Work k{};
   k.valid = false;
@@ -105,8 +107,8 @@ __device__ __forceinline__ Work decode_work(const PrefillArgs& a, int w) {
   w /= a.it.n_items;
   k.split = w % a.n_splits;
   const int mt = a.m_tiles - 1 - w / a.n_splits;
-  k.n_g = min(2, a.group - 2 * hg);  // an odd group leaves the last pair with one head
-  k.head0 = k.kvh * a.group + 2 * hg;
+  k.n_g = min(NH, a.group - NH * hg);  // the last heads of a group may be fewer
+  k.head0 = k.kvh * a.group + NH * hg;
   k.qlen = a.it.len[item];
   k.pos0 = a.it.pos0[item];
   k.qs = a.it.start[item];
@@ -152,10 +154,10 @@ __device__ __forceinline__ void widen4_key(uint32_t w, uint32_t& lo, uint32_t& h
   }
 }
 
-template <int D, int KIND, bool BF16>
-__global__ void __launch_bounds__(PCfg<D>::kThreads, PCfg<D>::kCtas)
+template <int D, int HEADS, int KIND, bool BF16>
+__global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCtas)
     kv8_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const PrefillArgs a) {
-  using C = PCfg<D>;
+  using C = PCfg<D, HEADS>;
   constexpr int NH = C::NH, SB = C::SB, ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -175,11 +177,11 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, PCfg<D>::kCtas)
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars[C::kBarQFull + b], 1);
-      mbar_init(&bars[C::kBarQFree + b], 1);
+      mbar_init(&bars[C::kBarQFree + b], C::kMma);
     }
     for (int s = 0; s < ST; ++s) {
       mbar_init(&bars[C::kBarKVFull + s], C::kConv);
-      mbar_init(&bars[C::kBarKVEmpty + s], 1);
+      mbar_init(&bars[C::kBarKVEmpty + s], C::kMma);
     }
     for (int g = 0; g < NH; ++g) {
       for (int b = 0; b < SB; ++b) {
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, PCfg<D>::kCtas)
         while (n == 0) {
           w0 += gridDim.x;
           if (w0 >= a.n_works) return;
-          const Work wk = decode_work(a, work_of(w0, a.n_works));
+          const Work wk = decode_work<NH>(a, work_of(w0, a.n_works));
           if (!wk.valid) continue;
           n = (wk.t1 - wk.t0) * C::kConvPages, pt_row = wk.pt_row;
           head = a.pool + int64_t(wk.kvh) * C::kBlock;
@@ -324,10 +326,30 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, PCfg<D>::kCtas)
         run = write(raw[h], scale[h], meta[h]);
       }
     }
-  } else if (warp == C::kWarpMma) {
-    // ================= MMA issuer (one thread)
+  } else if (warp >= C::kWarpMma) {
+    // ================= MMA issuers (one thread each): heads 2 mw and 2 mw + 1
+    const int mw = warp - C::kWarpMma;
     if (lane == 0) {
-      prefetch_tensormap(&qmap);
+      constexpr uint32_t idesc_qk = make_idesc_f16(kBM, kBN, BF16, false, false);
+      constexpr uint32_t idesc_pv = make_idesc_f16(kBM, D, false, false, false);
+      int lw = 0, kt = 0;
+      int h_tiles[2] = {0, 0}, h_works[2] = {0, 0};  // per head: S tiles consumed, works finished
+      // S_g (buffer buf) = Q_g K^T from Q buffer qb and stage s, for head g = 2 mw + i.
+      auto qk = [&](int i, int buf, int qb, int s) {
+        const int g = 2 * mw + i;
+        const uint32_t q_addr = smem_u32(sQ(qb, g)), k_addr = smem_u32(sK(s));
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          tc_mma_ss(tmem + C::col_s(g, buf), make_sdesc(q_addr + (kk >> 2) * (kBM * 128) + (kk & 3) * 32, 16, 1024, 2),
+                    make_sdesc(k_addr + (kk >> 2) * (kBN * 128) + (kk & 3) * 32, 16, 1024, 2), idesc_qk, kk > 0 ? 1u : 0u);
+        tc_commit(bar_s(g, buf));
+      };
+      auto kv_ready = [&](int t) -> bool {
+        if (!mbar_wait(&bars[C::kBarKVFull + t % ST], (t / ST) & 1, a.err)) return false;
+        tc_fence_after();
+        return true;
+      };
+      if (mw == 0) prefetch_tensormap(&qmap);
       // The Q tiles of work wk (the CTA's lw'th) into its buffer.
       auto load_q = [&](const Work& wk, int lw) -> bool {
         const int qb = lw & 1, use = lw >> 1;
@@ -341,58 +363,37 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, PCfg<D>::kCtas)
       auto next_work = [&](int& w0) -> Work {  // the next work of this CTA that has tiles
         Work wk{};
         for (wk.valid = false; w0 < a.n_works; w0 += gridDim.x) {
-          wk = decode_work(a, work_of(w0, a.n_works));
+          wk = decode_work<NH>(a, work_of(w0, a.n_works));
           if (wk.valid && wk.t0 < wk.t1) break;
           wk.valid = false;
         }
         return wk;
       };
-      constexpr uint32_t idesc_qk = make_idesc_f16(kBM, kBN, BF16, false, false);
-      constexpr uint32_t idesc_pv = make_idesc_f16(kBM, D, false, false, false);
-      int lw = 0, kt = 0;
-      int h_tiles[NH], h_works[NH];  // per head: S tiles consumed, works finished
-#pragma unroll
-      for (int g = 0; g < NH; ++g) h_tiles[g] = h_works[g] = 0;
-      // S_g (buffer buf) = Q_g K^T from Q buffer qb and stage s.
-      auto qk = [&](int g, int buf, int qb, int s) {
-        const uint32_t q_addr = smem_u32(sQ(qb, g)), k_addr = smem_u32(sK(s));
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          tc_mma_ss(tmem + C::col_s(g, buf), make_sdesc(q_addr + (kk >> 2) * (kBM * 128) + (kk & 3) * 32, 16, 1024, 2),
-                    make_sdesc(k_addr + (kk >> 2) * (kBN * 128) + (kk & 3) * 32, 16, 1024, 2), idesc_qk, kk > 0 ? 1u : 0u);
-        tc_commit(bar_s(g, buf));
-      };
-      auto kv_ready = [&](int t) -> bool {
-        if (!mbar_wait(&bars[C::kBarKVFull + t % ST], (t / ST) & 1, a.err)) return false;
-        tc_fence_after();
-        return true;
-      };
       bool ok = true;
-      int w0 = 0;
+      int w0 = 0, loaded = 0;  // works whose Q is on its way
       Work wk = next_work(w0);
-      if (wk.valid) ok = load_q(wk, 0);
-      int loaded = 1;  // works whose Q is on its way
+      if (wk.valid && mw == 0) ok = load_q(wk, 0), loaded = 1;
       while (wk.valid && ok) {
         w0 += gridDim.x;
         const Work nextw = next_work(w0);
-        const int qb = lw & 1, n = wk.t1 - wk.t0;
+        const int qb = lw & 1, n = wk.t1 - wk.t0, n_g = min(2, wk.n_g - 2 * mw);  // (none or fewer: this warp only counts along)
         ok = mbar_wait(&bars[C::kBarQFull + qb], (lw >> 1) & 1, a.err) && kv_ready(kt);
         if (!ok) break;
         // S_g(0) may overwrite columns that an earlier PV_g reads P from: MMAs run in issue order.
-        for (int g = 0; g < wk.n_g; ++g) qk(g, h_tiles[g] % SB, qb, kt % ST);
+        for (int i = 0; i < n_g; ++i) qk(i, h_tiles[i] % SB, qb, kt % ST);
         for (int j = 0; j < n && ok; ++j, ++kt) {
           const bool more = j + 1 < n;
           if (more) ok = kv_ready(kt + 1);
           if (SB == 2 && more && ok)  // the next S during this tile's softmax
-            for (int g = 0; g < wk.n_g; ++g) qk(g, (h_tiles[g] + 1) % SB, qb, (kt + 1) % ST);
-          for (int g = 0; g < wk.n_g && ok; ++g) {
+            for (int i = 0; i < n_g; ++i) qk(i, (h_tiles[i] + 1) % SB, qb, (kt + 1) % ST);
+          for (int i = 0; i < n_g && ok; ++i) {
             // O_g += P_g V once head g's softmax has written P_g; the work's first PV overwrites O_g, so it also
             // waits for the epilogue of the work before to have read it.
-            const int buf = h_tiles[g] % SB;
-            if (j == 0 && h_works[g] > 0) ok = mbar_wait(&bars[C::kBarODrained + g], (h_works[g] - 1) & 1, a.err);
-            if (ok) ok = mbar_wait(bar_p(g, buf), (h_tiles[g] / SB) & 1, a.err);
+            const int g = 2 * mw + i, buf = h_tiles[i] % SB;
+            if (j == 0 && h_works[i] > 0) ok = mbar_wait(&bars[C::kBarODrained + g], (h_works[i] - 1) & 1, a.err);
+            if (ok) ok = mbar_wait(bar_p(g, buf), (h_tiles[i] / SB) & 1, a.err);
             if (!ok) break;
-            ++h_tiles[g];
+            ++h_tiles[i];
             tc_fence_after();
             const uint32_t v_addr = smem_u32(sV(kt % ST));
 #pragma unroll
@@ -400,20 +401,20 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, PCfg<D>::kCtas)
               tc_mma_ts(tmem + C::col_o(g), tmem + C::col_s(g, buf) + kk * 8, make_sdesc(v_addr + kk * 32, 16, 1024, 2),
                         idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
             if (SB == 2) tc_commit(&bars[C::kBarPV + g]);
-            if (SB == 1 && more) qk(g, 0, qb, (kt + 1) % ST);
+            if (SB == 1 && more) qk(i, 0, qb, (kt + 1) % ST);
           }
           tc_commit(&bars[C::kBarKVEmpty + kt % ST]);  // K and V of this stage are consumed
           // the next work's Q, once the work before this one is done with the buffer (its last MMAs are issued)
-          if (j == 0 && ok && nextw.valid) {
+          if (j == 0 && ok && mw == 0 && nextw.valid) {
             ok = load_q(nextw, lw + 1);
             loaded = lw + 2;
           }
         }
         if (!ok) break;
         tc_commit(&bars[C::kBarQFree + qb]);  // every QK of this work has read its Q tiles
-        for (int g = 0; g < wk.n_g; ++g) {
-          tc_commit(&bars[C::kBarODone + g]);
-          ++h_works[g];
+        for (int i = 0; i < n_g; ++i) {
+          tc_commit(&bars[C::kBarODone + 2 * mw + i]);
+          ++h_works[i];
         }
         ++lw;
         wk = nextw;
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, PCfg<D>::kCtas)
     int h_tiles = 0, h_works = 0, kt = 0;
     bool ok = true;
     for (int w0 = 0; w0 < a.n_works && ok; w0 += gridDim.x) {
-      const Work wk = decode_work(a, work_of(w0, a.n_works));
+      const Work wk = decode_work<NH>(a, work_of(w0, a.n_works));
       if (!wk.valid) continue;
       const int n = wk.t1 - wk.t0, kt0 = kt;
       kt += n;
@@ -613,33 +614,40 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const float* __r
   }
 }
 
-template <int D, int KIND, bool BF16>
+template <int D, int HEADS, int KIND, bool BF16>
 void launch_t(cudaStream_t st, const CUtensorMap& qmap, const PrefillArgs& a, int grid) {
-  using C = PCfg<D>;
+  using C = PCfg<D, HEADS>;
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   const uint64_t bit = uint64_t(1) << (dev & 63);
   if (!(configured.load() & bit)) {
-    check_cuda(cudaFuncSetAttribute(kv8_prefill_kernel<D, KIND, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    check_cuda(cudaFuncSetAttribute(kv8_prefill_kernel<D, HEADS, KIND, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     C::kSmemBytes),
                "kv8 prefill smem attribute");
     configured.fetch_or(bit);
   }
-  kv8_prefill_kernel<D, KIND, BF16><<<grid, C::kThreads, C::kSmemBytes, st>>>(qmap, a);
+  kv8_prefill_kernel<D, HEADS, KIND, BF16><<<grid, C::kThreads, C::kSmemBytes, st>>>(qmap, a);
 }
 
-template <int D>
+template <int D, int HEADS>
 void launch_d(cudaStream_t st, int kind, bool bf16, const CUtensorMap& qmap, const PrefillArgs& a, int grid) {
   if (kind == NBL_I8) {
-    if (bf16) launch_t<D, NBL_I8, true>(st, qmap, a, grid);
-    else launch_t<D, NBL_I8, false>(st, qmap, a, grid);
+    if (bf16) launch_t<D, HEADS, NBL_I8, true>(st, qmap, a, grid);
+    else launch_t<D, HEADS, NBL_I8, false>(st, qmap, a, grid);
   } else {
-    if (bf16) launch_t<D, NBL_E4M3, true>(st, qmap, a, grid);
-    else launch_t<D, NBL_E4M3, false>(st, qmap, a, grid);
+    if (bf16) launch_t<D, HEADS, NBL_E4M3, true>(st, qmap, a, grid);
+    else launch_t<D, HEADS, NBL_E4M3, false>(st, qmap, a, grid);
   }
 }
 
+}  // namespace
+
+namespace {
+// Heads of a CTA: four at D = 64 where a group has three or more (one CTA per SM: each converted tile serves four heads),
+// two otherwise (D = 64: two CTAs per SM, so that with small groups four softmax chains still run on an SM; D = 128: two
+// fill TMEM).
+int heads_of(int d, int group) { return d == 64 && group > 2 ? 4 : 2; }
 }  // namespace
 
 Kv8PrefillPlan plan_kv8_prefill(const nbl_kv* kv, int n_items, int max_len, int64_t n_rows, int n_heads, int max_kv,
@@ -647,8 +655,9 @@ Kv8PrefillPlan plan_kv8_prefill(const nbl_kv* kv, int n_items, int max_len, int6
   Kv8PrefillPlan p;
   const int group = n_heads / kv->cfg.n_kv_heads;
   const int64_t m_tiles = (max_len + kBM - 1) / kBM;
-  const int64_t pairs = int64_t(n_items) * kv->cfg.n_kv_heads * ((group + 1) / 2) * m_tiles;
-  const int64_t slots = int64_t(num_sms) * (kv->cfg.head_dim == 64 ? PCfg<64>::kCtas : PCfg<128>::kCtas);
+  const int heads = heads_of(kv->cfg.head_dim, group);
+  const int64_t pairs = int64_t(n_items) * kv->cfg.n_kv_heads * ((group + heads - 1) / heads) * m_tiles;
+  const int64_t slots = int64_t(num_sms) * (kv->cfg.head_dim == 64 && heads == 2 ? 2 : 1);
   // Fewer works than CTAs: split the keys, each stretch at least 8 tiles.
   int64_t splits = 1;
   if (pairs < slots) splits = std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(pairs, 1), max_kv / (8 * kBN)));
@@ -684,13 +693,15 @@ void launch_kv8_prefill(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items
   a.n_heads = n_heads;
   a.n_kv_heads = c.n_kv_heads;
   a.group = n_heads / c.n_kv_heads;
-  a.n_hgroups = (a.group + 1) / 2;
+  const int heads = heads_of(d, a.group);
+  a.n_hgroups = (a.group + heads - 1) / heads;
   a.m_tiles = (items.max_len + kBM - 1) / kBM;
   a.n_splits = plan.n_splits;
   a.n_works = plan.n_works;
   a.scale_log2 = 1.4426950408889634f / std::sqrt(static_cast<float>(d));
-  if (d == 64) launch_d<64>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
-  else launch_d<128>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
+  if (d == 128) launch_d<128, 2>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
+  else if (heads == 4) launch_d<64, 4>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
+  else launch_d<64, 2>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
   check_cuda(cudaGetLastError(), "kv8 prefill launch");
   if (plan.n_splits > 1) {
     const int64_t units = int64_t(items.max_len) * n_heads * (d / 4);
