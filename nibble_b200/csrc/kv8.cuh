@@ -43,10 +43,6 @@ __device__ __forceinline__ int key_off(int tok, int dim) { return (dim >> 6) * 1
 __device__ __forceinline__ int value_off(int d, int t, int dim) {
   return kPage * d + (dim >> 5) * 512 + ((dim & 7) * 4 + t) * 16 + ((dim >> 3) & 3) * 4;
 }
-// Where a token's code stands: t of its word, and its place there.
-__device__ __forceinline__ int value_t(int tok) { return (tok & 7) >> 1; }
-__device__ __forceinline__ int value_i(int tok) { return (tok & 1) + 2 * (tok >> 3); }
-
 // KIND: NBL_I8 or NBL_E4M3.
 template <int KIND>
 __host__ __device__ constexpr float code_max() {

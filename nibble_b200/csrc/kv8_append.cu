@@ -16,27 +16,231 @@ namespace {
 
 using namespace kv8;
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128;  // import / export
 
-// Element indices of rotation pair p of a head (p < rotary_dim / 2), or of the p-th pair of untouched elements.
-__device__ __forceinline__ void pair_of(int p, int rd, bool neox, int& e0, int& e1) {
-  const int half = rd / 2;
-  if (p < half) {
-    e0 = neox ? p : 2 * p;
-    e1 = neox ? p + half : 2 * p + 1;
+// Threads of an append or read CTA, which has one (page, KV head): 8 dims (chunk c) of one token each. Warp w has the tokens
+// 2t, 2t + 1, 2t + 8, 2t + 9 with t = w % 4 (lane / 8 = place i among them), the four that share a value word, and
+// chunks 8 (w / 4) + lane % 8.
+template <int D>
+constexpr int kCtaThreads = kPage * D / 8;
+struct Place {
+  int t, i, tok, c;
+};
+__device__ __forceinline__ Place place_of(int thread) {
+  const int warp = thread >> 5, lane = thread & 31;
+  Place p;
+  p.t = warp & 3, p.i = lane >> 3;
+  p.tok = 2 * p.t + (p.i & 1) + 8 * (p.i >> 1);
+  p.c = (warp >> 2) * 8 + (lane & 7);
+  return p;
+}
+// The four lanes of a value word (lane bits 3 and 4) exchange bytes: lane i's byte k becomes lane k's byte i.
+__device__ __forceinline__ uint32_t transpose4(uint32_t w, int i) {
+  uint32_t x = __shfl_xor_sync(0xffffffffu, w, 8);
+  w = __byte_perm(w, x, i & 1 ? 0x3715 : 0x6240);
+  x = __shfl_xor_sync(0xffffffffu, w, 16);
+  return __byte_perm(w, x, i & 2 ? 0x3276 : 0x5410);
+}
+
+// Eight consecutive elements of a float type as fp32, and back; 16-byte aligned.
+__device__ __forceinline__ void load8v(const void* p, int64_t i, int dtype, float (&v)[8]) {
+  if (dtype == NBL_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   } else {
-    e0 = rd + 2 * (p - half);
-    e1 = e0 + 1;
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = dtype == NBL_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k]))
+                                        : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+      v[2 * k] = f.x, v[2 * k + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ void store8v(void* p, int64_t i, int dtype, const float (&v)[8]) {
+  if (dtype == NBL_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (dtype == NBL_F16) {
+        const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void load8(const void* p, int64_t i, int dtype, float (&v)[8]) {
+  if constexpr (VEC) {
+    load8v(p, i, dtype, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = load_as(p, i + k, dtype);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const float (&v)[8]) {
+  if constexpr (VEC) {
+    store8v(p, i, dtype, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) store_as(p, i + k, v[k], dtype);
+  }
+}
+__device__ __forceinline__ void add8(float (&v)[8], const float* b) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = __fadd_rn(v[k], b[k]);
+}
+
+// A chunk of a head with bias, rotated: element e and its partner (e ^ 1, or half the rotated part away) turn by the angle
+// of their pair. cs[k]: (cos, sin) for element 8c + k. VEC: the chunk, and its partner chunk where the partners are
+// elsewhere, are whole and 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ void rotated8(const void* src, int64_t row, int c, int dtype, const float* bias, bool neox, int rd,
+                                         const float2 (&cs)[8], float (&v)[8]) {
+  const int e0 = 8 * c, half = rd / 2;
+  load8<VEC>(src, row + e0, dtype, v);
+  if (bias) add8(v, bias + e0);
+  if (e0 >= rd) return;
+  float other[8];
+  if (!neox) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) other[k] = v[k ^ 1];
+  } else if (VEC) {
+    const int o0 = e0 < half ? e0 + half : e0 - half;
+    load8v(src, row + o0, dtype, other);
+    if (bias) add8(other, bias + o0);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int e = e0 + k, o = e < half ? e + half : e - half;
+      other[k] = 0.f;
+      if (e >= rd) continue;
+      other[k] = load_as(src, row + o, dtype);
+      if (bias) other[k] = __fadd_rn(other[k], bias[o]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int e = e0 + k;
+    if (!VEC && e >= rd) continue;
+    const bool first = neox ? e < half : (k & 1) == 0;
+    float ra, rb;
+    rope_rotate(first ? v[k] : other[k], first ? other[k] : v[k], cs[k], ra, rb);
+    other[k] = first ? ra : rb;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (VEC || e0 + k < rd) v[k] = other[k];
+}
+
+// Four consecutive elements as fp32, and back; VEC: 8- (16-bit types) or 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ void load4(const void* p, int64_t i, int dtype, float* v) {
+  if (!VEC) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = load_as(p, i + k, dtype);
+  } else if (dtype == NBL_F32) {
+    const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t w[2] = {x.x, x.y};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float2 f = dtype == NBL_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k]))
+                                        : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+      v[2 * k] = f.x, v[2 * k + 1] = f.y;
+    }
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store4(void* p, int64_t i, int dtype, const float* v) {
+  if (!VEC) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) store_as(p, i + k, v[k], dtype);
+  } else if (dtype == NBL_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    uint32_t w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (dtype == NBL_F16) {
+        const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(w[0], w[1]);
   }
 }
 
-// One CTA per (touched page of an item, KV head): the page's new tokens' keys and values, and the query heads of that
-// KV head for those tokens.
-template <int D, int KIND>
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const Kv8Items it, const Kv8Append a, uint8_t* pool,
-                                                              int64_t n_pages, int n_kv_heads, int max_blocks, int* err) {
-  __shared__ float xs[2][kPage][D + 1];
-  __shared__ float red[2][kThreads / 32];
+// Pairs 4c .. 4c + 3 of a query head: both elements of a pair are this thread's, so the rotation may be in place. The
+// first rd / 2 pairs are the rotated ones, the others the untouched elements two by two. cs[k]: (cos, sin) of pair 4c + k.
+template <bool VEC>
+__device__ __forceinline__ void query8(const void* src, void* dst, int64_t row, int c, int in_dtype, int out_dtype,
+                                       const float* bias, bool neox, int rd, const float2 (&cs)[4]) {
+  float v[8];
+  const int half = rd / 2;
+  if (VEC) {  // rd is a multiple of 8: a chunk is rotated whole or not at all
+    const bool split = neox && 8 * c < rd;
+    const int lo = split ? 4 * c : 8 * c, hi = split ? half + 4 * c : 8 * c + 4;
+    if (split) {
+      load4<true>(src, row + lo, in_dtype, v);
+      load4<true>(src, row + hi, in_dtype, v + 4);
+    } else {
+      load8v(src, row + lo, in_dtype, v);
+    }
+    if (bias) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = __fadd_rn(v[k], bias[lo + k]), v[4 + k] = __fadd_rn(v[4 + k], bias[hi + k]);
+    }
+    if (split) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) rope_rotate(v[k], v[4 + k], cs[k], v[k], v[4 + k]);
+      store4<true>(dst, row + lo, out_dtype, v);
+      store4<true>(dst, row + hi, out_dtype, v + 4);
+    } else {
+      if (8 * c < rd) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rope_rotate(v[2 * k], v[2 * k + 1], cs[k], v[2 * k], v[2 * k + 1]);
+      }
+      store8v(dst, row + lo, out_dtype, v);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int p = 4 * c + k;
+      const bool turn = p < half;
+      const int e0 = turn ? (neox ? p : 2 * p) : rd + 2 * (p - half), e1 = turn && neox ? p + half : e0 + 1;
+      float x = load_as(src, row + e0, in_dtype), y = load_as(src, row + e1, in_dtype);
+      if (bias) x = __fadd_rn(x, bias[e0]), y = __fadd_rn(y, bias[e1]);
+      if (turn) rope_rotate(x, y, cs[k], x, y);
+      store_as(dst, row + e0, x, out_dtype);
+      store_as(dst, row + e1, y, out_dtype);
+    }
+  }
+}
+
+// One CTA per (touched page of an item, KV head): the page's new tokens' keys and values, and the query heads of that KV
+// head for those tokens. Bound: memory (each input once, each output once); the queries' loads cover the latency of the
+// keys' and values' reduction.
+template <int D, int KIND, bool VEC>
+__global__ void __launch_bounds__(kCtaThreads<D>) kv8_append_kernel(const Kv8Items it, const Kv8Append a, uint8_t* pool,
+                                                                    int64_t n_pages, int n_kv_heads, int max_blocks,
+                                                                    int* err) {
+  __shared__ float red[2][kCtaThreads<D> / 32];
   const int item = blockIdx.x / max_blocks, kvh = blockIdx.y;
   const int start = it.start[item], len = it.len[item], pos0 = it.pos0[item];
   if (len <= 0) return;
@@ -47,47 +251,60 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const Kv8Items it,
     return;
   }
   if (block * kPage >= end) return;
-  const int first = static_cast<int>(max(int64_t(pos0), block * kPage));       // positions first .. last
-  const int last = static_cast<int>(min(end, block * kPage + kPage)) - 1;
-  const int n_new = last - first + 1, slot0 = first - static_cast<int>(block) * kPage;
-  const int group = a.n_heads / n_kv_heads, rd = a.rotary_dim, half = rd / 2;
-
-  // queries: rotated straight to q_out
-  for (int u = threadIdx.x; u < n_new * group * (D / 2); u += kThreads) {
-    const int p = u % (D / 2), h = kvh * group + (u / (D / 2)) % group, i = u / (D / 2 * group);
-    const int64_t base = (int64_t(start) + (first - pos0) + i) * a.n_heads * D + int64_t(h) * D;
-    int e0, e1;
-    pair_of(p, rd, a.neox, e0, e1);
-    float x0 = load_as(a.q_in, base + e0, a.in_dtype), x1 = load_as(a.q_in, base + e1, a.in_dtype);
-    if (a.bq) x0 = __fadd_rn(x0, a.bq[h * D + e0]), x1 = __fadd_rn(x1, a.bq[h * D + e1]);
-    if (p < half) rope_rotate(x0, x1, a.tab[int64_t(first + i) * half + p], x0, x1);
-    store_as(a.q_out, base + e0, x0, a.q_out_dtype);
-    store_as(a.q_out, base + e1, x1, a.q_out_dtype);
-  }
   const int32_t page = it.page_table[int64_t(item) * it.pt_stride + block];
-  if (page < 0 || page >= n_pages) {
-    if (threadIdx.x == 0) flag_error(err, kErrPageId);
-    return;
+  const int base = static_cast<int>(block) * kPage;
+  const int slot0 = max(pos0 - base, 0), slot1 = static_cast<int>(min(end - base, int64_t(kPage)));  // the new tokens' places
+  const int group = a.n_heads / n_kv_heads, rd = a.rotary_dim;
+  const bool good = page >= 0 && page < n_pages;
+  if (!good && threadIdx.x == 0) flag_error(err, kErrPageId);
+  uint8_t* blk = pool + int64_t(good ? page : 0) * page_bytes(D, n_kv_heads) + int64_t(kvh) * block_bytes(D);
+  float* sc = reinterpret_cast<float*>(blk + scale_off(D));
+
+  const Place pl = place_of(threadIdx.x);
+  const int c = pl.c, tok = pl.tok;
+  const bool is_new = tok >= slot0 && tok < slot1, is_old = tok < slot0;
+  const int64_t row = int64_t(start) + (base + tok - pos0);  // of the packed activations
+  float k8[8], v8[8];
+  if (is_new) {
+    float2 cs[8];
+    if (8 * c < rd) {
+      const float2* tab = a.tab + int64_t(base + tok) * (rd / 2);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int e = 8 * c + k;
+        if (VEC && !a.neox && (k & 1)) cs[k] = cs[k - 1];
+        else if (VEC || e < rd) cs[k] = tab[a.neox ? (e < rd / 2 ? e : e - rd / 2) : e >> 1];
+      }
+    }
+    load8<VEC>(a.v_in, (row * n_kv_heads + kvh) * D + 8 * c, a.in_dtype, v8);
+    rotated8<VEC>(a.k_in, (row * n_kv_heads + kvh) * D, c, a.in_dtype, a.bk ? a.bk + kvh * D : nullptr, a.neox, rd, cs, k8);
+    if (a.bv) add8(v8, a.bv + kvh * D + 8 * c);
+    const int64_t q0 = (row * a.n_heads + int64_t(kvh) * group) * D;
+    const float* bq = a.bq ? a.bq + kvh * group * D : nullptr;
+    float2 qcs[4];
+    if (4 * c < rd / 2) {
+      const float2* tab = a.tab + int64_t(base + tok) * (rd / 2) + 4 * c;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (VEC || 4 * c + k < rd / 2) qcs[k] = tab[k];
+    }
+#pragma unroll 4
+    for (int h = 0; h < group; ++h)
+      query8<VEC>(a.q_in, a.q_out, q0 + h * D, c, a.in_dtype, a.q_out_dtype, bq ? bq + h * D : nullptr, a.neox, rd, qcs);
   }
-  // keys and values of the new tokens into shared memory, with their largest magnitudes
+  if (!good) return;
+  // largest magnitudes of the new tokens
   float amax[2] = {0.f, 0.f};
   bool odd = false;
-  for (int u = threadIdx.x; u < 2 * n_new * (D / 2); u += kThreads) {
-    const int p = u % (D / 2), i = u / (D / 2) % n_new, w = u / (D / 2 * n_new);
-    const int64_t base = (int64_t(start) + (first - pos0) + i) * n_kv_heads * D + int64_t(kvh) * D;
-    int e0, e1;
-    pair_of(p, rd, a.neox, e0, e1);
-    const void* src = w ? a.v_in : a.k_in;
-    const float* bias = w ? a.bv : a.bk;
-    float x0 = load_as(src, base + e0, a.in_dtype), x1 = load_as(src, base + e1, a.in_dtype);
-    if (bias) x0 = __fadd_rn(x0, bias[kvh * D + e0]), x1 = __fadd_rn(x1, bias[kvh * D + e1]);
-    if (w == 0 && p < half) rope_rotate(x0, x1, a.tab[int64_t(first + i) * half + p], x0, x1);
-    odd = odd || !(fabsf(x0) <= kHuge) || !(fabsf(x1) <= kHuge);
-    x0 = x0 != x0 ? 0.f : fminf(fmaxf(x0, -kHuge), kHuge);
-    x1 = x1 != x1 ? 0.f : fminf(fmaxf(x1, -kHuge), kHuge);
-    xs[w][slot0 + i][e0] = x0;
-    xs[w][slot0 + i][e1] = x1;
-    amax[w] = fmaxf(amax[w], fmaxf(fabsf(x0), fabsf(x1)));
+  if (is_new) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      odd = odd || !(fabsf(k8[k]) <= kHuge) || !(fabsf(v8[k]) <= kHuge);
+      k8[k] = k8[k] != k8[k] ? 0.f : fminf(fmaxf(k8[k], -kHuge), kHuge);
+      v8[k] = v8[k] != v8[k] ? 0.f : fminf(fmaxf(v8[k], -kHuge), kHuge);
+      amax[0] = fmaxf(amax[0], fabsf(k8[k]));
+      amax[1] = fmaxf(amax[1], fabsf(v8[k]));
+    }
   }
   if (odd) flag_error(err, kErrNonFinite);
 #pragma unroll
@@ -96,9 +313,6 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const Kv8Items it,
     for (int o = 16; o > 0; o >>= 1) amax[w] = fmaxf(amax[w], __shfl_xor_sync(0xffffffffu, amax[w], o));
     if ((threadIdx.x & 31) == 0) red[w][threadIdx.x >> 5] = amax[w];
   }
-  uint8_t* pg = pool + int64_t(page) * page_bytes(D, n_kv_heads);
-  uint8_t* blk = pg + int64_t(kvh) * block_bytes(D);
-  float* sc = reinterpret_cast<float*>(blk + scale_off(D));
   float s[2], inv[2], ratio[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) s[w] = slot0 > 0 ? sc[w] : 0.f;  // the scale of the tokens already there
@@ -107,64 +321,59 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const Kv8Items it,
   for (int w = 0; w < 2; ++w) {
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) m = fmaxf(m, red[w][i]);
+    for (int i = 0; i < kCtaThreads<D> / 32; ++i) m = fmaxf(m, red[w][i]);
     const float old = s[w];
     s[w] = fmaxf(old, m >= kTiny ? __fmul_rn(m, 1.f / code_max<KIND>()) : 0.f);
     inv[w] = s[w] > 0.f ? __fdiv_rn(1.f, s[w]) : 0.f;
     ratio[w] = __fmul_rn(old, inv[w]);
   }
-  const int slot1 = slot0 + n_new;
-  // keys: 16 consecutive dims of one token per step
-  for (int u = threadIdx.x; u < kPage * D / 16; u += kThreads) {
-    const int tok = u / (D / 16), d0 = (u % (D / 16)) * 16;
-    uint4* dst = reinterpret_cast<uint4*>(blk + key_off(tok, d0));
-    const uint4 was = tok < slot0 ? *dst : uint4{};
-    const uint32_t o[4] = {was.x, was.y, was.z, was.w};
-    uint32_t w4[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t old = from_word<KIND>(o[k]);
-      w4[k] = 0;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const float x = tok < slot0 ? __fmul_rn(decode<KIND>(old >> (8 * b)), ratio[0])
-                                    : (tok < slot1 ? __fmul_rn(xs[0][tok][d0 + 4 * k + b], inv[0]) : 0.f);
-        w4[k] |= encode<KIND>(x) << (8 * b);
-      }
-      w4[k] = to_word<KIND>(w4[k]);
-    }
-    *dst = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+  // keys: two words of 4 dims; old ones are rounded again to the new scale
+  uint2* kdst = reinterpret_cast<uint2*>(blk + key_off(tok, 8 * c));
+  uint32_t kw[2];
+  if (is_old) {
+    const uint2 was = *kdst;
+    kw[0] = from_word<KIND>(was.x), kw[1] = from_word<KIND>(was.y);
   }
-  // values: dims 8j + g (j = 0..3) of tokens 2t, 2t+1, 2t+8, 2t+9 per step
-  for (int u = threadIdx.x; u < kPage * D / 16; u += kThreads) {
-    const int c = u >> 5, g = (u & 31) >> 2, t = u & 3;
-    uint4* dst = reinterpret_cast<uint4*>(blk + kPage * D + u * 16);
-    const uint4 was = slot0 > 0 ? *dst : uint4{};
-    const uint32_t o[4] = {was.x, was.y, was.z, was.w};
-    uint32_t w4[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t old = from_word<KIND>(o[j]);
-      w4[j] = 0;
+  for (int j = 0; j < 2; ++j) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const float x = is_old ? __fmul_rn(decode<KIND>(kw[j] >> (8 * b)), ratio[0])
+                             : (is_new ? __fmul_rn(k8[4 * j + b], inv[0]) : 0.f);
+      w |= encode<KIND>(x) << (8 * b);
+    }
+    kw[j] = to_word<KIND>(w);
+  }
+  *kdst = make_uint2(kw[0], kw[1]);
+  // values: this token's codes, exchanged among the four lanes of a word, so that lane i has the words of dims 8c + i and
+  // 8c + 4 + i
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) w |= encode<KIND>(is_new ? __fmul_rn(v8[4 * j + b], inv[1]) : 0.f) << (8 * b);
+    w = transpose4(w, pl.i);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(blk + value_off(D, pl.t, 8 * c + 4 * j + pl.i));
+    if (slot0 > 0) {
+      const uint32_t old = from_word<KIND>(*dst);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const int tok = 2 * t + (b & 1) + 8 * (b >> 1), dim = 32 * c + 8 * j + g;
-        const float x = tok < slot0 ? __fmul_rn(decode<KIND>(old >> (8 * b)), ratio[1])
-                                    : (tok < slot1 ? __fmul_rn(xs[1][tok][dim], inv[1]) : 0.f);
-        w4[j] |= encode<KIND>(x) << (8 * b);
+        if (2 * pl.t + (b & 1) + 8 * (b >> 1) >= slot0) continue;
+        const uint32_t x = encode<KIND>(__fmul_rn(decode<KIND>(old >> (8 * b)), ratio[1]));
+        w = (w & ~(0xffu << (8 * b))) | x << (8 * b);
       }
-      w4[j] = to_word<KIND>(w4[j]);
     }
-    *dst = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+    *dst = to_word<KIND>(w);
   }
   if (threadIdx.x < 2) sc[threadIdx.x] = s[threadIdx.x];
 }
 
 // One CTA per (touched page of an item, KV head): its rows as code * scale.
 template <int D, int KIND>
-__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const Kv8Items it, const uint8_t* pool, int64_t n_pages,
-                                                            int n_kv_heads, int max_blocks, void* k_out, void* v_out,
-                                                            int out_dtype, int* err) {
+__global__ void __launch_bounds__(kCtaThreads<D>) kv8_read_kernel(const Kv8Items it, const uint8_t* pool, int64_t n_pages,
+                                                                  int n_kv_heads, int max_blocks, void* k_out, void* v_out,
+                                                                  int out_dtype, bool vec, int* err) {
   const int item = blockIdx.x / max_blocks, kvh = blockIdx.y;
   const int start = it.start[item], len = it.len[item], pos0 = it.pos0[item];
   if (len <= 0) return;
@@ -180,24 +389,32 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const Kv8Items it, c
     if (threadIdx.x == 0) flag_error(err, kErrPageId);
     return;
   }
-  const int first = static_cast<int>(max(int64_t(pos0), block * kPage));
-  const int n = static_cast<int>(min(end, block * kPage + kPage)) - first;
-  const int slot0 = first - static_cast<int>(block) * kPage;
-  const uint8_t* pg = pool + int64_t(page) * page_bytes(D, n_kv_heads);
-  const uint8_t* blk = pg + int64_t(kvh) * block_bytes(D);
-  const float* sc = reinterpret_cast<const float*>(blk + scale_off(D));
-  const float ks = sc[0], vs = sc[1];
-  for (int u = threadIdx.x; u < n * D; u += kThreads) {
-    const int i = u / D, dim = u % D, tok = slot0 + i;
-    const int64_t at = (int64_t(start) + (first - pos0) + i) * n_kv_heads * D + int64_t(kvh) * D + dim;
-    if (k_out) {
-      const uint32_t w = from_word<KIND>(*reinterpret_cast<const uint32_t*>(blk + key_off(tok, dim & ~3)));
-      store_as(k_out, at, __fmul_rn(decode<KIND>(w >> (8 * (dim & 3))), ks), out_dtype);
-    }
-    if (v_out) {
-      const uint32_t w = from_word<KIND>(*reinterpret_cast<const uint32_t*>(blk + value_off(D, value_t(tok), dim)));
-      store_as(v_out, at, __fmul_rn(decode<KIND>(w >> (8 * value_i(tok))), vs), out_dtype);
-    }
+  const int base = static_cast<int>(block) * kPage;
+  const uint8_t* blk = pool + int64_t(page) * page_bytes(D, n_kv_heads) + int64_t(kvh) * block_bytes(D);
+  const float2 sc = *reinterpret_cast<const float2*>(blk + scale_off(D));
+  const Place pl = place_of(threadIdx.x);
+  const uint2 kw = *reinterpret_cast<const uint2*>(blk + key_off(pl.tok, 8 * pl.c));
+  uint32_t vw[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    vw[j] = transpose4(from_word<KIND>(*reinterpret_cast<const uint32_t*>(blk + value_off(D, pl.t, 8 * pl.c + 4 * j + pl.i))),
+                       pl.i);
+  const int pos = base + pl.tok;
+  if (pos < pos0 || pos >= end) return;
+  const int64_t at = ((int64_t(start) + (pos - pos0)) * n_kv_heads + kvh) * D + 8 * pl.c;
+  const uint32_t k2[2] = {from_word<KIND>(kw.x), from_word<KIND>(kw.y)};
+  float k8[8], v8[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    k8[k] = __fmul_rn(decode<KIND>(k2[k >> 2] >> (8 * (k & 3))), sc.x);
+    v8[k] = __fmul_rn(decode<KIND>(vw[k >> 2] >> (8 * (k & 3))), sc.y);
+  }
+  if (vec) {
+    if (k_out) store8v(k_out, at, out_dtype, k8);
+    if (v_out) store8v(v_out, at, out_dtype, v8);
+  } else {
+    if (k_out) store8<false>(k_out, at, out_dtype, k8);
+    if (v_out) store8<false>(v_out, at, out_dtype, v8);
   }
 }
 
@@ -321,9 +538,13 @@ void launch_kv8_append(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items,
   const int blocks = touched_pages(items.max_len);
   grid_check(int64_t(items.n_items) * blocks, "rotary_kv_append");
   const dim3 grid(static_cast<unsigned>(items.n_items) * blocks, static_cast<unsigned>(kv->cfg.n_kv_heads));
+  const auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  const bool vec = ((bits(a.q_in) | bits(a.k_in) | bits(a.v_in) | bits(a.q_out)) & 15u) == 0 &&
+                   a.rotary_dim % (a.neox ? 16 : 8) == 0;
   with_kind(kv, [&](auto d, auto kind) {
-    kv8_append_kernel<d(), kind()><<<grid, kThreads, 0, st>>>(items, a, static_cast<uint8_t*>(kv->pool),
-                                                              kv->cfg.n_pages, kv->cfg.n_kv_heads, blocks, err);
+    auto* k = vec ? kv8_append_kernel<d(), kind(), true> : kv8_append_kernel<d(), kind(), false>;
+    k<<<grid, kCtaThreads<d()>, 0, st>>>(items, a, static_cast<uint8_t*>(kv->pool), kv->cfg.n_pages, kv->cfg.n_kv_heads,
+                                         blocks, err);
   });
   check_cuda(cudaGetLastError(), "rotary_kv_append launch");
 }
@@ -333,10 +554,11 @@ void launch_kv8_read(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, v
   const int blocks = touched_pages(items.max_len);
   grid_check(int64_t(items.n_items) * blocks, "kv_read");
   const dim3 grid(static_cast<unsigned>(items.n_items) * blocks, static_cast<unsigned>(kv->cfg.n_kv_heads));
+  const bool vec = ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u) == 0;
   with_kind(kv, [&](auto d, auto kind) {
-    kv8_read_kernel<d(), kind()><<<grid, kThreads, 0, st>>>(items, static_cast<const uint8_t*>(kv->pool),
-                                                            kv->cfg.n_pages, kv->cfg.n_kv_heads, blocks, k_out, v_out,
-                                                            out_dtype, err);
+    kv8_read_kernel<d(), kind()><<<grid, kCtaThreads<d()>, 0, st>>>(items, static_cast<const uint8_t*>(kv->pool),
+                                                                    kv->cfg.n_pages, kv->cfg.n_kv_heads, blocks, k_out, v_out,
+                                                                    out_dtype, vec, err);
   });
   check_cuda(cudaGetLastError(), "kv_read launch");
 }
