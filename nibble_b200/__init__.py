@@ -60,6 +60,14 @@ class RotarySpec:
     freq_factors: tuple | None = None
 
     def _c(self):
+        """The C struct and the factors that it points to (made once)."""
+        made = self.__dict__.get("_made")
+        if made is None:
+            made = self._make()
+            object.__setattr__(self, "_made", made)
+        return made
+
+    def _make(self):
         if self.scaling not in _abi.ROTARY_SCALING:
             raise ValueError(f"unknown rotary scaling {self.scaling!r} (one of {', '.join(_abi.ROTARY_SCALING)})")
         ff = ptr = None
@@ -91,16 +99,22 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
+_codes: dict = {}  # torch dtype -> element type code
+
+
 def _dtype(t) -> int:
-    name = str(t.dtype).replace("torch.", "")
-    if name not in _DT:
-        raise ValueError(f"unsupported dtype {t.dtype}")
-    return _DT[name]
+    code = _codes.get(t.dtype)
+    if code is None:
+        name = str(t.dtype).replace("torch.", "")
+        if name not in _DT:
+            raise ValueError(f"unsupported dtype {t.dtype}")
+        code = _codes[t.dtype] = _DT[name]
+    return code
 
 
 def _same_shape(kv, q, k, v):
-    if tuple(q.shape[2:]) != (kv.head_dim,) or tuple(k.shape) != (q.shape[0], kv.n_kv_heads, kv.head_dim) \
-            or v.shape != k.shape:
+    want = (q.shape[0], kv.n_kv_heads, kv.head_dim)
+    if q.dim() != 3 or q.shape[2] != kv.head_dim or k.shape != want or v.shape != want:
         raise ValueError(f"expected q [rows, n_heads, {kv.head_dim}] and k, v [rows, {kv.n_kv_heads}, {kv.head_dim}]")
 
 

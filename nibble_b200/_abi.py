@@ -123,9 +123,9 @@ _lib = None
 
 def get_lib() -> C.CDLL:
     """The loaded library (loaded on first use, so the build step can import this package without it)."""
-    global _lib
+    global _lib, lib
     if _lib is None:
-        _lib = _load()
+        _lib = lib = _load()  # (`lib` is a plain name from here on: __getattr__ below is not asked again)
     return _lib
 
 

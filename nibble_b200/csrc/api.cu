@@ -633,7 +633,7 @@ int nbl_kv_create(nbl_ctx* ctx, const nbl_kv_config* cfg, nbl_kv** out) {
       if ((c.head_dim != 64 && c.head_dim != 128) || c.page_size != 16)
         nbl::fail(NBL_E_UNSUPPORTED, "kv_create: the 8-bit kernels take head_dim 64 or 128 and page_size 16 (got " +
                                          std::to_string(c.head_dim) + ", " + std::to_string(c.page_size) + ")");
-      require(c.n_pages <= INT32_MAX && c.n_kv_heads <= 65535, "kv_create: too many pages or KV heads");
+      require(c.n_pages <= INT32_MAX && c.n_kv_heads <= 32767, "kv_create: too many pages or KV heads");
     } else if (c.head_dim != 64 || c.page_size != 16)
       nbl::fail(NBL_E_UNSUPPORTED, "kv_create: the paged kernels take head_dim 64 and page_size 16 (got " +
                                        std::to_string(c.head_dim) + ", " + std::to_string(c.page_size) + ")");

@@ -24,8 +24,8 @@ int guarded(F&& f) {
   }
 }
 
-void require(bool ok, const std::string& msg) {
-  if (!ok) nbl::fail(NBL_E_INVALID, msg);
+void require(bool ok, const char* what, const char* msg) {
+  if (!ok) nbl::fail(NBL_E_INVALID, std::string(what) + ": " + msg);
 }
 
 void use(nbl_ctx* ctx) {
@@ -35,20 +35,20 @@ void use(nbl_ctx* ctx) {
 
 bool is_float(int32_t d) { return d == NBL_F32 || d == NBL_F16 || d == NBL_BF16; }
 
-void require_pool(const nbl_ctx* ctx, const nbl_kv* kv, const std::string& what) {
-  require(kv->ctx == ctx, what + ": pool belongs to another context");
+void require_pool(const nbl_ctx* ctx, const nbl_kv* kv, const char* what) {
+  require(kv->ctx == ctx, what, "pool belongs to another context");
 }
-void require_kv8(const nbl_ctx* ctx, const nbl_kv* kv, const std::string& what) {
+void require_kv8(const nbl_ctx* ctx, const nbl_kv* kv, const char* what) {
   require_pool(ctx, kv, what);
-  require(nbl::is_kv8(kv->cfg.dtype), what + ": takes an NBL_I8 or NBL_E4M3 pool");
+  require(nbl::is_kv8(kv->cfg.dtype), what, "takes an NBL_I8 or NBL_E4M3 pool");
 }
 
 nbl::Kv8Items items_of(const nbl_kv* kv, int64_t n_rows, const int32_t* start, const int32_t* len, const int32_t* pos0,
                        const int32_t* page_table, int32_t pt_stride, int32_t n_items, int32_t max_len,
-                       const std::string& what) {
-  require(n_rows >= 0 && n_items >= 0 && max_len >= 0 && pt_stride > 0, what + ": negative size");
+                       const char* what) {
+  require(n_rows >= 0 && n_items >= 0 && max_len >= 0 && pt_stride > 0, what, "negative size");
   require(int64_t(pt_stride) * kv->cfg.page_size <= INT32_MAX && max_len <= pt_stride * kv->cfg.page_size,
-          what + ": max_len exceeds pt_stride * page_size");
+          what, "max_len exceeds pt_stride * page_size");
   nbl::Kv8Items it;
   it.start = start;
   it.len = len;
@@ -101,21 +101,21 @@ void rotary_frequencies(const nbl_rotary_params& rp, int n, std::vector<double>&
     for (int i = 0; i < n / 2; ++i) freq[i] /= rp.freq_factors[i];
 }
 
-void check_rotary(const nbl_rotary_params& rp, int head_dim, const std::string& what) {
-  require(std::isfinite(rp.freq_base) && rp.freq_base > 1.f, what + ": freq_base must be greater than 1");
+void check_rotary(const nbl_rotary_params& rp, int head_dim, const char* what) {
+  require(std::isfinite(rp.freq_base) && rp.freq_base > 1.f, what, "freq_base must be greater than 1");
   require(rp.rotary_dim >= 0 && rp.rotary_dim <= head_dim && rp.rotary_dim % 2 == 0,
-          what + ": rotary_dim must be even and at most head_dim (0: all of it)");
-  require(rp.scaling >= NBL_ROTARY_NONE && rp.scaling <= NBL_ROTARY_WAVELENGTH, what + ": unknown scaling");
-  require(std::isfinite(rp.attn_factor) && rp.attn_factor >= 0.f, what + ": attn_factor must not be negative");
+          what, "rotary_dim must be even and at most head_dim (0: all of it)");
+  require(rp.scaling >= NBL_ROTARY_NONE && rp.scaling <= NBL_ROTARY_WAVELENGTH, what, "unknown scaling");
+  require(std::isfinite(rp.attn_factor) && rp.attn_factor >= 0.f, what, "attn_factor must not be negative");
   if (rp.scaling != NBL_ROTARY_NONE)
-    require(std::isfinite(rp.factor) && rp.factor >= 1.f, what + ": the scaling factor must be at least 1");
+    require(std::isfinite(rp.factor) && rp.factor >= 1.f, what, "the scaling factor must be at least 1");
   if (rp.scaling == NBL_ROTARY_YARN)
     require(rp.original_ctx > 0 && rp.beta_slow > 0.f && rp.beta_fast >= rp.beta_slow && std::isfinite(rp.beta_fast),
-            what + ": yarn needs original_ctx > 0 and beta_fast >= beta_slow > 0");
+            what, "yarn needs original_ctx > 0 and beta_fast >= beta_slow > 0");
   if (rp.scaling == NBL_ROTARY_WAVELENGTH)
     require(rp.original_ctx > 0 && rp.low_freq_factor > 0.f && rp.high_freq_factor > rp.low_freq_factor &&
                 std::isfinite(rp.high_freq_factor),
-            what + ": wavelength needs original_ctx > 0 and high_freq_factor > low_freq_factor > 0");
+            what, "wavelength needs original_ctx > 0 and high_freq_factor > low_freq_factor > 0");
 }
 
 bool same_rotary(const nbl::RotaryTable& t, const nbl_rotary_params& rp, int n) {
@@ -171,9 +171,9 @@ const nbl::RotaryTable& rotary_table(nbl_ctx* ctx, const nbl_rotary_params& rp, 
 }
 
 nbl::PageBook book_of(const nbl_kv* kv, int32_t* table, int32_t pt_stride, int32_t n_rows, int32_t* lens, int32_t* refs,
-                      const std::string& what) {
-  require(pt_stride > 0 && n_rows >= 0, what + ": negative size");
-  require(int64_t(pt_stride) * kv->cfg.page_size <= INT32_MAX, what + ": pt_stride too large");
+                      const char* what) {
+  require(pt_stride > 0 && n_rows >= 0, what, "negative size");
+  require(int64_t(pt_stride) * kv->cfg.page_size <= INT32_MAX, what, "pt_stride too large");
   nbl::PageBook b;
   b.table = table;
   b.lens = lens;
@@ -194,12 +194,12 @@ int nbl_rotary_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const void*
                          const int32_t* kv_pos0, const int32_t* page_table, int32_t pt_stride, int32_t n_items,
                          int32_t n_heads, int32_t max_q_len, const nbl_rotary_params* rotary) {
   return guarded([&] {
-    const std::string what = "rotary_kv_append";
+    const char* what = "rotary_kv_append";
     require(ctx && kv && q_in && k_in && v_in && q_out && q_start && q_len && kv_pos0 && page_table && rotary,
-            what + ": NULL argument");
+            what, "NULL argument");
     require_kv8(ctx, kv, what);
-    require(is_float(in_dtype) && is_float(q_out_dtype), what + ": bad dtype");
-    require(n_heads > 0 && n_heads % kv->cfg.n_kv_heads == 0, what + ": n_heads must be a multiple of n_kv_heads");
+    require(is_float(in_dtype) && is_float(q_out_dtype), what, "bad dtype");
+    require(n_heads > 0 && n_heads % kv->cfg.n_kv_heads == 0, what, "n_heads must be a multiple of n_kv_heads");
     const auto it = items_of(kv, n_rows, q_start, q_len, kv_pos0, page_table, pt_stride, n_items, max_q_len, what);
     check_rotary(*rotary, kv->cfg.head_dim, what);
     if (n_items == 0 || max_q_len == 0 || n_rows == 0) return;
@@ -228,10 +228,10 @@ int nbl_kv_read(nbl_ctx* ctx, const nbl_kv* kv, int64_t n_rows, const int32_t* s
                 const int32_t* kv_pos0, const int32_t* page_table, int32_t pt_stride, int32_t n_items, int32_t max_len,
                 void* k_out, void* v_out, int32_t out_dtype) {
   return guarded([&] {
-    const std::string what = "kv_read";
-    require(ctx && kv && start && len && kv_pos0 && page_table && (k_out || v_out), what + ": NULL argument");
+    const char* what = "kv_read";
+    require(ctx && kv && start && len && kv_pos0 && page_table && (k_out || v_out), what, "NULL argument");
     require_kv8(ctx, kv, what);
-    require(is_float(out_dtype), what + ": bad dtype");
+    require(is_float(out_dtype), what, "bad dtype");
     const auto it = items_of(kv, n_rows, start, len, kv_pos0, page_table, pt_stride, n_items, max_len, what);
     if (n_items == 0 || max_len == 0 || n_rows == 0) return;
     use(ctx);
@@ -241,9 +241,9 @@ int nbl_kv_read(nbl_ctx* ctx, const nbl_kv* kv, int64_t n_rows, const int32_t* s
 
 int nbl_kv_import(nbl_ctx* ctx, nbl_kv* kv, const int32_t* page_ids, int64_t n, const void* codes, const float* scales) {
   return guarded([&] {
-    require(ctx && kv && page_ids && codes && scales, "kv_import: NULL argument");
+    require(ctx && kv && page_ids && codes && scales, "kv_import", "NULL argument");
     require_kv8(ctx, kv, "kv_import");
-    require(n >= 0 && n <= INT32_MAX, "kv_import: bad page count");
+    require(n >= 0 && n <= INT32_MAX, "kv_import", "bad page count");
     if (n == 0) return;
     use(ctx);
     nbl::launch_kv8_import(ctx->stream, kv, page_ids, n, codes, scales, ctx->d_err);
@@ -252,9 +252,9 @@ int nbl_kv_import(nbl_ctx* ctx, nbl_kv* kv, const int32_t* page_ids, int64_t n, 
 
 int nbl_kv_export(nbl_ctx* ctx, const nbl_kv* kv, const int32_t* page_ids, int64_t n, void* codes, float* scales) {
   return guarded([&] {
-    require(ctx && kv && page_ids && codes && scales, "kv_export: NULL argument");
+    require(ctx && kv && page_ids && codes && scales, "kv_export", "NULL argument");
     require_kv8(ctx, kv, "kv_export");
-    require(n >= 0 && n <= INT32_MAX, "kv_export: bad page count");
+    require(n >= 0 && n <= INT32_MAX, "kv_export", "bad page count");
     if (n == 0) return;
     use(ctx);
     nbl::launch_kv8_export(ctx->stream, kv, page_ids, n, codes, scales, ctx->d_err);
@@ -263,9 +263,9 @@ int nbl_kv_export(nbl_ctx* ctx, const nbl_kv* kv, const int32_t* page_ids, int64
 
 int nbl_kv_copy_pages(nbl_ctx* ctx, nbl_kv* kv, const int32_t* src_pages, const int32_t* dst_pages, int32_t n) {
   return guarded([&] {
-    require(ctx && kv && src_pages && dst_pages, "kv_copy_pages: NULL argument");
+    require(ctx && kv && src_pages && dst_pages, "kv_copy_pages", "NULL argument");
     require_pool(ctx, kv, "kv_copy_pages");
-    require(n >= 0, "kv_copy_pages: negative size");
+    require(n >= 0, "kv_copy_pages", "negative size");
     if (n == 0) return;
     use(ctx);
     nbl::launch_copy_pages(ctx->stream, kv, src_pages, dst_pages, n, ctx->d_err, ctx->num_sms);
@@ -275,10 +275,10 @@ int nbl_kv_copy_pages(nbl_ctx* ctx, nbl_kv* kv, const int32_t* src_pages, const 
 int nbl_kv_fork(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride, int32_t n_rows, int32_t* seq_lens,
                 int32_t* ref_counts, const int32_t* src_rows, const int32_t* dst_rows, int32_t n) {
   return guarded([&] {
-    require(ctx && kv && page_table && seq_lens && ref_counts && src_rows && dst_rows, "kv_fork: NULL argument");
+    require(ctx && kv && page_table && seq_lens && ref_counts && src_rows && dst_rows, "kv_fork", "NULL argument");
     require_pool(ctx, kv, "kv_fork");
     const auto b = book_of(kv, page_table, pt_stride, n_rows, seq_lens, ref_counts, "kv_fork");
-    require(n >= 0 && n <= n_rows, "kv_fork: n must be 0..n_rows");
+    require(n >= 0 && n <= n_rows, "kv_fork", "n must be 0..n_rows");
     if (n == 0) return;
     use(ctx);
     nbl::ensure_scratch(ctx, nbl::kv_book_scratch(n, kv->cfg.n_pages));
@@ -289,10 +289,10 @@ int nbl_kv_fork(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride
 int nbl_kv_release(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride, int32_t n_rows, int32_t* seq_lens,
                    int32_t* ref_counts, const int32_t* rows, int32_t n) {
   return guarded([&] {
-    require(ctx && kv && page_table && seq_lens && ref_counts && rows, "kv_release: NULL argument");
+    require(ctx && kv && page_table && seq_lens && ref_counts && rows, "kv_release", "NULL argument");
     require_pool(ctx, kv, "kv_release");
     const auto b = book_of(kv, page_table, pt_stride, n_rows, seq_lens, ref_counts, "kv_release");
-    require(n >= 0, "kv_release: negative size");
+    require(n >= 0, "kv_release", "negative size");
     if (n == 0) return;
     use(ctx);
     nbl::launch_kv_release(ctx->stream, b, rows, n, ctx->d_err);
@@ -302,10 +302,10 @@ int nbl_kv_release(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_str
 int nbl_kv_extend(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride, int32_t n_rows, int32_t* seq_lens,
                   int32_t* ref_counts, const int32_t* rows, const int32_t* new_lens, int32_t n) {
   return guarded([&] {
-    require(ctx && kv && page_table && seq_lens && ref_counts && rows && new_lens, "kv_extend: NULL argument");
+    require(ctx && kv && page_table && seq_lens && ref_counts && rows && new_lens, "kv_extend", "NULL argument");
     require_pool(ctx, kv, "kv_extend");
     const auto b = book_of(kv, page_table, pt_stride, n_rows, seq_lens, ref_counts, "kv_extend");
-    require(n >= 0 && n <= n_rows, "kv_extend: n must be 0..n_rows");
+    require(n >= 0 && n <= n_rows, "kv_extend", "n must be 0..n_rows");
     if (n == 0) return;
     use(ctx);
     nbl::ensure_scratch(ctx, nbl::kv_book_scratch(n, kv->cfg.n_pages));
@@ -318,17 +318,17 @@ int nbl_kv_compact(nbl_ctx* ctx, const nbl_kv* src, nbl_kv* dst, const int32_t* 
                    int32_t* n_used) {
   return guarded([&] {
     require(ctx && src && dst && page_table && seq_lens && table_out && ref_counts_out && n_used,
-            "kv_compact: NULL argument");
+            "kv_compact", "NULL argument");
     require_pool(ctx, src, "kv_compact");
     require_pool(ctx, dst, "kv_compact");
     const auto &s = src->cfg, &d = dst->cfg;
     require(src != dst && s.dtype == d.dtype && s.head_dim == d.head_dim && s.n_kv_heads == d.n_kv_heads &&
                 s.page_size == d.page_size,
-            "kv_compact: the pools must be two of the same dtype, head_dim, n_kv_heads and page_size");
-    require(page_table != table_out, "kv_compact: table_out must not be page_table");
+            "kv_compact", "the pools must be two of the same dtype, head_dim, n_kv_heads and page_size");
+    require(page_table != table_out, "kv_compact", "table_out must not be page_table");
     const auto b = book_of(src, const_cast<int32_t*>(page_table), pt_stride, n_rows, const_cast<int32_t*>(seq_lens),
                            nullptr, "kv_compact");
-    require(int64_t(n_rows) * pt_stride <= INT32_MAX, "kv_compact: n_rows * pt_stride exceeds 2^31");
+    require(int64_t(n_rows) * pt_stride <= INT32_MAX, "kv_compact", "n_rows * pt_stride exceeds 2^31");
     use(ctx);
     if (n_rows == 0) {
       nbl::check_cuda(cudaMemsetAsync(n_used, 0, sizeof(int32_t), ctx->stream), "kv_compact");

@@ -42,9 +42,14 @@ __device__ __forceinline__ uint32_t transpose4(uint32_t w, int i) {
   return __byte_perm(w, x, i & 2 ? 0x3276 : 0x5410);
 }
 
-// Eight consecutive elements of a float type as fp32, and back; 16-byte aligned.
-__device__ __forceinline__ void load8v(const void* p, int64_t i, int dtype, float (&v)[8]) {
-  if (dtype == NBL_F32) {
+// Loads are typed by the template parameter IN, so that a thread's loads are all issued before the first is used (a branch
+// on the type at each load would wait for it there). IN < 0: any type and alignment, element by element.
+template <int IN>
+__device__ __forceinline__ void load8(const void* p, int64_t i, int dtype, float (&v)[8]) {
+  if constexpr (IN < 0) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = load_as(p, i + k, dtype);
+  } else if constexpr (IN == NBL_F32) {
     const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
     const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
@@ -53,12 +58,50 @@ __device__ __forceinline__ void load8v(const void* p, int64_t i, int dtype, floa
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float2 f = dtype == NBL_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k]))
-                                        : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+      const float2 f = IN == NBL_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k]))
+                                     : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
       v[2 * k] = f.x, v[2 * k + 1] = f.y;
     }
   }
 }
+// Eight elements as they are (elements lo .. lo + 3 and hi .. hi + 3; whole: hi = lo + 4), and widened: a thread reads several
+// before it widens the first.
+template <int IN>
+struct Raw8 {
+  uint4 r[IN == NBL_F32 ? 2 : 1];
+};
+template <int IN>
+__device__ __forceinline__ Raw8<IN> read8(const void* p, int64_t lo, int64_t hi, bool whole) {
+  Raw8<IN> x;
+  if constexpr (IN == NBL_F32) {
+    x.r[0] = *reinterpret_cast<const uint4*>(static_cast<const float*>(p) + lo);
+    x.r[1] = *reinterpret_cast<const uint4*>(static_cast<const float*>(p) + hi);
+  } else if (whole) {
+    x.r[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + lo);
+  } else {
+    const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + lo);
+    const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + hi);
+    x.r[0] = make_uint4(a.x, a.y, b.x, b.y);
+  }
+  return x;
+}
+template <int IN>
+__device__ __forceinline__ void widen8(const Raw8<IN>& x, float (&v)[8]) {
+  const uint32_t w[4] = {x.r[0].x, x.r[0].y, x.r[0].z, x.r[0].w};
+  if constexpr (IN == NBL_F32) {
+    const uint32_t z[4] = {x.r[1].x, x.r[1].y, x.r[1].z, x.r[1].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]), v[4 + k] = __uint_as_float(z[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = IN == NBL_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k]))
+                                     : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+      v[2 * k] = f.x, v[2 * k + 1] = f.y;
+    }
+  }
+}
+// Eight (four) consecutive fp32 values as `dtype`; 16-byte (8-byte for four 16-bit ones) aligned.
 __device__ __forceinline__ void store8v(void* p, int64_t i, int dtype, const float (&v)[8]) {
   if (dtype == NBL_F32) {
     *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
@@ -78,23 +121,27 @@ __device__ __forceinline__ void store8v(void* p, int64_t i, int dtype, const flo
     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-template <bool VEC>
-__device__ __forceinline__ void load8(const void* p, int64_t i, int dtype, float (&v)[8]) {
-  if constexpr (VEC) {
-    load8v(p, i, dtype, v);
+__device__ __forceinline__ void store4v(void* p, int64_t i, int dtype, const float* v) {
+  if (dtype == NBL_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
   } else {
+    uint32_t w[2];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = load_as(p, i + k, dtype);
+    for (int k = 0; k < 2; ++k) {
+      if (dtype == NBL_F16) {
+        const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(w[0], w[1]);
   }
 }
-template <bool VEC>
 __device__ __forceinline__ void store8(void* p, int64_t i, int dtype, const float (&v)[8]) {
-  if constexpr (VEC) {
-    store8v(p, i, dtype, v);
-  } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) store_as(p, i + k, v[k], dtype);
-  }
+  for (int k = 0; k < 8; ++k) store_as(p, i + k, v[k], dtype);
 }
 __device__ __forceinline__ void add8(float (&v)[8], const float* b) {
 #pragma unroll
@@ -102,13 +149,14 @@ __device__ __forceinline__ void add8(float (&v)[8], const float* b) {
 }
 
 // A chunk of a head with bias, rotated: element e and its partner (e ^ 1, or half the rotated part away) turn by the angle
-// of their pair. cs[k]: (cos, sin) for element 8c + k. VEC: the chunk, and its partner chunk where the partners are
+// of their pair. cs[k]: (cos, sin) for element 8c + k. IN >= 0: the chunk, and its partner chunk where the partners are
 // elsewhere, are whole and 16-byte aligned.
-template <bool VEC>
+template <int IN>
 __device__ __forceinline__ void rotated8(const void* src, int64_t row, int c, int dtype, const float* bias, bool neox, int rd,
                                          const float2 (&cs)[8], float (&v)[8]) {
+  constexpr bool VEC = IN >= 0;
   const int e0 = 8 * c, half = rd / 2;
-  load8<VEC>(src, row + e0, dtype, v);
+  load8<IN>(src, row + e0, dtype, v);
   if (bias) add8(v, bias + e0);
   if (e0 >= rd) return;
   float other[8];
@@ -117,7 +165,7 @@ __device__ __forceinline__ void rotated8(const void* src, int64_t row, int c, in
     for (int k = 0; k < 8; ++k) other[k] = v[k ^ 1];
   } else if (VEC) {
     const int o0 = e0 < half ? e0 + half : e0 - half;
-    load8v(src, row + o0, dtype, other);
+    load8<IN>(src, row + o0, dtype, other);
     if (bias) add8(other, bias + o0);
   } else {
 #pragma unroll
@@ -143,132 +191,176 @@ __device__ __forceinline__ void rotated8(const void* src, int64_t row, int c, in
     if (VEC || e0 + k < rd) v[k] = other[k];
 }
 
-// Four consecutive elements as fp32, and back; VEC: 8- (16-bit types) or 16-byte aligned.
-template <bool VEC>
-__device__ __forceinline__ void load4(const void* p, int64_t i, int dtype, float* v) {
-  if (!VEC) {
+// Pairs 4c .. 4c + 3 of a query head: both elements of a pair are one thread's, so the rotation may be in place. The first
+// rd / 2 pairs are the rotated ones, the others the untouched elements two by two. cs[k]: (cos, sin) of pair 4c + k.
+// The pairs of a whole chunk: elements lo .. lo + 3 and hi .. hi + 3 (rd is a multiple of 8: a chunk is rotated whole or not
+// at all).
+struct Chunk {
+  bool turn, split;
+  int lo, hi;
+};
+__device__ __forceinline__ Chunk chunk_of(int c, bool neox, int rd) {
+  Chunk k;
+  k.turn = 8 * c < rd, k.split = neox && k.turn;
+  k.lo = k.split ? 4 * c : 8 * c, k.hi = k.split ? rd / 2 + 4 * c : 8 * c + 4;
+  return k;
+}
+__device__ __forceinline__ void turn8(const Chunk& k, const float2 (&cs)[4], const float* bias, float (&v)[8]) {
+  if (bias) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = load_as(p, i + k, dtype);
-  } else if (dtype == NBL_F32) {
-    const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-  } else {
-    const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-    const uint32_t w[2] = {x.x, x.y};
+    for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(v[i], bias[k.lo + i]), v[4 + i] = __fadd_rn(v[4 + i], bias[k.hi + i]);
+  }
+  if (k.split) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float2 f = dtype == NBL_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k]))
-                                        : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
-      v[2 * k] = f.x, v[2 * k + 1] = f.y;
-    }
+    for (int i = 0; i < 4; ++i) rope_rotate(v[i], v[4 + i], cs[i], v[i], v[4 + i]);
+  } else if (k.turn) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rope_rotate(v[2 * i], v[2 * i + 1], cs[i], v[2 * i], v[2 * i + 1]);
   }
 }
-template <bool VEC>
-__device__ __forceinline__ void store4(void* p, int64_t i, int dtype, const float* v) {
-  if (!VEC) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) store_as(p, i + k, v[k], dtype);
-  } else if (dtype == NBL_F32) {
-    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-    uint32_t w[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (dtype == NBL_F16) {
-        const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-        w[k] = *reinterpret_cast<const uint32_t*>(&h);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-        w[k] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-    }
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(w[0], w[1]);
-  }
-}
-
-// Pairs 4c .. 4c + 3 of a query head: both elements of a pair are this thread's, so the rotation may be in place. The
-// first rd / 2 pairs are the rotated ones, the others the untouched elements two by two. cs[k]: (cos, sin) of pair 4c + k.
-template <bool VEC>
-__device__ __forceinline__ void query8(const void* src, void* dst, int64_t row, int c, int in_dtype, int out_dtype,
-                                       const float* bias, bool neox, int rd, const float2 (&cs)[4]) {
-  float v[8];
+__device__ __forceinline__ void query8_any(const void* src, void* dst, int64_t row, int c, int in_dtype, int out_dtype,
+                                           const float* bias, bool neox, int rd, const float2 (&cs)[4]) {
   const int half = rd / 2;
-  if (VEC) {  // rd is a multiple of 8: a chunk is rotated whole or not at all
-    const bool split = neox && 8 * c < rd;
-    const int lo = split ? 4 * c : 8 * c, hi = split ? half + 4 * c : 8 * c + 4;
-    if (split) {
-      load4<true>(src, row + lo, in_dtype, v);
-      load4<true>(src, row + hi, in_dtype, v + 4);
-    } else {
-      load8v(src, row + lo, in_dtype, v);
-    }
-    if (bias) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = __fadd_rn(v[k], bias[lo + k]), v[4 + k] = __fadd_rn(v[4 + k], bias[hi + k]);
-    }
-    if (split) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) rope_rotate(v[k], v[4 + k], cs[k], v[k], v[4 + k]);
-      store4<true>(dst, row + lo, out_dtype, v);
-      store4<true>(dst, row + hi, out_dtype, v + 4);
-    } else {
-      if (8 * c < rd) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) rope_rotate(v[2 * k], v[2 * k + 1], cs[k], v[2 * k], v[2 * k + 1]);
-      }
-      store8v(dst, row + lo, out_dtype, v);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int p = 4 * c + k;
-      const bool turn = p < half;
-      const int e0 = turn ? (neox ? p : 2 * p) : rd + 2 * (p - half), e1 = turn && neox ? p + half : e0 + 1;
-      float x = load_as(src, row + e0, in_dtype), y = load_as(src, row + e1, in_dtype);
-      if (bias) x = __fadd_rn(x, bias[e0]), y = __fadd_rn(y, bias[e1]);
-      if (turn) rope_rotate(x, y, cs[k], x, y);
-      store_as(dst, row + e0, x, out_dtype);
-      store_as(dst, row + e1, y, out_dtype);
-    }
+  for (int k = 0; k < 4; ++k) {
+    const int p = 4 * c + k;
+    const bool turn = p < half;
+    const int e0 = turn ? (neox ? p : 2 * p) : rd + 2 * (p - half), e1 = turn && neox ? p + half : e0 + 1;
+    float x = load_as(src, row + e0, in_dtype), y = load_as(src, row + e1, in_dtype);
+    if (bias) x = __fadd_rn(x, bias[e0]), y = __fadd_rn(y, bias[e1]);
+    if (turn) rope_rotate(x, y, cs[k], x, y);
+    store_as(dst, row + e0, x, out_dtype);
+    store_as(dst, row + e1, y, out_dtype);
   }
 }
 
-// One CTA per (touched page of an item, KV head): the page's new tokens' keys and values, and the query heads of that KV
-// head for those tokens. Bound: memory (each input once, each output once); the queries' loads cover the latency of the
-// keys' and values' reduction.
-template <int D, int KIND, bool VEC>
-__global__ void __launch_bounds__(kCtaThreads<D>) kv8_append_kernel(const Kv8Items it, const Kv8Append a, uint8_t* pool,
-                                                                    int64_t n_pages, int n_kv_heads, int max_blocks,
-                                                                    int* err) {
-  __shared__ float red[2][kCtaThreads<D> / 32];
-  const int item = blockIdx.x / max_blocks, kvh = blockIdx.y;
-  const int start = it.start[item], len = it.len[item], pos0 = it.pos0[item];
-  if (len <= 0) return;
+// The touched pages of the items, one after another: page u's item, its fields, and the page's number in the sequence.
+// With one page an item at most (decode steps), or more than kScanItems items, page u is page u % max_blocks of item
+// u / max_blocks, and may be empty; otherwise every warp adds up the items' pages, 32 items at a time, and the grid is
+// bounded by the rows of the packed activations (24 prompts of 97..2047 tokens: 1085 pages in place of 3096, of which two
+// thirds were empty; an empty CTA still reads its item).
+constexpr int kScanItems = 256;
+struct Page {
+  int item, start, len, pos0, block;
+  bool valid;
+};
+__host__ __device__ inline bool scanned(int n_items, int max_blocks) { return max_blocks > 1 && n_items <= kScanItems; }
+__device__ __forceinline__ bool item_ok(const Kv8Items& it, int start, int len, int pos0, int64_t tab_pos) {
   const int64_t end = int64_t(pos0) + len;
-  const int64_t block = int64_t(pos0) / kPage + blockIdx.x % max_blocks;
-  if (pos0 < 0 || start < 0 || int64_t(start) + len > it.n_rows || end > int64_t(it.pt_stride) * kPage || end > a.tab_pos) {
-    if (threadIdx.x == 0) flag_error(err, kErrLength);
-    return;
+  return pos0 >= 0 && start >= 0 && int64_t(start) + len <= it.n_rows && end <= int64_t(it.pt_stride) * kPage && end <= tab_pos;
+}
+__device__ __forceinline__ Page page_at(const Kv8Items& it, int max_blocks, int64_t tab_pos, int u, int* err) {
+  Page p;
+  p.valid = false;
+  if (!scanned(it.n_items, max_blocks)) {
+    p.item = u / max_blocks;
+    p.start = it.start[p.item], p.len = it.len[p.item], p.pos0 = it.pos0[p.item];
+    if (p.len <= 0) return p;
+    if (!item_ok(it, p.start, p.len, p.pos0, tab_pos)) {
+      if (threadIdx.x == 0) flag_error(err, kErrLength);
+      return p;
+    }
+    p.block = p.pos0 / kPage + u % max_blocks;
+    p.valid = int64_t(p.block) * kPage < int64_t(p.pos0) + p.len;
+    return p;
   }
-  if (block * kPage >= end) return;
-  const int32_t page = it.page_table[int64_t(item) * it.pt_stride + block];
-  const int base = static_cast<int>(block) * kPage;
-  const int slot0 = max(pos0 - base, 0), slot1 = static_cast<int>(min(end - base, int64_t(kPage)));  // the new tokens' places
-  const int group = a.n_heads / n_kv_heads, rd = a.rotary_dim;
-  const bool good = page >= 0 && page < n_pages;
-  if (!good && threadIdx.x == 0) flag_error(err, kErrPageId);
-  uint8_t* blk = pool + int64_t(good ? page : 0) * page_bytes(D, n_kv_heads) + int64_t(kvh) * block_bytes(D);
-  float* sc = reinterpret_cast<float*>(blk + scale_off(D));
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int i0 = 0; i0 < it.n_items; i0 += 32) {
+    const int i = i0 + lane;
+    int start = 0, len = 0, pos0 = 0, n = 0;
+    if (i < it.n_items) {
+      start = it.start[i], len = it.len[i], pos0 = it.pos0[i];
+      if (len > 0) {
+        if (item_ok(it, start, len, pos0, tab_pos)) n = (pos0 + len - 1) / kPage - pos0 / kPage + 1;
+        else if (u == 0) flag_error(err, kErrLength);
+      }
+    }
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    const uint32_t at = __ballot_sync(0xffffffffu, u < before + inc);
+    if (at) {
+      const int l = __ffs(at) - 1;  // the first item that ends behind u
+      p.item = i0 + l;
+      p.start = __shfl_sync(0xffffffffu, start, l), p.len = __shfl_sync(0xffffffffu, len, l);
+      p.pos0 = __shfl_sync(0xffffffffu, pos0, l);
+      p.block = p.pos0 / kPage + u - before - __shfl_sync(0xffffffffu, inc - n, l);
+      p.valid = true;
+      return p;
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return p;
+}
 
+// CTAs (touched page, part): a part for every KV head (the page's new tokens' keys and values), then one for every 8 query
+// heads of those tokens, 8 (fp32: 4) of them in flight. Bound: memory (each input once, each output once). One part per CTA:
+// 888 CTAs that took the parts in turn were slower (83 against 48 us for 24 ragged prompts).
+template <int D, int KIND, int IN>
+__global__ void __launch_bounds__(kCtaThreads<D>, D == 64 ? 7 : 4)
+    kv8_append_kernel(const Kv8Items it, const Kv8Append a, uint8_t* pool, int64_t n_pages, int n_kv_heads, int max_blocks,
+                      int* err) {
+  constexpr bool VEC = IN >= 0;
+  __shared__ float red[2][kCtaThreads<D> / 32];
+  const int rd = a.rotary_dim, part = blockIdx.y;
+  const Page pg = page_at(it, max_blocks, a.tab_pos, blockIdx.x, err);
+  if (!pg.valid) return;
   const Place pl = place_of(threadIdx.x);
   const int c = pl.c, tok = pl.tok;
+  const int64_t end = int64_t(pg.pos0) + pg.len;
+  const int base = pg.block * kPage;
+  const int slot0 = max(pg.pos0 - base, 0), slot1 = static_cast<int>(min(end - base, int64_t(kPage)));  // the new tokens' places
   const bool is_new = tok >= slot0 && tok < slot1, is_old = tok < slot0;
-  const int64_t row = int64_t(start) + (base + tok - pos0);  // of the packed activations
+  const int64_t row = int64_t(pg.start) + (base + tok - pg.pos0);  // of the packed activations
+  const float2* tab = a.tab + int64_t(base + tok) * (rd / 2);
+
+  if (part >= n_kv_heads) {
+    if (!is_new) return;
+    const int head0 = (part - n_kv_heads) * 8, heads = min(8, a.n_heads - head0);
+    const int64_t q0 = (row * a.n_heads + head0) * D;
+    const float* bq = a.bq ? a.bq + head0 * D : nullptr;
+    float2 cs[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) cs[k] = 4 * c + k < rd / 2 ? tab[4 * c + k] : make_float2(1.f, 0.f);
+    if constexpr (VEC) {
+      const Chunk ch = chunk_of(c, a.neox, rd);
+      constexpr int kQHeads = IN == NBL_F32 ? 4 : 8;
+      for (int h0 = 0; h0 < heads; h0 += kQHeads) {
+        Raw8<IN> x[kQHeads];
+#pragma unroll
+        for (int h = 0; h < kQHeads; ++h)
+          if (h0 + h < heads) x[h] = read8<IN>(a.q_in, q0 + (h0 + h) * D + ch.lo, q0 + (h0 + h) * D + ch.hi, !ch.split);
+#pragma unroll
+        for (int h = 0; h < kQHeads; ++h) {
+          if (h0 + h >= heads) break;
+          float v[8];
+          widen8<IN>(x[h], v);
+          turn8(ch, cs, bq ? bq + (h0 + h) * D : nullptr, v);
+          if (ch.split) {
+            store4v(a.q_out, q0 + (h0 + h) * D + ch.lo, a.q_out_dtype, v);
+            store4v(a.q_out, q0 + (h0 + h) * D + ch.hi, a.q_out_dtype, v + 4);
+          } else {
+            store8v(a.q_out, q0 + (h0 + h) * D + ch.lo, a.q_out_dtype, v);
+          }
+        }
+      }
+    } else {
+      for (int h = 0; h < heads; ++h)
+        query8_any(a.q_in, a.q_out, q0 + h * D, c, a.in_dtype, a.q_out_dtype, bq ? bq + h * D : nullptr, a.neox, rd, cs);
+    }
+    return;
+  }
+
+  const int kvh = part;
+  const int32_t page = it.page_table[int64_t(pg.item) * it.pt_stride + pg.block];
   float k8[8], v8[8];
   if (is_new) {
     float2 cs[8];
     if (8 * c < rd) {
-      const float2* tab = a.tab + int64_t(base + tok) * (rd / 2);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int e = 8 * c + k;
@@ -276,23 +368,16 @@ __global__ void __launch_bounds__(kCtaThreads<D>) kv8_append_kernel(const Kv8Ite
         else if (VEC || e < rd) cs[k] = tab[a.neox ? (e < rd / 2 ? e : e - rd / 2) : e >> 1];
       }
     }
-    load8<VEC>(a.v_in, (row * n_kv_heads + kvh) * D + 8 * c, a.in_dtype, v8);
-    rotated8<VEC>(a.k_in, (row * n_kv_heads + kvh) * D, c, a.in_dtype, a.bk ? a.bk + kvh * D : nullptr, a.neox, rd, cs, k8);
+    load8<IN>(a.v_in, (row * n_kv_heads + kvh) * D + 8 * c, a.in_dtype, v8);
+    rotated8<IN>(a.k_in, (row * n_kv_heads + kvh) * D, c, a.in_dtype, a.bk ? a.bk + kvh * D : nullptr, a.neox, rd, cs, k8);
     if (a.bv) add8(v8, a.bv + kvh * D + 8 * c);
-    const int64_t q0 = (row * a.n_heads + int64_t(kvh) * group) * D;
-    const float* bq = a.bq ? a.bq + kvh * group * D : nullptr;
-    float2 qcs[4];
-    if (4 * c < rd / 2) {
-      const float2* tab = a.tab + int64_t(base + tok) * (rd / 2) + 4 * c;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (VEC || 4 * c + k < rd / 2) qcs[k] = tab[k];
-    }
-#pragma unroll 4
-    for (int h = 0; h < group; ++h)
-      query8<VEC>(a.q_in, a.q_out, q0 + h * D, c, a.in_dtype, a.q_out_dtype, bq ? bq + h * D : nullptr, a.neox, rd, qcs);
   }
-  if (!good) return;
+  if (page < 0 || page >= n_pages) {
+    if (threadIdx.x == 0) flag_error(err, kErrPageId);
+    return;
+  }
+  uint8_t* blk = pool + int64_t(page) * page_bytes(D, n_kv_heads) + int64_t(kvh) * block_bytes(D);
+  float* sc = reinterpret_cast<float*>(blk + scale_off(D));
   // largest magnitudes of the new tokens
   float amax[2] = {0.f, 0.f};
   bool odd = false;
@@ -369,52 +454,61 @@ __global__ void __launch_bounds__(kCtaThreads<D>) kv8_append_kernel(const Kv8Ite
   if (threadIdx.x < 2) sc[threadIdx.x] = s[threadIdx.x];
 }
 
-// One CTA per (touched page of an item, KV head): its rows as code * scale.
+// CTAs (touched page, stretch of kReadHeads KV heads, all in flight): a row is code * scale.
+constexpr int kReadHeads = 4;
 template <int D, int KIND>
 __global__ void __launch_bounds__(kCtaThreads<D>) kv8_read_kernel(const Kv8Items it, const uint8_t* pool, int64_t n_pages,
                                                                   int n_kv_heads, int max_blocks, void* k_out, void* v_out,
                                                                   int out_dtype, bool vec, int* err) {
-  const int item = blockIdx.x / max_blocks, kvh = blockIdx.y;
-  const int start = it.start[item], len = it.len[item], pos0 = it.pos0[item];
-  if (len <= 0) return;
-  const int64_t end = int64_t(pos0) + len;
-  const int64_t block = int64_t(pos0) / kPage + blockIdx.x % max_blocks;
-  if (pos0 < 0 || start < 0 || int64_t(start) + len > it.n_rows || end > int64_t(it.pt_stride) * kPage) {
-    if (threadIdx.x == 0) flag_error(err, kErrLength);
-    return;
-  }
-  if (block * kPage >= end) return;
-  const int32_t page = it.page_table[int64_t(item) * it.pt_stride + block];
+  const Page at_page = page_at(it, max_blocks, INT64_MAX, blockIdx.x, err);
+  if (!at_page.valid) return;
+  const Place pl = place_of(threadIdx.x);
+  const int start = at_page.start, pos0 = at_page.pos0;
+  const int64_t end = int64_t(pos0) + at_page.len;
+  const int base = at_page.block * kPage;
+  const int32_t page = it.page_table[int64_t(at_page.item) * it.pt_stride + at_page.block];
   if (page < 0 || page >= n_pages) {
     if (threadIdx.x == 0) flag_error(err, kErrPageId);
     return;
   }
-  const int base = static_cast<int>(block) * kPage;
-  const uint8_t* blk = pool + int64_t(page) * page_bytes(D, n_kv_heads) + int64_t(kvh) * block_bytes(D);
-  const float2 sc = *reinterpret_cast<const float2*>(blk + scale_off(D));
-  const Place pl = place_of(threadIdx.x);
-  const uint2 kw = *reinterpret_cast<const uint2*>(blk + key_off(pl.tok, 8 * pl.c));
-  uint32_t vw[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    vw[j] = transpose4(from_word<KIND>(*reinterpret_cast<const uint32_t*>(blk + value_off(D, pl.t, 8 * pl.c + 4 * j + pl.i))),
-                       pl.i);
   const int pos = base + pl.tok;
-  if (pos < pos0 || pos >= end) return;
-  const int64_t at = ((int64_t(start) + (pos - pos0)) * n_kv_heads + kvh) * D + 8 * pl.c;
-  const uint32_t k2[2] = {from_word<KIND>(kw.x), from_word<KIND>(kw.y)};
-  float k8[8], v8[8];
+  const bool mine = pos >= pos0 && pos < end;
+  const int64_t row = int64_t(start) + (pos - pos0);
+  const uint8_t* pg = pool + int64_t(page) * page_bytes(D, n_kv_heads);
+  const int h0 = blockIdx.y * kReadHeads, n = min(kReadHeads, n_kv_heads - h0);
+  uint2 kw[kReadHeads];
+  uint32_t vw[kReadHeads][2];
+  float2 sc[kReadHeads];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    k8[k] = __fmul_rn(decode<KIND>(k2[k >> 2] >> (8 * (k & 3))), sc.x);
-    v8[k] = __fmul_rn(decode<KIND>(vw[k >> 2] >> (8 * (k & 3))), sc.y);
+  for (int h = 0; h < kReadHeads; ++h) {
+    if (h >= n) break;
+    const uint8_t* blk = pg + int64_t(h0 + h) * block_bytes(D);
+    kw[h] = *reinterpret_cast<const uint2*>(blk + key_off(pl.tok, 8 * pl.c));
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      vw[h][j] = *reinterpret_cast<const uint32_t*>(blk + value_off(D, pl.t, 8 * pl.c + 4 * j + pl.i));
+    sc[h] = *reinterpret_cast<const float2*>(blk + scale_off(D));
   }
-  if (vec) {
-    if (k_out) store8v(k_out, at, out_dtype, k8);
-    if (v_out) store8v(v_out, at, out_dtype, v8);
-  } else {
-    if (k_out) store8<false>(k_out, at, out_dtype, k8);
-    if (v_out) store8<false>(v_out, at, out_dtype, v8);
+#pragma unroll
+  for (int h = 0; h < kReadHeads; ++h) {
+    if (h >= n) break;
+    const uint32_t v2[2] = {transpose4(from_word<KIND>(vw[h][0]), pl.i), transpose4(from_word<KIND>(vw[h][1]), pl.i)};
+    const uint32_t k2[2] = {from_word<KIND>(kw[h].x), from_word<KIND>(kw[h].y)};
+    float k8[8], v8[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      k8[k] = __fmul_rn(decode<KIND>(k2[k >> 2] >> (8 * (k & 3))), sc[h].x);
+      v8[k] = __fmul_rn(decode<KIND>(v2[k >> 2] >> (8 * (k & 3))), sc[h].y);
+    }
+    if (!mine) continue;
+    const int64_t at = (row * n_kv_heads + h0 + h) * D + 8 * pl.c;
+    if (vec) {
+      if (k_out) store8v(k_out, at, out_dtype, k8);
+      if (v_out) store8v(v_out, at, out_dtype, v8);
+    } else {
+      if (k_out) store8(k_out, at, out_dtype, k8);
+      if (v_out) store8(v_out, at, out_dtype, v8);
+    }
   }
 }
 
@@ -520,8 +614,13 @@ void with_kind(const nbl_kv* kv, F&& f) {
 // Pages that max_len tokens can touch, from any first position.
 int touched_pages(int max_len) { return (max_len + kPage - 2) / kPage + 1; }
 
-void grid_check(int64_t ctas, const char* what) {
-  if (ctas > 0x7fffffff) fail(NBL_E_INVALID, std::string(what) + ": n_items * pages per item exceeds 2^31");
+// Pages that the items can touch (see page_at).
+unsigned pages_bound(const Kv8Items& it, const char* what) {
+  const int blocks = touched_pages(it.max_len);
+  int64_t n = int64_t(it.n_items) * blocks;
+  if (scanned(it.n_items, blocks)) n = std::min<int64_t>(n, it.n_rows / kPage + 2 * int64_t(it.n_items));
+  if (n > 0x7fffffff) fail(NBL_E_INVALID, std::string(what) + ": n_items * pages per item exceeds 2^31");
+  return static_cast<unsigned>(n);
 }
 
 }  // namespace
@@ -536,13 +635,17 @@ void launch_kv8_clear(cudaStream_t st, const nbl_kv* kv) {
 
 void launch_kv8_append(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, const Kv8Append& a, int* err) {
   const int blocks = touched_pages(items.max_len);
-  grid_check(int64_t(items.n_items) * blocks, "rotary_kv_append");
-  const dim3 grid(static_cast<unsigned>(items.n_items) * blocks, static_cast<unsigned>(kv->cfg.n_kv_heads));
+  const int64_t parts = kv->cfg.n_kv_heads + (a.n_heads + 7) / 8;
+  if (parts > 65535) fail(NBL_E_INVALID, "rotary_kv_append: too many heads");
+  const dim3 grid(pages_bound(items, "rotary_kv_append"), static_cast<unsigned>(parts));
   const auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
   const bool vec = ((bits(a.q_in) | bits(a.k_in) | bits(a.v_in) | bits(a.q_out)) & 15u) == 0 &&
                    a.rotary_dim % (a.neox ? 16 : 8) == 0;
   with_kind(kv, [&](auto d, auto kind) {
-    auto* k = vec ? kv8_append_kernel<d(), kind(), true> : kv8_append_kernel<d(), kind(), false>;
+    auto* k = !vec                      ? kv8_append_kernel<d(), kind(), -1>
+              : a.in_dtype == NBL_F32 ? kv8_append_kernel<d(), kind(), NBL_F32>
+              : a.in_dtype == NBL_F16 ? kv8_append_kernel<d(), kind(), NBL_F16>
+                                      : kv8_append_kernel<d(), kind(), NBL_BF16>;
     k<<<grid, kCtaThreads<d()>, 0, st>>>(items, a, static_cast<uint8_t*>(kv->pool), kv->cfg.n_pages, kv->cfg.n_kv_heads,
                                          blocks, err);
   });
@@ -552,8 +655,7 @@ void launch_kv8_append(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items,
 void launch_kv8_read(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, void* k_out, void* v_out, int out_dtype,
                      int* err) {
   const int blocks = touched_pages(items.max_len);
-  grid_check(int64_t(items.n_items) * blocks, "kv_read");
-  const dim3 grid(static_cast<unsigned>(items.n_items) * blocks, static_cast<unsigned>(kv->cfg.n_kv_heads));
+  const dim3 grid(pages_bound(items, "kv_read"), static_cast<unsigned>((kv->cfg.n_kv_heads + kReadHeads - 1) / kReadHeads));
   const bool vec = ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u) == 0;
   with_kind(kv, [&](auto d, auto kind) {
     kv8_read_kernel<d(), kind()><<<grid, kCtaThreads<d()>, 0, st>>>(items, static_cast<const uint8_t*>(kv->pool),
