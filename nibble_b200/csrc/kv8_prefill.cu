@@ -334,14 +334,18 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       constexpr uint32_t idesc_pv = make_idesc_f16(kBM, D, false, false, false);
       int lw = 0, kt = 0;
       int h_tiles[2] = {0, 0}, h_works[2] = {0, 0};  // per head: S tiles consumed, works finished
+      // descriptors differ in the address alone: 16-byte units, whose sums stay inside its 14 bits
+      const uint64_t desc0 = make_sdesc(smem_u32(smem), 16, 1024, 2);
+      auto desc_of = [&](const uint8_t* p) { return desc0 + (static_cast<uint32_t>(p - smem) >> 4); };
       // S_g (buffer buf) = Q_g K^T from Q buffer qb and stage s, for head g = 2 mw + i.
       auto qk = [&](int i, int buf, int qb, int s) {
         const int g = 2 * mw + i;
-        const uint32_t q_addr = smem_u32(sQ(qb, g)), k_addr = smem_u32(sK(s));
+        const uint64_t q_desc = desc_of(sQ(qb, g)), k_desc = desc_of(sK(s));
+        const uint32_t to = tmem + C::col_s(g, buf);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          tc_mma_ss(tmem + C::col_s(g, buf), make_sdesc(q_addr + (kk >> 2) * (kBM * 128) + (kk & 3) * 32, 16, 1024, 2),
-                    make_sdesc(k_addr + (kk >> 2) * (kBN * 128) + (kk & 3) * 32, 16, 1024, 2), idesc_qk, kk > 0 ? 1u : 0u);
+          tc_mma_ss(to, q_desc + ((kk >> 2) * (kBM * 128) + (kk & 3) * 32) / 16,
+                    k_desc + ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) / 16, idesc_qk, kk > 0 ? 1u : 0u);
         tc_commit(bar_s(g, buf));
       };
       auto kv_ready = [&](int t) -> bool {
@@ -380,13 +384,19 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
         ok = mbar_wait(&bars[C::kBarQFull + qb], (lw >> 1) & 1, a.err) && kv_ready(kt);
         if (!ok) break;
         // S_g(0) may overwrite columns that an earlier PV_g reads P from: MMAs run in issue order.
-        for (int i = 0; i < n_g; ++i) qk(i, h_tiles[i] % SB, qb, kt % ST);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i < n_g) qk(i, h_tiles[i] % SB, qb, kt % ST);
         for (int j = 0; j < n && ok; ++j, ++kt) {
           const bool more = j + 1 < n;
           if (more) ok = kv_ready(kt + 1);
           if (SB == 2 && more && ok)  // the next S during this tile's softmax
-            for (int i = 0; i < n_g; ++i) qk(i, (h_tiles[i] + 1) % SB, qb, (kt + 1) % ST);
-          for (int i = 0; i < n_g && ok; ++i) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (i < n_g) qk(i, (h_tiles[i] + 1) % SB, qb, (kt + 1) % ST);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (i >= n_g || !ok) break;
             // O_g += P_g V once head g's softmax has written P_g; the work's first PV overwrites O_g, so it also
             // waits for the epilogue of the work before to have read it.
             const int g = 2 * mw + i, buf = h_tiles[i] % SB;
@@ -395,10 +405,10 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
             if (!ok) break;
             ++h_tiles[i];
             tc_fence_after();
-            const uint32_t v_addr = smem_u32(sV(kt % ST));
+            const uint64_t v_desc = desc_of(sV(kt % ST));
 #pragma unroll
             for (int kk = 0; kk < kBN / 16; ++kk)
-              tc_mma_ts(tmem + C::col_o(g), tmem + C::col_s(g, buf) + kk * 8, make_sdesc(v_addr + kk * 32, 16, 1024, 2),
+              tc_mma_ts(tmem + C::col_o(g), tmem + C::col_s(g, buf) + kk * 8, v_desc + kk * 2,
                         idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
             if (SB == 2) tc_commit(&bars[C::kBarPV + g]);
             if (SB == 1 && more) qk(i, 0, qb, (kt + 1) % ST);
@@ -412,7 +422,9 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
         }
         if (!ok) break;
         tc_commit(&bars[C::kBarQFree + qb]);  // every QK of this work has read its Q tiles
-        for (int i = 0; i < n_g; ++i) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (i >= n_g) break;
           tc_commit(&bars[C::kBarODone + 2 * mw + i]);
           ++h_works[i];
         }
