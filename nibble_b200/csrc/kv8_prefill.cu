@@ -154,6 +154,13 @@ __device__ __forceinline__ void widen4_key(uint32_t w, uint32_t& lo, uint32_t& h
   }
 }
 
+// One lane of the converged warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 template <int D, int HEADS, int KIND, bool BF16>
 __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCtas)
     kv8_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const PrefillArgs a) {
@@ -327,115 +334,121 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       }
     }
   } else if (warp >= C::kWarpMma) {
-    // ================= MMA issuers (one thread each): heads 2 mw and 2 mw + 1
-    const int mw = warp - C::kWarpMma;
-    if (lane == 0) {
-      constexpr uint32_t idesc_qk = make_idesc_f16(kBM, kBN, BF16, false, false);
-      constexpr uint32_t idesc_pv = make_idesc_f16(kBM, D, false, false, false);
-      int lw = 0, kt = 0;
-      int h_tiles[2] = {0, 0}, h_works[2] = {0, 0};  // per head: S tiles consumed, works finished
-      // descriptors differ in the address alone: 16-byte units, whose sums stay inside its 14 bits
-      const uint64_t desc0 = make_sdesc(smem_u32(smem), 16, 1024, 2);
-      auto desc_of = [&](const uint8_t* p) { return desc0 + (static_cast<uint32_t>(p - smem) >> 4); };
-      // S_g (buffer buf) = Q_g K^T from Q buffer qb and stage s, for head g = 2 mw + i.
-      auto qk = [&](int i, int buf, int qb, int s) {
-        const int g = 2 * mw + i;
-        const uint64_t q_desc = desc_of(sQ(qb, g)), k_desc = desc_of(sK(s));
-        const uint32_t to = tmem + C::col_s(g, buf);
+    // ================= MMA issuers: heads 2 mw and 2 mw + 1. The whole warp walks the loop and waits; one lane, always the
+    // same, issues. The descriptors are then values of the warp, kept in uniform registers: with the loop inside one
+    // lane's branch every instruction's operands were moved there one by one, which cost 80 cycles an instruction (511
+    // tokens over 16.4k at head_dim 128: 241 us against 176).
+    const int mw = __shfl_sync(0xffffffffu, warp - C::kWarpMma, 0);
+    constexpr uint32_t idesc_qk = make_idesc_f16(kBM, kBN, BF16, false, false);
+    constexpr uint32_t idesc_pv = make_idesc_f16(kBM, D, false, false, false);
+    int lw = 0, kt = 0;
+    int h_tiles[2] = {0, 0}, h_works[2] = {0, 0};  // per head: S tiles consumed, works finished
+    // descriptors differ in the address alone: 16-byte units, whose sums stay inside its 14 bits
+    const uint64_t desc0 = make_sdesc(smem_u32(smem), 16, 1024, 2);
+    auto desc_of = [&](const uint8_t* p) { return desc0 + (static_cast<uint32_t>(p - smem) >> 4); };
+    // S_g (buffer buf) = Q_g K^T from Q buffer qb and stage s, for head g = 2 mw + i.
+    auto qk = [&](int i, int buf, int qb, int s) {
+      const int g = 2 * mw + i;
+      const uint64_t q_desc = desc_of(sQ(qb, g)), k_desc = desc_of(sK(s));
+      const uint32_t to = tmem + C::col_s(g, buf);
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
           tc_mma_ss(to, q_desc + ((kk >> 2) * (kBM * 128) + (kk & 3) * 32) / 16,
                     k_desc + ((kk >> 2) * (kBN * 128) + (kk & 3) * 32) / 16, idesc_qk, kk > 0 ? 1u : 0u);
         tc_commit(bar_s(g, buf));
-      };
-      auto kv_ready = [&](int t) -> bool {
-        if (!mbar_wait(&bars[C::kBarKVFull + t % ST], (t / ST) & 1, a.err)) return false;
-        tc_fence_after();
-        return true;
-      };
-      if (mw == 0) prefetch_tensormap(&qmap);
-      // The Q tiles of work wk (the CTA's lw'th) into its buffer.
-      auto load_q = [&](const Work& wk, int lw) -> bool {
-        const int qb = lw & 1, use = lw >> 1;
-        if (use > 0 && !mbar_wait(&bars[C::kBarQFree + qb], (use - 1) & 1, a.err)) return false;
+      }
+    };
+    auto kv_ready = [&](int t) -> bool {
+      if (!warp_wait(&bars[C::kBarKVFull + t % ST], (t / ST) & 1, a.err)) return false;
+      tc_fence_after();
+      return true;
+    };
+    if (mw == 0 && elect_one()) prefetch_tensormap(&qmap);
+    // The Q tiles of work wk (the CTA's lw'th) into its buffer.
+    auto load_q = [&](const Work& wk, int lw) -> bool {
+      const int qb = lw & 1, use = lw >> 1;
+      if (use > 0 && !warp_wait(&bars[C::kBarQFree + qb], (use - 1) & 1, a.err)) return false;
+      if (elect_one()) {
         mbar_arrive_expect_tx(&bars[C::kBarQFull + qb], wk.n_g * C::kQBytes);
         for (int g = 0; g < wk.n_g; ++g)
           for (int x = 0; x < D; x += 64)
             tma_load_3d(sQ(qb, g) + x * kBM * 2, &qmap, x, wk.head0 + g, wk.qs + wk.m0, &bars[C::kBarQFull + qb]);
-        return true;
-      };
-      auto next_work = [&](int& w0) -> Work {  // the next work of this CTA that has tiles
-        Work wk{};
-        for (wk.valid = false; w0 < a.n_works; w0 += gridDim.x) {
-          wk = decode_work<NH>(a, work_of(w0, a.n_works));
-          if (wk.valid && wk.t0 < wk.t1) break;
-          wk.valid = false;
-        }
-        return wk;
-      };
-      bool ok = true;
-      int w0 = 0, loaded = 0;  // works whose Q is on its way
-      Work wk = next_work(w0);
-      if (wk.valid && mw == 0) ok = load_q(wk, 0), loaded = 1;
-      while (wk.valid && ok) {
-        w0 += gridDim.x;
-        const Work nextw = next_work(w0);
-        const int qb = lw & 1, n = wk.t1 - wk.t0, n_g = min(2, wk.n_g - 2 * mw);  // (none or fewer: this warp only counts along)
-        ok = mbar_wait(&bars[C::kBarQFull + qb], (lw >> 1) & 1, a.err) && kv_ready(kt);
-        if (!ok) break;
-        // S_g(0) may overwrite columns that an earlier PV_g reads P from: MMAs run in issue order.
+      }
+      return true;
+    };
+    auto next_work = [&](int& w0) -> Work {  // the next work of this CTA that has tiles
+      Work wk{};
+      for (wk.valid = false; w0 < a.n_works; w0 += gridDim.x) {
+        wk = decode_work<NH>(a, work_of(w0, a.n_works));
+        if (wk.valid && wk.t0 < wk.t1) break;
+        wk.valid = false;
+      }
+      return wk;
+    };
+    bool ok = true;
+    int w0 = 0, loaded = 0;  // works whose Q is on its way
+    Work wk = next_work(w0);
+    if (wk.valid && mw == 0) ok = load_q(wk, 0), loaded = 1;
+    while (wk.valid && ok) {
+      w0 += gridDim.x;
+      const Work nextw = next_work(w0);
+      const int qb = lw & 1, n = wk.t1 - wk.t0, n_g = min(2, wk.n_g - 2 * mw);  // (none or fewer: this warp only counts along)
+      ok = warp_wait(&bars[C::kBarQFull + qb], (lw >> 1) & 1, a.err) && kv_ready(kt);
+      if (!ok) break;
+      // S_g(0) may overwrite columns that an earlier PV_g reads P from: MMAs run in issue order.
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i < n_g) qk(i, h_tiles[i] % SB, qb, kt % ST);
-        for (int j = 0; j < n && ok; ++j, ++kt) {
-          const bool more = j + 1 < n;
-          if (more) ok = kv_ready(kt + 1);
-          if (SB == 2 && more && ok)  // the next S during this tile's softmax
+      for (int i = 0; i < 2; ++i)
+        if (i < n_g) qk(i, h_tiles[i] % SB, qb, kt % ST);
+      for (int j = 0; j < n && ok; ++j, ++kt) {
+        const bool more = j + 1 < n;
+        if (more) ok = kv_ready(kt + 1);
+        if (SB == 2 && more && ok)  // the next S during this tile's softmax
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (i < n_g) qk(i, (h_tiles[i] + 1) % SB, qb, (kt + 1) % ST);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (i >= n_g || !ok) break;
-            // O_g += P_g V once head g's softmax has written P_g; the work's first PV overwrites O_g, so it also
-            // waits for the epilogue of the work before to have read it.
-            const int g = 2 * mw + i, buf = h_tiles[i] % SB;
-            if (j == 0 && h_works[i] > 0) ok = mbar_wait(&bars[C::kBarODrained + g], (h_works[i] - 1) & 1, a.err);
-            if (ok) ok = mbar_wait(bar_p(g, buf), (h_tiles[i] / SB) & 1, a.err);
-            if (!ok) break;
-            ++h_tiles[i];
-            tc_fence_after();
-            const uint64_t v_desc = desc_of(sV(kt % ST));
-#pragma unroll
-            for (int kk = 0; kk < kBN / 16; ++kk)
-              tc_mma_ts(tmem + C::col_o(g), tmem + C::col_s(g, buf) + kk * 8, v_desc + kk * 2,
-                        idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-            if (SB == 2) tc_commit(&bars[C::kBarPV + g]);
-            if (SB == 1 && more) qk(i, 0, qb, (kt + 1) % ST);
-          }
-          tc_commit(&bars[C::kBarKVEmpty + kt % ST]);  // K and V of this stage are consumed
-          // the next work's Q, once the work before this one is done with the buffer (its last MMAs are issued)
-          if (j == 0 && ok && mw == 0 && nextw.valid) {
-            ok = load_q(nextw, lw + 1);
-            loaded = lw + 2;
-          }
-        }
-        if (!ok) break;
-        tc_commit(&bars[C::kBarQFree + qb]);  // every QK of this work has read its Q tiles
+          for (int i = 0; i < 2; ++i)
+            if (i < n_g) qk(i, (h_tiles[i] + 1) % SB, qb, (kt + 1) % ST);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (i >= n_g) break;
-          tc_commit(&bars[C::kBarODone + 2 * mw + i]);
-          ++h_works[i];
+          if (i >= n_g || !ok) break;
+          // O_g += P_g V once head g's softmax has written P_g; the work's first PV overwrites O_g, so it also
+          // waits for the epilogue of the work before to have read it.
+          const int g = 2 * mw + i, buf = h_tiles[i] % SB;
+          if (j == 0 && h_works[i] > 0) ok = warp_wait(&bars[C::kBarODrained + g], (h_works[i] - 1) & 1, a.err);
+          if (ok) ok = warp_wait(bar_p(g, buf), (h_tiles[i] / SB) & 1, a.err);
+          if (!ok) break;
+          ++h_tiles[i];
+          tc_fence_after();
+          const uint64_t v_desc = desc_of(sV(kt % ST));
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kBN / 16; ++kk)
+              tc_mma_ts(tmem + C::col_o(g), tmem + C::col_s(g, buf) + kk * 8, v_desc + kk * 2, idesc_pv,
+                        (j > 0 || kk > 0) ? 1u : 0u);
+            if (SB == 2) tc_commit(&bars[C::kBarPV + g]);
+          }
+          if (SB == 1 && more) qk(i, 0, qb, (kt + 1) % ST);
         }
-        ++lw;
-        wk = nextw;
+        if (elect_one()) tc_commit(&bars[C::kBarKVEmpty + kt % ST]);  // K and V of this stage are consumed
+        // the next work's Q, once the work before this one is done with the buffer (its last MMAs are issued)
+        if (j == 0 && ok && mw == 0 && nextw.valid) {
+          ok = load_q(nextw, lw + 1);
+          loaded = lw + 2;
+        }
       }
-      // Q tiles in flight end before the CTA does (bounded)
-      if (!ok)
-        for (int i = max(0, loaded - 2); i < loaded; ++i) mbar_wait(&bars[C::kBarQFull + (i & 1)], (i >> 1) & 1, a.err);
+      if (!ok) break;
+      if (elect_one()) tc_commit(&bars[C::kBarQFree + qb]);  // every QK of this work has read its Q tiles
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i >= n_g) break;
+        if (elect_one()) tc_commit(&bars[C::kBarODone + 2 * mw + i]);
+        ++h_works[i];
+      }
+      ++lw;
+      wk = nextw;
     }
-    __syncwarp();
+    // Q tiles in flight end before the CTA does (bounded)
+    if (!ok)
+      for (int i = max(0, loaded - 2); i < loaded; ++i) warp_wait(&bars[C::kBarQFull + (i & 1)], (i >> 1) & 1, a.err);
   } else {
     // ================= softmax / correction / epilogue of head g: thread = query row = TMEM lane
     const int g = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
