@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
           for (int u = 0; u < 8; ++u) {  // pair of keys 2u, 2u + 1: to pair 2 (u & 3) + (u >> 2) of the block's columns
             const int c = 16 * b + 2 * u;
             const float2 x = __ffma2_rn(make_float2(__uint_as_float(t[c]), __uint_as_float(t[c + 1])), f, add2);
-            const float2 e = poly_pair(c >> 1) ? exp2_poly2(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
             sum[u & 1] = __fadd2_rn(sum[u & 1], e);
             p[8 * b + 2 * (u & 3) + (u >> 2)] = pack2<false>(e.x, e.y);
           }
