@@ -7,21 +7,28 @@
 // without s_v: per block, sum(p') * (vref / s_v) / 2^6. vref is at least twice every s_v met so far (it moves rarely,
 // with the accumulators), so p' <= 2^13 fits fp16, which holds it to 2^-12 relative: below the output's rounding.
 //
-// Work. As the 16-bit prefill: persistent CTAs walk works, a work being a 128-row query tile of two heads of a KV group
-// (all of its keys, or one of n_splits stretches of them when there are fewer works than SMs). Warps:
-//   0..7    softmax, one warpgroup per head: thread = query row = TMEM lane. A tile is 64 keys (4 pages).
-//   converters (D = 64: the softmax warps themselves, while they would wait for S, each the keys or the values of one of
-//           the tile's pages; D = 128: four more warps, each a page): the block's codes straight from global memory (L2: the
-//           works that run at one time share their keys) through registers, widened, into the MMA operands: K [64 keys][D]
-//           and V transposed, [D][64 keys], both K-major with 128-byte swizzle. A block's value words hold the tokens
-//           2t, 2t+1, 2t+8, 2t+9 of a dim, so key 2t + (i & 1) + 8 (i >> 1) of a block is at place 4t + i of its V
-//           columns, and P is packed in that order. They run two tiles ahead, across works.
-//   last    MMA issuer (one thread): Q tiles by TMA into one of two buffers, S_g = Q_g K^T, O_g += P_g V with P read from
-//           TMEM.
-// D = 64: S and P share 64 columns, two CTAs per SM (four softmax chains hide each other's hand-offs; the exponentials
-// set the pace). D = 128: O takes 128 columns a head, so one CTA fills TMEM; S is double-buffered instead, and the next
-// tile's S is computed during a tile's softmax. Converting in one warp of its own (D = 64) took 232 us for 4 prompts of
-// 2048 tokens, 32/4 heads, where the same kernel without any conversion takes 138.
+// Work. Persistent CTAs walk works, a work being a 128-row query tile of two or four heads of a KV group over all of its
+// keys (or a part of them, see Walk). Warps:
+//   softmax, one warpgroup per head: thread = query row = TMEM lane. A tile is 64 keys (4 pages).
+//   converters: find the works, and bring each page's block straight from global memory (L2: the works that run at one time
+//           share their keys) through registers, widened, into the MMA operands: K [64 keys][D] and V transposed,
+//           [D][64 keys], both K-major with 128-byte swizzle. A block's value words hold the tokens 2t, 2t+1, 2t+8, 2t+9 of
+//           a dim, so key 2t + (i & 1) + 8 (i >> 1) of a block is at place 4t + i of its V columns, and P is packed in that
+//           order. They share the pages in turn and run up to three tiles ahead, across works. The first also hands the
+//           works on and loads their Q tiles by TMA into one of two buffers.
+//   last    MMA issuer: S_g = Q_g K^T, O_g += P_g V with P read from TMEM.
+// D = 64, groups of three heads or more: four heads a CTA (TMEM is then full: S and P share 64 columns a head), so a
+// converted tile serves four heads; three converting warps (with two, which also kept the pace of 4200 cycles a tile, 4
+// prompts of 2048 tokens at 32/4 heads took 138 us, with three 125; a fourth would leave the others too few registers).
+// Smaller groups: two heads, two CTAs per SM. D = 128: two heads fill TMEM with S double-buffered, the next tile's S is
+// computed during a tile's softmax; four converting warps.
+// What bounds it: at D = 64 the chain S -> max -> exponentials -> P -> P V of a head (the SFU, 16 exponentials a clock, is
+// busy 50 % of the time, the tensor cores 25 %); at D = 128 the tensor cores' reading of Q and K from shared memory for
+// 64-key tiles (48 cycles an instruction where the product takes 32) beside the same chain. Measured: 4 prompts of 2048
+// tokens, 32/4 heads of 64: 125 us; one of 8192: 408 us, 670 TFLOP/s; at D = 128 540 us, 1000 TFLOP/s.
+// Taking the weights against the last tiles' maximum while this tile's is found (to shorten the chain) spilled registers:
+// 208 us. Polynomials for one exponential in 8, 4, 3: 145, 147, 151 us where none took 138. Fetching Q and finding works
+// in the issuing warp and the softmax warps cost 4000 cycles of a tile's 3900 at each work's start.
 //
 // Every mbarrier wait is bounded (nbl_device.cuh): a lost completion ends the CTA with kErrTimeout set.
 #include <algorithm>
@@ -43,18 +50,26 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: p may reach 2^8 before
 constexpr float kPShift = 6.0f;            // p' carries 2^6
 constexpr float kMinLv = -24.0f;           // smallest log2(s_v / vref) kept: below it a block adds nothing to fp16 weights
 
+constexpr int kRing = 4;                   // works handed from the first converting warp to the other roles
+
+// A work as the issuing and the softmax warps need it.
+struct alignas(16) Slot {
+  int t0, n, n_g, head0;  // first tile, tiles (0: no more works), heads, the first
+  int pos, row, live;     // position and row of the tile's first query token, rows of it
+  int part;               // which part of the work; + kLastPart: the last one
+};
+constexpr int kLastPart = 1 << 16;
+
 template <int D, int HEADS>
 struct PCfg {
   static constexpr int NH = HEADS;                      // heads of a CTA
   static constexpr int kCtas = D == 64 && NH == 2 ? 2 : 1;  // per SM
   static constexpr int SB = D == 64 ? 1 : 2;            // S buffers of a head
   static constexpr int ST = 3;                          // tiles of K and V operands
-  static constexpr int kConv = D == 128 ? 4 : NH / 2;   // converting warps
-  static constexpr int kConvPages = kTilePages / kConv; // pages of a tile that one of them converts
-  static constexpr int kAhead = D == 64 ? 2 : 1;        // pages whose codes are on their way
-  static constexpr int kMma = NH / 2;                   // issuing warps, two heads each
+  static constexpr int kConv = D == 128 ? 4 : NH == 4 ? 3 : 1;  // converting warps
+  static constexpr int kAhead = kConv == 1 ? 2 : 1;     // pages whose codes are on their way
   static constexpr int kWarpConv = 4 * NH, kWarpMma = kWarpConv + kConv;
-  static constexpr int kThreads = (kWarpMma + kMma) * 32;
+  static constexpr int kThreads = (kWarpMma + 1) * 32;
   static constexpr int kQBytes = kBM * D * 2;           // one head's Q tile: D / 64 parts of [128][64]
   static constexpr int kTileBytes = kBN * D * 2;        // K (or V) operand tile
   static constexpr int kBlock = block_bytes(D);
@@ -64,12 +79,29 @@ struct PCfg {
   static constexpr int kOffBar = kOffScale + ST * kTilePages * 16;
   static constexpr int kBarQFull = 0, kBarQFree = 2, kBarKVFull = 4, kBarKVEmpty = kBarKVFull + ST, kBarS = kBarKVEmpty + ST,
                        kBarP = kBarS + NH * SB, kBarODone = kBarP + NH * SB, kBarODrained = kBarODone + NH,
-                       kBarPV = kBarODrained + NH, kNumBars = kBarPV + NH;
+                       kBarPV = kBarODrained + NH, kBarWFull = kBarPV + NH, kBarWFree = kBarWFull + kRing, kNumBars = kBarWFree + kRing;
   static constexpr int kOffTmemSlot = kOffBar + ((kNumBars * 8 + 15) & ~15);
-  static constexpr int kSmemBytes = kOffTmemSlot + 16;
+  static constexpr int kOffRing = kOffTmemSlot + 16;
+  static constexpr int kSmemBytes = kOffRing + kRing * 32;
   static constexpr uint32_t kTmemCols = kCtas == 2 ? 256 : 512;
   __host__ __device__ static constexpr uint32_t col_s(int g, int buf) { return (g * SB + buf) * kBN; }
   __host__ __device__ static constexpr uint32_t col_o(int g) { return NH * SB * kBN + g * D; }
+};
+
+// n / d and n % d of n < 2^31 without a division: q = (high word of n m + n) >> l with l = ceil(log2 d) and
+// m = floor(2^32 (2^l - d) / d) + 1.
+struct Divisor {
+  uint32_t d = 1, m = 1, l = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t d) : d(d) {
+    while ((uint64_t(1) << l) < d) ++l;
+    m = static_cast<uint32_t>(((uint64_t(1) << l) - d << 32) / d) + 1;
+  }
+  __device__ __forceinline__ int split(int& n) const {  // n becomes the quotient; returns the remainder
+    const uint32_t x = static_cast<uint32_t>(n), q = (__umulhi(x, m) + x) >> l;
+    n = static_cast<int>(q);
+    return static_cast<int>(x - q * d);
+  }
 };
 
 struct PrefillArgs {
@@ -80,33 +112,32 @@ struct PrefillArgs {
   int* err;
   int64_t n_pages;
   int out_dtype;
-  int n_heads, n_kv_heads, group, n_hgroups, m_tiles, n_splits;
-  int n_works;  // query tiles x splits x items x KV heads x head pairs
+  int n_heads, n_kv_heads, group, n_hgroups, m_tiles;
+  int n_splits;  // > 1: tiles are dealt evenly (Walk), a work's parts to at most so many CTAs
+  Divisor by_hgroups, by_kv_heads, by_items;
+  int n_works;  // query tiles x items x KV heads x head groups
   float scale_log2;
 };
 
 struct Work {
-  int kvh, n_g, head0, qlen, pos0, qs, m0, t0, t1, n_item_pages, split;
+  int kvh, n_g, head0, qlen, pos0, qs, m0, t0, t1, n_item_pages;
+  int split;  // which part of the work this is
   const int32_t* pt_row;
-  bool valid;
+  bool valid, last;  // last: the work's last part
 };
 
 // Work w (-1: none); the same in every warp. Works are numbered with the query tile (latest, so heaviest, first) slowest,
-// then the split, the item, the KV head and the head pair: the works of a round are about equally long, whatever the
+// then the item, the KV head and the heads of the group: the works of a round are about equally long, whatever the
 // number of items (with the item slowest, 4 prompts of 2048 tokens left the busiest CTA with 1.6 times the mean).
 template <int NH>
 __device__ __forceinline__ Work decode_work(const PrefillArgs& a, int w) {
   Work k{};
   k.valid = false;
   if (w < 0) return k;
-  const int hg = w % a.n_hgroups;
-  w /= a.n_hgroups;
-  k.kvh = w % a.n_kv_heads;
-  w /= a.n_kv_heads;
-  const int item = w % a.it.n_items;
-  w /= a.it.n_items;
-  k.split = w % a.n_splits;
-  const int mt = a.m_tiles - 1 - w / a.n_splits;
+  const int hg = a.by_hgroups.split(w);
+  k.kvh = a.by_kv_heads.split(w);
+  const int item = a.by_items.split(w);
+  const int mt = a.m_tiles - 1 - w;
   k.n_g = min(NH, a.group - NH * hg);  // the last heads of a group may be fewer
   k.head0 = k.kvh * a.group + NH * hg;
   k.qlen = a.it.len[item];
@@ -122,11 +153,107 @@ __device__ __forceinline__ Work decode_work(const PrefillArgs& a, int w) {
     return k;
   }
   const int kv_end = static_cast<int>(min(kv_len, int64_t(k.pos0) + k.m0 + kBM));
-  const int n_tiles = (kv_end + kBN - 1) / kBN;
-  k.t0 = static_cast<int>(int64_t(n_tiles) * k.split / a.n_splits);
-  k.t1 = static_cast<int>(int64_t(n_tiles) * (k.split + 1) / a.n_splits);
+  k.t1 = (kv_end + kBN - 1) / kBN;
+  k.last = true;
   k.n_item_pages = static_cast<int>((kv_len + kPage - 1) / kPage);
   k.pt_row = a.it.page_table + int64_t(item) * a.it.pt_stride;
+  return k;
+}
+
+// Which works a CTA takes; every role walks the same. Many works: rounds of gridDim.x consecutive ones; CTA c takes work c
+// of even rounds and gridDim.x - 1 - c of odd ones (heavy and light query tiles of a round even out over two). Few: all
+// their tiles in a row are dealt in equal shares, so a CTA has the end of one work, perhaps whole ones, and the start of
+// another; the parts' results are joined afterwards (511 tokens over 16.4k, 32/8 heads of 128: 157 us; with each work's
+// tiles cut in two equal parts 165).
+struct Walk {
+  int w = 0;                         // next work (rounds: the round's first)
+  int round = 0;
+  int base = 0, x = 0, end = 0;      // dealt: tiles before work w, the CTA's next tile and its end
+  int share = 1;                     // tiles of a share; 0: one whole work instead
+};
+
+template <int NH>
+__device__ __forceinline__ Work next_work(const PrefillArgs& a, Walk& k) {
+  if (a.n_splits > 1 && k.share == 0) {
+    const Work wk = decode_work<NH>(a, k.w < a.n_works ? k.w : -1);
+    k.w = a.n_works;
+    return wk;
+  }
+  if (a.n_splits > 1) {
+    while (k.x < k.end && k.w < a.n_works) {
+      Work wk = decode_work<NH>(a, k.w++);
+      if (!wk.valid) continue;
+      const int n = wk.t1;
+      wk.t0 = k.x - k.base;
+      wk.t1 = min(n, k.end - k.base);
+      wk.split = k.x / k.share - k.base / k.share;
+      wk.last = wk.t1 == n;
+      k.x = k.base + wk.t1;
+      k.base += n;
+      return wk;
+    }
+  } else {
+    while (k.w < a.n_works) {
+      const int grid = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
+      const int w = k.w + ((k.round++ & 1) ? grid - 1 - c : c);
+      k.w += grid;
+      const Work wk = decode_work<NH>(a, w < a.n_works ? w : -1);
+      if (wk.valid) return wk;
+    }
+  }
+  Work none{};
+  none.valid = false;
+  return none;
+}
+
+// The CTA's share, by a whole warp: equal shares of all tiles, of at least kMinShare tiles (or a work) each, and so that no
+// work has more than n_splits parts. Starting on another work costs a CTA about kSwitch tiles; where short works make that
+// dearer than leaving CTAs idle, each work goes to a CTA of its own (one prompt of 1300 tokens would otherwise end with
+// works of two tiles).
+constexpr int kMinShare = 8, kSwitch = 3;
+template <int NH>
+__device__ __forceinline__ Walk deal(const PrefillArgs& a) {
+  const int lane = threadIdx.x & 31, n = a.m_tiles * a.it.n_items, per = a.n_kv_heads * a.n_hgroups;
+  auto tiles_of = [&](int p) -> int {  // of each of the `per` works of query tile and item p
+    if (p >= n) return 0;
+    const Work wk = decode_work<NH>(a, p * per);
+    return wk.valid ? wk.t1 : 0;
+  };
+  int total = 0, longest = 0, shortest = INT32_MAX;
+  for (int p0 = 0; p0 < n; p0 += 32) {
+    const int t = tiles_of(p0 + lane);
+    total += __reduce_add_sync(0xffffffffu, t) * per;
+    longest = max(longest, __reduce_max_sync(0xffffffffu, t));
+    shortest = min(shortest, __reduce_min_sync(0xffffffffu, t > 0 ? t : INT32_MAX));
+  }
+  Walk k;
+  const int grid = static_cast<int>(gridDim.x);
+  k.share = max(max((total + grid - 1) / grid, (longest + a.n_splits - 2) / (a.n_splits - 1)), max(1, min(kMinShare, longest)));
+  if (a.n_works <= grid && longest < k.share + kSwitch * ((k.share - 1) / shortest + 1)) {
+    k.share = 0;
+    k.w = static_cast<int>(blockIdx.x);
+    return k;
+  }
+  k.x = min(total, k.share * static_cast<int>(blockIdx.x));
+  k.end = min(total, k.x + k.share);
+  for (int p0 = 0, before = 0; p0 < n && k.x < k.end; p0 += 32) {
+    const int t = tiles_of(p0 + lane), mine = t * per;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > k.x);
+    if (hit) {
+      const int l = __ffs(hit) - 1, first = before + __shfl_sync(0xffffffffu, upto - mine, l), tl = __shfl_sync(0xffffffffu, t, l);
+      const int h = (k.x - first) / tl;
+      k.w = (p0 + l) * per + h;
+      k.base = first + h * tl;
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
   return k;
 }
 
@@ -184,11 +311,15 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars[C::kBarQFull + b], 1);
-      mbar_init(&bars[C::kBarQFree + b], C::kMma);
+      mbar_init(&bars[C::kBarQFree + b], 4 * NH);
+    }
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&bars[C::kBarWFull + i], 1);
+      mbar_init(&bars[C::kBarWFree + i], 4 * NH + 1);
     }
     for (int s = 0; s < ST; ++s) {
-      mbar_init(&bars[C::kBarKVFull + s], C::kConv);
-      mbar_init(&bars[C::kBarKVEmpty + s], C::kMma);
+      mbar_init(&bars[C::kBarKVFull + s], kTilePages);
+      mbar_init(&bars[C::kBarKVEmpty + s], 1);
     }
     for (int g = 0; g < NH; ++g) {
       for (int b = 0; b < SB; ++b) {
@@ -210,15 +341,17 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Rounds of gridDim.x consecutive works; CTA c takes work c of even rounds and gridDim.x - 1 - c of odd ones (heavy and
-  // light query tiles of a round even out over two), -1 past the end. Every role walks the same works, so the phase counts
-  // below agree: lw = this CTA's valid works so far (Q buffer lw & 1), kt = its tiles so far (stage kt % ST), and per
+  // The converting warps find the CTA's works; the first of them hands each to the other roles in a ring of kRing slots.
+  // Phases: lw = the CTA's works so far (Q buffer lw & 1, slot lw % kRing), kt = its tiles so far (stage kt % ST), and per
   // head the tiles and works that the head took part in.
-  auto work_of = [](int w0, int n_works) {
-    const int w = w0 + (((w0 / static_cast<int>(gridDim.x)) & 1)
-                            ? static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)
-                            : static_cast<int>(blockIdx.x));
-    return w < n_works ? w : -1;
+  Slot* ring = reinterpret_cast<Slot*>(smem + C::kOffRing);
+  auto take = [&](int lw, Slot& w) -> bool {  // by a whole warp
+    const int i = lw % kRing;
+    if (!warp_wait(&bars[C::kBarWFull + i], (lw / kRing) & 1, a.err)) return false;
+    w = ring[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars[C::kBarWFree + i]);
+    return true;
   };
   if (warp >= C::kWarpConv && warp < C::kWarpMma) {
     // ================= converters: a page at a time, in order across works; the codes of the next kAhead pages are on
@@ -227,18 +360,46 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
     constexpr int kA = C::kAhead, NB = kA + 1;
     const int cw = warp - C::kWarpConv;
     const int64_t pg_bytes = page_bytes(D, a.n_kv_heads);
+    Walk walk;
+    if (a.n_splits > 1) walk = deal<NH>(a);
+    int works = 0;  // handed on (first warp)
+    if (cw == 0 && elect_one()) prefetch_tensormap(&qmap);
+    // Hands a work on (one that is not valid: the end), its Q tiles on their way to their buffer.
+    auto publish = [&](const Work& wk) -> bool {
+      const int i = works % kRing, qb = works & 1;
+      if (works >= kRing && !warp_wait(&bars[C::kBarWFree + i], ((works / kRing) & 1) ^ 1, a.err)) return false;
+      if (wk.valid && works >= 2 && !warp_wait(&bars[C::kBarQFree + qb], ((works >> 1) & 1) ^ 1, a.err)) return false;
+      if (elect_one()) {
+        Slot w{};
+        if (wk.valid)
+          w = Slot{wk.t0, wk.t1 - wk.t0, wk.n_g, wk.head0, wk.pos0 + wk.m0, wk.qs + wk.m0, wk.qlen - wk.m0,
+                   wk.split + (wk.last ? kLastPart : 0)};
+        ring[i] = w;
+        mbar_arrive(&bars[C::kBarWFull + i]);
+        if (wk.valid) {
+          mbar_arrive_expect_tx(&bars[C::kBarQFull + qb], wk.n_g * C::kQBytes);
+          for (int g = 0; g < wk.n_g; ++g)
+            for (int x = 0; x < D; x += 64)
+              tma_load_3d(sQ(qb, g) + x * kBM * 2, &qmap, x, wk.head0 + g, wk.qs + wk.m0, &bars[C::kBarQFull + qb]);
+        }
+      }
+      __syncwarp();
+      works += wk.valid;
+      return true;
+    };
+    bool run = true;
     uint4 raw[NB][kRaw];
     float2 scale[NB];
-    int meta[NB];  // tile of the CTA * 4 + page of this warp in it; -1: no more
-    // The page that is read next: round, place among the work's pages of this warp and their number, tile of the CTA; the
-    // work's first page and its end, the page table row, the KV head's place in a page, and the ids of 32 of the
-    // work's pages of this warp (lane = place % 32) and the next 32.
-    int w0 = -static_cast<int>(gridDim.x), at = 0, n = 1, kt = -1, page0 = 0, last = 0;
+    int meta[NB];  // tile of the CTA * 4 + page of the tile; -1: no more
+    // The page that is read next: its place among the work's pages and their number (0: no more works), the tile of the CTA
+    // before the work's first; the work's first page and its end, the page table row, the KV head's place in a page, and
+    // the ids of the 32 pages around it and the next 32 (lane = place % 32).
+    int at = cw - C::kConv, n = -1, kt = 0, page0 = 0, last = 0;
     int32_t ids = -1, ids2 = -1;
     const int32_t* pt_row = nullptr;
     const uint8_t* head = nullptr;
     auto read_ids = [&](int place) -> int32_t {
-      const int pg = page0 + place / C::kConvPages * kTilePages + place % C::kConvPages;
+      const int pg = page0 + place;
       if (place >= n || pg >= last) return -1;
       const int32_t id = pt_row[pg];
       if (id >= 0 && id < a.n_pages) return id;
@@ -248,26 +409,24 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
     auto read_next = [&](uint4 (&x)[kRaw], float2& sc, int& m) {
       m = -1;
       if (n == 0) return;
-      if (++at >= n) {
-        at = n = 0;
-        while (n == 0) {
-          w0 += gridDim.x;
-          if (w0 >= a.n_works) return;
-          const Work wk = decode_work<NH>(a, work_of(w0, a.n_works));
-          if (!wk.valid) continue;
-          n = (wk.t1 - wk.t0) * C::kConvPages, pt_row = wk.pt_row;
-          head = a.pool + int64_t(wk.kvh) * C::kBlock;
-          page0 = wk.t0 * kTilePages + cw * C::kConvPages, last = min(wk.n_item_pages, wk.t1 * kTilePages);
-        }
+      const int was = at >> 5;
+      at += C::kConv;
+      if (at >= n) {  // (a work has four pages or more, so every warp has some of each)
+        if (n > 0) at -= n, kt += n / kTilePages;
+        n = 0;
+        const Work wk = next_work<NH>(a, walk);
+        if (cw == 0 && !publish(wk)) run = false;
+        if (!wk.valid || !run) return;
+        n = (wk.t1 - wk.t0) * kTilePages, pt_row = wk.pt_row;
+        head = a.pool + int64_t(wk.kvh) * C::kBlock;
+        page0 = wk.t0 * kTilePages, last = min(wk.n_item_pages, wk.t1 * kTilePages);
         ids = read_ids(lane);
         ids2 = read_ids(32 + lane);
-      } else if ((at & 31) == 0) {
+      } else if ((at >> 5) != was) {
         ids = ids2;
-        ids2 = read_ids(at + 32 + lane);
+        ids2 = read_ids((at & ~31) + 32 + lane);
       }
-      const int step = at % C::kConvPages;
-      if (step == 0) ++kt;
-      m = kt * 4 + step;
+      m = kt * kTilePages + at;
       const int32_t id = __shfl_sync(0xffffffffu, ids, at & 31);
       sc = make_float2(0.f, 0.f);
       if (id < 0) {  // no such page: codes of 0
@@ -284,8 +443,8 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
     };
     // A page's codes as operands; false after a wait that gave up.
     auto write = [&](const uint4 (&x)[kRaw], float2 sc, int m) -> bool {
-      const int tile = m >> 2, st = m & 3, s = tile % ST, b = cw * C::kConvPages + st;  // b: page of the tile
-      if (st == 0 && tile >= ST && !warp_wait(&bars[C::kBarKVEmpty + s], ((tile / ST) & 1) ^ 1, a.err)) return false;
+      const int tile = m / kTilePages, b = m % kTilePages, s = tile % ST;
+      if (tile >= ST && !warp_wait(&bars[C::kBarKVEmpty + s], ((tile / ST) & 1) ^ 1, a.err)) return false;
       // keys: 16 dims of a token a piece, to its row's chunks 2c and 2c + 1
 #pragma unroll
       for (int k = 0; k < kRaw / 2; ++k) {
@@ -315,40 +474,38 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       const float ks = fmaxf(sc.x, 1e-34f), vs = fmaxf(sc.y, 1e-34f);
       const float4 out = make_float4(ks * (unit<KIND>() * a.scale_log2), __log2f(vs), __fdividef(1.f, vs), 0.f);
       if (lane == 0) scales[s * kTilePages + b] = out;
-      if (st == C::kConvPages - 1) {
-        fence_proxy_async_smem();  // the operands, for the tensor core
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[C::kBarKVFull + s]);
-      }
+      fence_proxy_async_smem();  // the operands, for the tensor core
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[C::kBarKVFull + s]);
       return true;
     };
 #pragma unroll
     for (int i = 0; i < kA; ++i) read_next(raw[i], scale[i], meta[i]);
-    for (bool run = true; run;) {
+    while (run) {
 #pragma unroll
       for (int h = 0; h < NB; ++h) {
         if (meta[h] < 0) run = false;
         if (!run) break;
         read_next(raw[(h + kA) % NB], scale[(h + kA) % NB], meta[(h + kA) % NB]);
-        run = write(raw[h], scale[h], meta[h]);
+        if (run) run = write(raw[h], scale[h], meta[h]);
       }
     }
+    // Q tiles in flight end before the CTA does (bounded)
+    for (int i = max(0, works - 2); i < works; ++i) warp_wait(&bars[C::kBarQFull + (i & 1)], (i >> 1) & 1, a.err);
   } else if (warp >= C::kWarpMma) {
-    // ================= MMA issuers: heads 2 mw and 2 mw + 1. The whole warp walks the loop and waits; one lane, always the
+    // ================= MMA issuer. The whole warp walks the loop and waits; one lane, always the
     // same, issues. The descriptors are then values of the warp, kept in uniform registers: with the loop inside one
     // lane's branch every instruction's operands were moved there one by one, which cost 80 cycles an instruction (511
     // tokens over 16.4k at head_dim 128: 241 us against 176).
-    const int mw = __shfl_sync(0xffffffffu, warp - C::kWarpMma, 0);
     constexpr uint32_t idesc_qk = make_idesc_f16(kBM, kBN, BF16, false, false);
     constexpr uint32_t idesc_pv = make_idesc_f16(kBM, D, false, false, false);
     int lw = 0, kt = 0;
-    int h_tiles[2] = {0, 0}, h_works[2] = {0, 0};  // per head: S tiles consumed, works finished
+    int h_tiles[NH] = {}, h_works[NH] = {};  // per head: S tiles consumed, works finished
     // descriptors differ in the address alone: 16-byte units, whose sums stay inside its 14 bits
     const uint64_t desc0 = make_sdesc(smem_u32(smem), 16, 1024, 2);
     auto desc_of = [&](const uint8_t* p) { return desc0 + (static_cast<uint32_t>(p - smem) >> 4); };
-    // S_g (buffer buf) = Q_g K^T from Q buffer qb and stage s, for head g = 2 mw + i.
-    auto qk = [&](int i, int buf, int qb, int s) {
-      const int g = 2 * mw + i;
+    // S_g (buffer buf) = Q_g K^T from Q buffer qb and stage s.
+    auto qk = [&](int g, int buf, int qb, int s) {
       const uint64_t q_desc = desc_of(sQ(qb, g)), k_desc = desc_of(sK(s));
       const uint32_t to = tmem + C::col_s(g, buf);
       if (elect_one()) {
@@ -364,59 +521,35 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       tc_fence_after();
       return true;
     };
-    if (mw == 0 && elect_one()) prefetch_tensormap(&qmap);
-    // The Q tiles of work wk (the CTA's lw'th) into its buffer.
-    auto load_q = [&](const Work& wk, int lw) -> bool {
-      const int qb = lw & 1, use = lw >> 1;
-      if (use > 0 && !warp_wait(&bars[C::kBarQFree + qb], (use - 1) & 1, a.err)) return false;
-      if (elect_one()) {
-        mbar_arrive_expect_tx(&bars[C::kBarQFull + qb], wk.n_g * C::kQBytes);
-        for (int g = 0; g < wk.n_g; ++g)
-          for (int x = 0; x < D; x += 64)
-            tma_load_3d(sQ(qb, g) + x * kBM * 2, &qmap, x, wk.head0 + g, wk.qs + wk.m0, &bars[C::kBarQFull + qb]);
-      }
-      return true;
-    };
-    auto next_work = [&](int& w0) -> Work {  // the next work of this CTA that has tiles
-      Work wk{};
-      for (wk.valid = false; w0 < a.n_works; w0 += gridDim.x) {
-        wk = decode_work<NH>(a, work_of(w0, a.n_works));
-        if (wk.valid && wk.t0 < wk.t1) break;
-        wk.valid = false;
-      }
-      return wk;
-    };
     bool ok = true;
-    int w0 = 0, loaded = 0;  // works whose Q is on its way
-    Work wk = next_work(w0);
-    if (wk.valid && mw == 0) ok = load_q(wk, 0), loaded = 1;
-    while (wk.valid && ok) {
-      w0 += gridDim.x;
-      const Work nextw = next_work(w0);
-      const int qb = lw & 1, n = wk.t1 - wk.t0, n_g = min(2, wk.n_g - 2 * mw);  // (none or fewer: this warp only counts along)
+    for (;; ++lw) {
+      Slot wk;
+      ok = take(lw, wk);
+      if (!ok || wk.n == 0) break;
+      const int qb = lw & 1, n = wk.n, n_g = wk.n_g;
       ok = warp_wait(&bars[C::kBarQFull + qb], (lw >> 1) & 1, a.err) && kv_ready(kt);
       if (!ok) break;
       // S_g(0) may overwrite columns that an earlier PV_g reads P from: MMAs run in issue order.
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (i < n_g) qk(i, h_tiles[i] % SB, qb, kt % ST);
+      for (int g = 0; g < NH; ++g)
+        if (g < n_g) qk(g, h_tiles[g] % SB, qb, kt % ST);
       for (int j = 0; j < n && ok; ++j, ++kt) {
         const bool more = j + 1 < n;
         if (more) ok = kv_ready(kt + 1);
         if (SB == 2 && more && ok)  // the next S during this tile's softmax
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (i < n_g) qk(i, (h_tiles[i] + 1) % SB, qb, (kt + 1) % ST);
+          for (int g = 0; g < NH; ++g)
+            if (g < n_g) qk(g, (h_tiles[g] + 1) % SB, qb, (kt + 1) % ST);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (i >= n_g || !ok) break;
+        for (int g = 0; g < NH; ++g) {
+          if (g >= n_g || !ok) break;
           // O_g += P_g V once head g's softmax has written P_g; the work's first PV overwrites O_g, so it also
           // waits for the epilogue of the work before to have read it.
-          const int g = 2 * mw + i, buf = h_tiles[i] % SB;
-          if (j == 0 && h_works[i] > 0) ok = warp_wait(&bars[C::kBarODrained + g], (h_works[i] - 1) & 1, a.err);
-          if (ok) ok = warp_wait(bar_p(g, buf), (h_tiles[i] / SB) & 1, a.err);
+          const int buf = h_tiles[g] % SB;
+          if (j == 0 && h_works[g] > 0) ok = warp_wait(&bars[C::kBarODrained + g], (h_works[g] - 1) & 1, a.err);
+          if (ok) ok = warp_wait(bar_p(g, buf), (h_tiles[g] / SB) & 1, a.err);
           if (!ok) break;
-          ++h_tiles[i];
+          ++h_tiles[g];
           tc_fence_after();
           const uint64_t v_desc = desc_of(sV(kt % ST));
           if (elect_one()) {
@@ -426,29 +559,18 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
                         (j > 0 || kk > 0) ? 1u : 0u);
             if (SB == 2) tc_commit(&bars[C::kBarPV + g]);
           }
-          if (SB == 1 && more) qk(i, 0, qb, (kt + 1) % ST);
+          if (SB == 1 && more) qk(g, 0, qb, (kt + 1) % ST);
         }
         if (elect_one()) tc_commit(&bars[C::kBarKVEmpty + kt % ST]);  // K and V of this stage are consumed
-        // the next work's Q, once the work before this one is done with the buffer (its last MMAs are issued)
-        if (j == 0 && ok && mw == 0 && nextw.valid) {
-          ok = load_q(nextw, lw + 1);
-          loaded = lw + 2;
-        }
       }
       if (!ok) break;
-      if (elect_one()) tc_commit(&bars[C::kBarQFree + qb]);  // every QK of this work has read its Q tiles
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (i >= n_g) break;
-        if (elect_one()) tc_commit(&bars[C::kBarODone + 2 * mw + i]);
-        ++h_works[i];
+      for (int g = 0; g < NH; ++g) {
+        if (g >= n_g) break;
+        if (elect_one()) tc_commit(&bars[C::kBarODone + g]);
+        ++h_works[g];
       }
-      ++lw;
-      wk = nextw;
     }
-    // Q tiles in flight end before the CTA does (bounded)
-    if (!ok)
-      for (int i = max(0, loaded - 2); i < loaded; ++i) warp_wait(&bars[C::kBarQFull + (i & 1)], (i >> 1) & 1, a.err);
   } else {
     // ================= softmax / correction / epilogue of head g: thread = query row = TMEM lane
     const int g = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
@@ -456,15 +578,19 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
     const uint32_t tO = tmem + C::col_o(g) + lane_off;
     int h_tiles = 0, h_works = 0, kt = 0;
     bool ok = true;
-    for (int w0 = 0; w0 < a.n_works && ok; w0 += gridDim.x) {
-      const Work wk = decode_work<NH>(a, work_of(w0, a.n_works));
-      if (!wk.valid) continue;
-      const int n = wk.t1 - wk.t0, kt0 = kt;
+    for (int lw = 0; ok; ++lw) {
+      Slot wk;
+      ok = take(lw, wk);
+      if (!ok || wk.n == 0) break;
+      const int n = wk.n, kt0 = kt;
       kt += n;
-      if (g >= wk.n_g) continue;
-      const int qpos = wk.pos0 + wk.m0 + r;
-      const int64_t orow = (int64_t(wk.qs) + wk.m0 + r) * a.n_heads + wk.head0 + g;
-      const bool live = wk.m0 + r < wk.qlen;
+      if (g >= wk.n_g) {
+        if (lane == 0) mbar_arrive(&bars[C::kBarQFree + (lw & 1)]);
+        continue;
+      }
+      const int qpos = wk.pos + r;
+      const int64_t orow = (int64_t(wk.row) + r) * a.n_heads + wk.head0 + g;
+      const bool live = r < wk.live;
       float m_ref = -INFINITY, l_run = 0.f;
       float lref = -INFINITY, vrefc = 0.f;  // log2 of vref, and vref / 2^6
       for (int j = 0; j < n; ++j, ++h_tiles) {
@@ -555,47 +681,61 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       }
       if (!ok) break;
       // ---- epilogue: O_g out of TMEM, normalised and stored; then the next work's first PV may overwrite it
-      if (m_ref == -INFINITY) l_run = 0.f;  // no key seen (a split past the row's position)
+      if (m_ref == -INFINITY) l_run = 0.f;  // no key seen (a part past the row's position)
       const float inv = l_run > 0.f ? vrefc * unit<KIND>() / l_run : 0.f;
-      if (n > 0) {
-        ok = warp_wait(&bars[C::kBarODone + g], h_works & 1, a.err);
-        if (!ok) break;
-        ++h_works;
-        tc_fence_after();
-      }
+      ok = warp_wait(&bars[C::kBarODone + g], h_works & 1, a.err);
+      if (!ok) break;
+      ++h_works;
+      tc_fence_after();
+      // through shared memory (the head's own Q tile, no longer read), so that 8 lanes store 128 bytes of a row: a lane
+      // storing its own row takes a cycle for each 16 bytes, 13000 a work for fp32 parts of four heads
+      const bool wide = a.n_splits > 1 || a.out_dtype == NBL_F32;
+      uint8_t* stage = sQ(lw & 1, g) + quarter * (32 * 128);
+      const int64_t row_bytes = int64_t(a.n_heads) * D * (wide ? 4 : 2);
+      uint8_t* dst = a.n_splits > 1
+                         ? reinterpret_cast<uint8_t*>(a.part_o + int64_t(wk.part & (kLastPart - 1)) * a.it.n_rows * a.n_heads * D)
+                         : static_cast<uint8_t*>(a.out);
+      dst += (int64_t(wk.row) + quarter * 32 + (lane >> 3)) * row_bytes + int64_t(wk.head0 + g) * D * (wide ? 4 : 2) + (lane & 7) * 16;
+      const int rows = wk.live - quarter * 32 - (lane >> 3);  // of this warp, from this lane's first on
+      auto put = [&](int chunk, uint4 v) { *reinterpret_cast<uint4*>(stage + swz128(lane, chunk)) = v; };
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
-        if (n > 0) {
-          tmem_ld32_wait(tO + c, o);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
-        }
-        if (c + 32 == D && n > 0) {
+        tmem_ld32_wait(tO + c, o);
+        if (c + 32 == D) {
           tc_fence_before();
           mbar_arrive(&bars[C::kBarODrained + g]);
         }
-        if (!live) continue;
-        if (a.n_splits > 1 || a.out_dtype == NBL_F32) {
-          float* base = a.n_splits > 1 ? a.part_o + int64_t(wk.split) * a.it.n_rows * a.n_heads * D : static_cast<float*>(a.out);
-          float4* dst = reinterpret_cast<float4*>(base + orow * D + c);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                 __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+        if (wide) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) put(i, make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
         } else {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + orow * D + c);
+          auto two = [&](int i) { return pack2<BF16>(__uint_as_float(o[i]), __uint_as_float(o[i + 1])); };
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            dst[i] = make_uint4(pack2<BF16>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv),
-                                pack2<BF16>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv),
-                                pack2<BF16>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv),
-                                pack2<BF16>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv));
+          for (int i = 0; i < 4; ++i) put((c & 32) / 8 + i, make_uint4(two(8 * i), two(8 * i + 2), two(8 * i + 4), two(8 * i + 6)));
+          if (!(c & 32)) continue;
         }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + swz128(4 * i + (lane >> 3), lane & 7));
+          if (4 * i < rows) *reinterpret_cast<uint4*>(dst + 4 * i * row_bytes) = v;
+        }
+        dst += 128;
+        __syncwarp();
       }
-      if (live && a.n_splits > 1)
-        a.part_lse[int64_t(wk.split) * a.it.n_rows * a.n_heads + orow] = l_run > 0.f ? m_ref + log2f(l_run) : -INFINITY;
+      fence_proxy_async_smem();  // the next Q tile in this place comes by TMA
+      if (lane == 0) mbar_arrive(&bars[C::kBarQFree + (lw & 1)]);
+      if (live && a.n_splits > 1) {
+        float* lse = a.part_lse + orow;
+        const int64_t step = a.it.n_rows * a.n_heads;
+        const int part = wk.part & (kLastPart - 1);
+        lse[part * step] = l_run > 0.f ? m_ref + log2f(l_run) : -INFINITY;
+        if (wk.part & kLastPart)
+          for (int p = part + 1; p < a.n_splits; ++p) lse[p * step] = -INFINITY;  // parts that the work does not have
+      }
     }
   }
   tc_fence_before();
@@ -606,7 +746,7 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
   }
 }
 
-// Joins the splits of each (token, head) row: part_lse in log2 units. A thread takes 4 dims.
+// Joins the parts of each (token, head) row: part_lse in log2 units. A thread takes 4 dims.
 template <int D>
 __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse,
                                                                 int n_splits, const Kv8Items it, int n_heads, void* out,
@@ -681,16 +821,19 @@ Kv8PrefillPlan plan_kv8_prefill(const nbl_kv* kv, int n_items, int max_len, int6
   const int group = n_heads / kv->cfg.n_kv_heads;
   const int64_t m_tiles = (max_len + kBM - 1) / kBM;
   const int heads = heads_of(kv->cfg.head_dim, group);
-  const int64_t pairs = int64_t(n_items) * kv->cfg.n_kv_heads * ((group + heads - 1) / heads) * m_tiles;
+  const int64_t works = int64_t(n_items) * kv->cfg.n_kv_heads * ((group + heads - 1) / heads) * m_tiles;
   const int64_t slots = int64_t(num_sms) * (kv->cfg.head_dim == 64 && heads == 2 ? 2 : 1);
-  // Fewer works than CTAs: split the keys, each stretch at least 8 tiles.
-  int64_t splits = 1;
-  if (pairs < slots) splits = std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(pairs, 1), max_kv / (8 * kBN)));
-  p.n_splits = static_cast<int>(std::min<int64_t>(splits, 64));
-  const int64_t works = pairs * p.n_splits;
   if (works > INT32_MAX) fail(NBL_E_INVALID, "prefill: items * heads * query tiles exceeds 2^31 works");
   p.n_works = static_cast<int>(works);
   p.grid = static_cast<int>(std::min<int64_t>(works, slots));
+  // A quarter of the CTAs or more without a work, and keys enough to share them: dealt, with room for the parts that equal
+  // works have. (With 144 works on 148 SMs dealing took 96 us where a work each takes 72; one prompt of 1300 tokens, whose
+  // works end up whole anyway, 57 us with the joining kernel and 46 without.)
+  const int64_t max_tiles = (max_kv + kBN - 1) / kBN;
+  if (4 * works <= 3 * slots && max_tiles >= 4 * kMinShare && max_tiles * 4 * slots < INT32_MAX) {
+    p.n_splits = static_cast<int>(std::min({(slots + works - 1) / works + 1, max_tiles / kMinShare + 2, int64_t(64)}));
+    p.grid = static_cast<int>(slots);
+  }
   if (p.n_splits > 1)
     p.scratch_bytes = size_t(p.n_splits) * size_t(n_rows) * size_t(n_heads) * (kv->cfg.head_dim + 1) * sizeof(float);
   return p;
@@ -723,6 +866,9 @@ void launch_kv8_prefill(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items
   a.m_tiles = (items.max_len + kBM - 1) / kBM;
   a.n_splits = plan.n_splits;
   a.n_works = plan.n_works;
+  a.by_hgroups = Divisor(a.n_hgroups);
+  a.by_kv_heads = Divisor(a.n_kv_heads);
+  a.by_items = Divisor(items.n_items);
   a.scale_log2 = 1.4426950408889634f / std::sqrt(static_cast<float>(d));
   if (d == 128) launch_d<128, 2>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
   else if (heads == 4) launch_d<64, 4>(st, c.dtype, q_dtype == NBL_BF16, qmap, a, plan.grid);
