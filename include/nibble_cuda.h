@@ -319,7 +319,8 @@ NBL_API int nbl_attn_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int3
  * every q_len. In a page that already holds tokens, s = max(old scale, largest new magnitude / 127 (I8) or 448 (E4M3)):
  * when the scale grows the old codes are rounded again to it (at most half a step of the new scale each time).
  * Magnitudes below 1e-30 in a whole page are stored as 0; an infinity or NaN is stored saturated or as 0 and flagged
- * (nbl_ctx_check). A page may be written by one item only in a call. */
+ * (nbl_ctx_check). A page may be written by one item only in a call, and the items' rows do not overlap. An item with
+ * rows, positions or a length out of bounds is left out and flagged. */
 NBL_API int nbl_rotary_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const void* k_in, const void* v_in,
                                  int32_t in_dtype, const float* bq, const float* bk, const float* bv, void* q_out,
                                  int32_t q_out_dtype, int64_t n_rows, const int32_t* q_start, const int32_t* q_len,
@@ -327,7 +328,7 @@ NBL_API int nbl_rotary_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, con
                                  int32_t n_heads, int32_t max_q_len, const nbl_rotary_params* rotary);
 /* The values that an 8-bit pool stands for: item i's positions kv_pos0[i] .. + len[i] as rows start[i].. of k_out / v_out
  * ([n_rows, n_kv_heads, head_dim] of out_dtype; either may be NULL), code * scale rounded once. max_len bounds every
- * len. */
+ * len; the items' rows do not overlap. */
 NBL_API int nbl_kv_read(nbl_ctx* ctx, const nbl_kv* kv, int64_t n_rows, const int32_t* start, const int32_t* len,
                         const int32_t* kv_pos0, const int32_t* page_table, int32_t pt_stride, int32_t n_items,
                         int32_t max_len, void* k_out, void* v_out, int32_t out_dtype);

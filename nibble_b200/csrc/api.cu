@@ -340,8 +340,8 @@ void kv8_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype,
   it.n_rows = n_q_rows;
   const int max_kv = pt_stride * kv->cfg.page_size;
   const bool aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
-  if (q_dtype == NBL_F32 || !aligned || max_q_len <= nbl::kKv8FewTokens || n_items > 65535 ||
-      n_q_rows * n_heads >= (int64_t(1) << 31)) {
+  const bool few = nbl::kv8_few_tokens(kv->cfg.head_dim, n_heads / kv->cfg.n_kv_heads, max_q_len);
+  if (q_dtype == NBL_F32 || !aligned || few || n_items > 65535 || n_q_rows * n_heads >= (int64_t(1) << 31)) {
     kv8_attention(ctx, kv, it, q, q_dtype, n_heads, out, out_dtype, nullptr, max_kv);
     return;
   }

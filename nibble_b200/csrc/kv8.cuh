@@ -187,8 +187,15 @@ void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, c
                      void* out, int out_dtype, float* lse, const Kv8AttnPlan& plan, void* scratch, unsigned* counts,
                      int* err);
 
-// Longest query stretch that the warp-level kernel takes; longer ones go to the tcgen05 one.
-constexpr int kKv8FewTokens = 24;
+// Whether the warp-level kernel takes query stretches of max_len tokens (else the tcgen05 one): its time grows with the rows
+// (tokens x heads of a group) that share each key, the other's stays until they pass 128 tokens. Measured, warp-level against
+// tcgen05, 8 items at 4000 keys, heads of 64: 32/4 heads 27 / 37 / 60 us for 8 / 16 / 32 tokens against 68 / 68 / 72, 8/8
+// heads 39 for 64 tokens against 76. Heads of 128: one item at 16k, 32/8 heads, 41 / 50 / 75 for 8 / 16 / 32 against 54 / 54 /
+// 55; 8 items at 4000, 8/8 heads, 77 for 64 against 49.
+inline bool kv8_few_tokens(int head_dim, int group, int max_len) {
+  return head_dim == 64 ? max_len <= 64 && int64_t(max_len) * group <= 288
+                        : max_len <= 24 && int64_t(max_len) * group <= 72;
+}
 // kv8_prefill.cu: the same for many query tokens of 16-bit type (q and out 16-byte aligned) on the tensor cores. n_rows:
 // rows of q; split keys leave partial results in scratch.
 struct Kv8PrefillPlan {

@@ -238,7 +238,8 @@ __device__ __forceinline__ void query8_any(const void* src, void* dst, int64_t r
 // With one page an item at most (decode steps), or more than kScanItems items, page u is page u % max_blocks of item
 // u / max_blocks, and may be empty; otherwise every warp adds up the items' pages, 32 items at a time, and the grid is
 // bounded by the rows of the packed activations (24 prompts of 97..2047 tokens: 1085 pages in place of 3096, of which two
-// thirds were empty; an empty CTA still reads its item).
+// thirds were empty; an empty CTA still reads its item). Items whose rows overlap can have more pages
+// than that: the last CTA flags it.
 constexpr int kScanItems = 256;
 struct Page {
   int item, start, len, pos0, block;
@@ -247,7 +248,7 @@ struct Page {
 __host__ __device__ inline bool scanned(int n_items, int max_blocks) { return max_blocks > 1 && n_items <= kScanItems; }
 __device__ __forceinline__ bool item_ok(const Kv8Items& it, int start, int len, int pos0, int64_t tab_pos) {
   const int64_t end = int64_t(pos0) + len;
-  return pos0 >= 0 && start >= 0 && int64_t(start) + len <= it.n_rows && end <= int64_t(it.pt_stride) * kPage && end <= tab_pos;
+  return len <= it.max_len && pos0 >= 0 && start >= 0 && int64_t(start) + len <= it.n_rows && end <= int64_t(it.pt_stride) * kPage && end <= tab_pos;
 }
 __device__ __forceinline__ Page page_at(const Kv8Items& it, int max_blocks, int64_t tab_pos, int u, int* err) {
   Page p;
@@ -265,6 +266,7 @@ __device__ __forceinline__ Page page_at(const Kv8Items& it, int max_blocks, int6
     return p;
   }
   const int lane = threadIdx.x & 31;
+  const bool last = u == static_cast<int>(gridDim.x) - 1;
   int before = 0;
   for (int i0 = 0; i0 < it.n_items; i0 += 32) {
     const int i = i0 + lane;
@@ -283,17 +285,18 @@ __device__ __forceinline__ Page page_at(const Kv8Items& it, int max_blocks, int6
       if (lane >= o) inc += y;
     }
     const uint32_t at = __ballot_sync(0xffffffffu, u < before + inc);
-    if (at) {
+    if (at && !p.valid) {
       const int l = __ffs(at) - 1;  // the first item that ends behind u
       p.item = i0 + l;
       p.start = __shfl_sync(0xffffffffu, start, l), p.len = __shfl_sync(0xffffffffu, len, l);
       p.pos0 = __shfl_sync(0xffffffffu, pos0, l);
       p.block = p.pos0 / kPage + u - before - __shfl_sync(0xffffffffu, inc - n, l);
       p.valid = true;
-      return p;
+      if (!last) return p;
     }
     before += __shfl_sync(0xffffffffu, inc, 31);
   }
+  if (before > static_cast<int>(gridDim.x) && threadIdx.x == 0) flag_error(err, kErrLength);
   return p;
 }
 

@@ -486,6 +486,28 @@ def test_prefill_few_and_long(nbl_ctx, dtype, out_dtype, D):
         kv.close()
 
 
+@pytest.mark.parametrize("H,KV", [(4, 2), (5, 1), (12, 2), (3, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("items", [[(2500, 40), (0, 130), (3000, 257), (10, 1), (5, 0), (0, 400)], [(9001, 300)],
+                                   [(2000, 290), (0, 0), (2300, 150)], [(0, 2600)]])
+def test_prefill_few_ragged_items(nbl_ctx, H, KV, D, items):
+    """Fewer query tiles than SMs, of unlike lengths, groups that do not fill a CTA's heads: tiles dealt over the CTAs."""
+    table, n_pages = make_page_tables([p + m for p, m in items], shuffle_seed=H)
+    kv, values = random_pool(nbl_ctx, "e4m3", n_pages, KV, D, H, spread=0.5)
+    check_prefill(nbl_ctx, kv, values, table, items, H, "float16", H, stride=37)
+    kv.close()
+
+
+@pytest.mark.parametrize("H,KV,D", [(10, 2, 64), (6, 2, 128), (2, 2, 64)])
+def test_prefill_many_short_items(nbl_ctx, H, KV, D):
+    """More works than CTAs, most of one to three tiles."""
+    items = [(7 * i % 90, 65 + 17 * i % 130) for i in range(150)]
+    table, n_pages = make_page_tables([p + m for p, m in items], shuffle_seed=H)
+    kv, values = random_pool(nbl_ctx, "int8", n_pages, KV, D, H, spread=0.5)
+    check_prefill(nbl_ctx, kv, values, table, items, H, "bfloat16", H, stride=61)
+    kv.close()
+
+
 def test_attention_on_another_stream(nbl_ctx):
     import torch
     import nibble_b200 as nb
@@ -514,6 +536,23 @@ def test_repeated_calls_give_the_same_bits(nbl_ctx):
     for o in outs:
         nbl_ctx.attn_decode(kv, q, dev(table), ints(lens), 4000, o)
     assert all(torch.equal(outs[0], o) for o in outs)
+    kv.close()
+
+
+def test_append_items_out_of_bounds_are_flagged(nbl_ctx):
+    """Items longer than max_len, past the rows or the table, and so many that share rows that their pages exceed the launch."""
+    import torch
+    import nibble_b200 as nb
+    kv = nbl_ctx.kv_pool(64, 1, dtype=nb.I8)
+    x = torch.ones((160, 1, 64), device="cuda")
+    spec = nb.RotarySpec(1e4, True)
+    table = ints(np.arange(60).reshape(3, 20))
+    for start, length, pos0, most in [([0, 0, 0], [160, 160, 160], [0, 0, 0], 160), ([0, 0, 0], [1, 30, 1], [0, 0, 0], 20),
+                                      ([0, 150, 0], [1, 20, 1], [0, 0, 0], 20), ([0, 0, 0], [1, 20, 1], [0, 310, 0], 20),
+                                      ([0, -1, 0], [1, 20, 1], [0, 0, 0], 20), ([0, 0, 0], [1, 20, 1], [0, -1, 0], 20)]:
+        nbl_ctx.rotary_kv_append(kv, x, x, x, x.clone(), ints(start), ints(length), ints(pos0), table, most, spec)
+        with pytest.raises(nb.NibbleError):
+            nbl_ctx.check()
     kv.close()
 
 
