@@ -28,6 +28,11 @@
 // - A chunk's P V is accumulated from zero by the tensor cores and added to O in fp32: the tensor cores truncate, and
 //   over thousands of pages that shows (4e-6 relative at 131k tokens, 8e-7 this way). The addition is the
 //   multiply-add that rescales O anyway.
+//
+// Measured: 256 rows of 4097 tokens, 32/8 heads of 64: 187 us, 5.8 TB/s of codes and scales (90 % of the measured copy rate);
+// 4 rows of 131073, 32/8 heads of 128: 176 us, 6.1 TB/s (95 %); 48 rows of 511..16384, 28/4 heads of 128: 54 us, 4.2 TB/s: the
+// launch, the CTAs' search for their stretch, the first loads and the joining of partials take about 12 us of a call that
+// short. One row of 257 tokens: 10 us, the launch and one chain of loads.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
