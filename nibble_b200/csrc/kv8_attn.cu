@@ -29,10 +29,12 @@
 //   over thousands of pages that shows (4e-6 relative at 131k tokens, 8e-7 this way). The addition is the
 //   multiply-add that rescales O anyway.
 //
-// Measured: 256 rows of 4097 tokens, 32/8 heads of 64: 187 us, 5.8 TB/s of codes and scales (90 % of the measured copy rate);
-// 4 rows of 131073, 32/8 heads of 128: 176 us, 6.1 TB/s (95 %); 48 rows of 511..16384, 28/4 heads of 128: 54 us, 4.2 TB/s: the
-// launch, the CTAs' search for their stretch, the first loads and the joining of partials take about 12 us of a call that
-// short. One row of 257 tokens: 10 us, the launch and one chain of loads.
+// Measured: 256 rows of 4097 tokens, 32/8 heads of 64: 217 us, 5.0 TB/s of codes and scales (77 % of the measured copy rate)
+// with other pools of that size read in between, 187 us on the same pool again and again; 4 rows of 131073, 32/8 heads of 128:
+// 195 us, 5.5 TB/s (85 %), and 176; 48 rows of 511..16384, 28/4 heads of 128: 55 us, 4.1 TB/s: the launch, the CTAs' search
+// for their stretch, the first loads and the joining of partials take about 12 us of a call that short. One row of 257 tokens:
+// 9 us, the launch and one chain of loads. Walking the KV heads of the same pages side by side in neighbouring CTAs, for
+// the sake of whole pages: 217 and 199 us, and 18.4 against 16.8 for 8 items of 5 drafted tokens.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

@@ -27,8 +27,8 @@
 // 64-key tiles (48 cycles an instruction where the product takes 32) beside the same chain. Measured: 4 prompts of 2048
 // tokens, 32/4 heads of 64: 125 us; one of 8192: 408 us, 670 TFLOP/s; at D = 128 540 us, 1000 TFLOP/s.
 // Taking the weights against the last tiles' maximum while this tile's is found (to shorten the chain) spilled registers:
-// 208 us. Polynomials for one exponential in 8, 4, 3: 145, 147, 151 us where none took 138. Fetching Q and finding works
-// in the issuing warp and the softmax warps cost 4000 cycles of a tile's 3900 at each work's start.
+// 208 us. Polynomials for one exponential in 8, 4, 3: 145, 147, 151 us where none took 138. With the works found, and Q
+// fetched, by the issuing warp and the softmax warps each for itself, starting on a work took 4000 cycles, as long as a tile.
 //
 // Every mbarrier wait is bounded (nbl_device.cuh): a lost completion ends the CTA with kErrTimeout set.
 #include <algorithm>
