@@ -965,7 +965,10 @@ def main():
                 "vs_baseline": None, "data": "synthetic (seeded N(0,1))"})
     res["gpu_launches"] = res.pop("gpu_launches_per_step", 2) * args.steps
     if rank == 0 and world == 1 and args.cpu_seconds > 0 and args.workload == "decode_batched":
-        res["cpu_baseline"] = cpu_baseline(args.cpu_seconds)
+        try:
+            res["cpu_baseline"] = cpu_baseline(args.cpu_seconds)
+        except OSError as e:  # nibble's own backend could not be compiled: its sources are not there
+            res["cpu_baseline"] = {"unavailable": str(e)}
     if world > 1:
         import torch.distributed as dist
         dist.barrier()
