@@ -299,7 +299,8 @@ NBL_API int nbl_attn_decode_static(nbl_ctx* ctx, const nbl_kv* kv, const float* 
 /* Causal prefill (Backend::attention with n >= 1) over the paged pool for n_items independent items. q and out
  * hold n_q_rows rows of [n_heads, head_dim]. Item i: query rows q[q_start[i] .. q_start[i] + q_len[i])
  * (q_dtype = the pool dtype, already roped) at positions kv_pos0[i] + t, attending keys 0..kv_pos0[i]+t of
- * page-table row i (those keys must already be in the pool). max_q_len bounds every q_len[i]. Writes the
+ * page-table row i (those keys must already be in the pool). max_q_len bounds every q_len[i] (8-bit pools: an item
+ * with more, or with rows or positions out of bounds, is left out and flagged, see nbl_ctx_check). Writes the
  * items' out rows in out_dtype (F32 or the pool dtype). Tensor-core kernel (tcgen05): bf16/fp16 operands, fp32
  * accumulation in TMEM.
  * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes q in F32, F16 or BF16 and writes out in F32 or q's dtype;

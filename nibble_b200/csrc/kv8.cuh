@@ -152,6 +152,12 @@ struct Kv8Items {
   int n_items = 0, max_len = 0;
   int64_t n_rows = 0;  // rows of the packed activations
 };
+// Whether an item of len > 0 tokens is inside the launch (max_len), the activations and its page-table row; one that is
+// not is flagged and left out by every kernel.
+__device__ __forceinline__ bool item_fits(const Kv8Items& it, int start, int len, int pos0) {
+  return len <= it.max_len && pos0 >= 0 && start >= 0 && int64_t(start) + len <= it.n_rows &&
+         int64_t(pos0) + len <= int64_t(it.pt_stride) * kv8::kPage;
+}
 struct Kv8Append {
   const void *q_in = nullptr, *k_in = nullptr, *v_in = nullptr;
   const float *bq = nullptr, *bk = nullptr, *bv = nullptr;

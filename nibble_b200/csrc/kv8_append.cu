@@ -252,8 +252,7 @@ struct Page {
 };
 __host__ __device__ inline bool scanned(int n_items, int max_blocks) { return max_blocks > 1 && n_items <= kScanItems; }
 __device__ __forceinline__ bool item_ok(const Kv8Items& it, int start, int len, int pos0, int64_t tab_pos) {
-  const int64_t end = int64_t(pos0) + len;
-  return len <= it.max_len && pos0 >= 0 && start >= 0 && int64_t(start) + len <= it.n_rows && end <= int64_t(it.pt_stride) * kPage && end <= tab_pos;
+  return item_fits(it, start, len, pos0) && int64_t(pos0) + len <= tab_pos;
 }
 __device__ __forceinline__ Page page_at(const Kv8Items& it, int max_blocks, int64_t tab_pos, int u, int* err) {
   Page p;

@@ -188,7 +188,7 @@ __device__ __forceinline__ Item load_item(const AttnArgs& a, int i) {
   if (a.it.len) {
     x.q_start = a.it.start[i], x.q_len = a.it.len[i], x.pos0 = a.it.pos0[i];
     const int64_t kv = int64_t(x.pos0) + x.q_len;
-    const bool ok = x.pos0 >= 0 && x.q_start >= 0 && int64_t(x.q_start) + x.q_len <= a.it.n_rows && kv <= max_kv;
+    const bool ok = item_fits(a.it, x.q_start, x.q_len, x.pos0);
     if (x.q_len > 0 && !ok) flag_error(a.err, kErrLength);
     x.pages = x.q_len > 0 && ok ? static_cast<int>((kv + kPage - 1) / kPage) : 0;
     if (x.pages == 0) x.q_len = 0;

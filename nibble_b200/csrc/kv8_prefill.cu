@@ -147,7 +147,7 @@ __device__ __forceinline__ Work decode_work(const PrefillArgs& a, int w) {
   k.valid = k.qlen > 0 && k.m0 < k.qlen;
   if (!k.valid) return k;
   const int64_t kv_len = int64_t(k.pos0) + k.qlen;
-  if (k.pos0 < 0 || k.qs < 0 || int64_t(k.qs) + k.qlen > a.it.n_rows || kv_len > int64_t(a.it.pt_stride) * kPage) {
+  if (!item_fits(a.it, k.qs, k.qlen, k.pos0)) {
     flag_error(a.err, kErrLength);
     k.valid = false;
     return k;
@@ -753,9 +753,7 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const float* __r
                                                                 int out_dtype) {
   const int item = blockIdx.y;
   const int start = it.start[item], len = it.len[item], pos0 = it.pos0[item];
-  if (len <= 0 || pos0 < 0 || start < 0 || int64_t(start) + len > it.n_rows ||
-      int64_t(pos0) + len > int64_t(it.pt_stride) * kPage)
-    return;
+  if (len <= 0 || !item_fits(it, start, len, pos0)) return;
   const int64_t rows = it.n_rows * n_heads;
   for (int64_t u = blockIdx.x * 256ll + threadIdx.x; u < int64_t(len) * n_heads * (D / 4); u += gridDim.x * 256ll) {
     const int64_t row = int64_t(start) * n_heads + u / (D / 4);
