@@ -276,7 +276,9 @@ __global__ void __launch_bounds__(kExtendThreads) kv_extend_kernel(const PageBoo
 // ---- compact: a page's new id is its rank by first appearance in the tables (row by row): the first entry that names each
 // page (an integer minimum), the firsts of each row, their ranks, then the move. Latency bound up to the move, so each kernel
 // is launched while the one before still runs (all of whose CTAs have started then) and waits for its end before it reads
-// anything (128 rows, 458 MB moved: 96 -> 88 us).
+// anything (128 rows, 458 MB moved: 96 -> 88 us). What an earlier kernel of the chain writes comes through plain pointers and
+// is read with __ldcg: a const __restrict__ one would promise that it does not change while the kernel lives, and let the
+// compiler read it before the wait.
 __device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ int held_pages(const PageBook& b, int row, int* err) {
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(kThreads) compact_first_kernel(const PageBook 
   }
 }
 
-__global__ void __launch_bounds__(kThreads) compact_count_kernel(const PageBook b, const unsigned* __restrict__ first,
+__global__ void __launch_bounds__(kThreads) compact_count_kernel(const PageBook b, const unsigned* first,
                                                                  int32_t* counts, int32_t* refs_out, int64_t n_dst) {
   next_may_start();
   wait_for_previous();
@@ -309,15 +311,15 @@ __global__ void __launch_bounds__(kThreads) compact_count_kernel(const PageBook 
   for (int j = threadIdx.x; j < held; j += kThreads) {
     const int64_t at = int64_t(row) * b.pt_stride + j;
     const int32_t e = b.table[at];
-    mine += page_ok(b, e) && first[e] == static_cast<unsigned>(at);
+    mine += page_ok(b, e) && __ldcg(&first[e]) == static_cast<unsigned>(at);
   }
   int total;
   block_scan(mine, total);
   if (threadIdx.x == 0) counts[row] = total;
 }
 
-__global__ void __launch_bounds__(kThreads) compact_rank_kernel(const PageBook b, const unsigned* __restrict__ first,
-                                                                const int32_t* __restrict__ counts, int32_t* new_id,
+__global__ void __launch_bounds__(kThreads) compact_rank_kernel(const PageBook b, const unsigned* first,
+                                                                const int32_t* counts, int32_t* new_id,
                                                                 int32_t* source, int32_t* n_used, int64_t n_dst,
                                                                 int* err) {
   next_may_start();
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(kThreads) compact_rank_kernel(const PageBook b
   const int row = blockIdx.x, held = held_pages(b, row, nullptr);
   int sum = 0, all = 0;
   for (int r = threadIdx.x; r < b.n_rows; r += kThreads) {
-    const int c = counts[r];
+    const int c = __ldcg(&counts[r]);
     all += c;
     if (r < row) sum += c;
   }
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(kThreads) compact_rank_kernel(const PageBook b
     const int j = j0 + threadIdx.x;
     const int64_t at = int64_t(row) * b.pt_stride + j;
     const int32_t e = j < held ? b.table[at] : -1;
-    const bool lead = page_ok(b, e) && first[e] == static_cast<unsigned>(at);
+    const bool lead = page_ok(b, e) && __ldcg(&first[e]) == static_cast<unsigned>(at);
     int add;
     const int id = before + block_scan(lead, add);
     if (lead) {
@@ -352,9 +354,8 @@ __global__ void __launch_bounds__(kThreads) compact_rank_kernel(const PageBook b
 }
 
 // CTAs 0 .. n_rows - 1 also rewrite one table row each; all of them copy pages.
-__global__ void __launch_bounds__(kThreads) compact_move_kernel(const PageBook b, const int32_t* __restrict__ new_id,
-                                                                const int32_t* __restrict__ source,
-                                                                const int32_t* __restrict__ n_used, int64_t n_dst,
+__global__ void __launch_bounds__(kThreads) compact_move_kernel(const PageBook b, const int32_t* new_id,
+                                                                const int32_t* source, const int32_t* n_used, int64_t n_dst,
                                                                 int32_t* table_out, int32_t* refs_out,
                                                                 const uint8_t* __restrict__ from, uint8_t* __restrict__ to,
                                                                 int64_t page_bytes) {
@@ -364,15 +365,15 @@ __global__ void __launch_bounds__(kThreads) compact_move_kernel(const PageBook b
     for (int j = threadIdx.x; j < b.pt_stride; j += kThreads) {
       const int64_t at = int64_t(row) * b.pt_stride + j;
       const int32_t e = j < held ? b.table[at] : -1;
-      int32_t id = page_ok(b, e) ? new_id[e] : -1;
+      int32_t id = page_ok(b, e) ? __ldcg(&new_id[e]) : -1;
       if (id >= n_dst) id = -1;
       if (id >= 0) atomicAdd(&refs_out[id], 1);
       table_out[at] = id;
     }
   }
-  const int used = static_cast<int>(min(int64_t(*n_used), n_dst));
+  const int used = static_cast<int>(min(int64_t(__ldcg(n_used)), n_dst));
   for (int p = blockIdx.x; p < used; p += gridDim.x) {
-    const uint4* s = reinterpret_cast<const uint4*>(from + source[p] * page_bytes);
+    const uint4* s = reinterpret_cast<const uint4*>(from + __ldcg(&source[p]) * page_bytes);
     uint4* d = reinterpret_cast<uint4*>(to + p * page_bytes);
     for (int64_t u = threadIdx.x; u < page_bytes / 16; u += kThreads) d[u] = s[u];
   }
