@@ -390,6 +390,12 @@ class Context:
     def kv_read(self, kv: KVPool, start, length, kv_pos0, page_table, max_len: int, k_out=None, v_out=None):
         """Item i's positions kv_pos0[i].. as rows start[i].. of k_out / v_out [rows, n_kv_heads, D] (see nbl_kv_read)."""
         like = k_out if k_out is not None else v_out
+        if like is None:
+            raise ValueError("kv_read needs k_out or v_out")
+        want = (like.shape[0], kv.n_kv_heads, kv.head_dim)
+        if like.shape != want or (k_out is not None and v_out is not None and
+                                  (v_out.shape != want or v_out.dtype != k_out.dtype)):
+            raise ValueError(f"expected k_out and v_out [rows, {kv.n_kv_heads}, {kv.head_dim}] of one shape and dtype")
         check(_abi.lib.nbl_kv_read(self.handle, kv.handle, like.shape[0], _ptr(start), _ptr(length), _ptr(kv_pos0),
                                    _ptr(page_table), page_table.shape[-1], start.shape[0], max_len, _ptr(k_out),
                                    _ptr(v_out), _dtype(like)))

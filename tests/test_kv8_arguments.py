@@ -1,0 +1,68 @@
+"""What the Python calls of the 8-bit cache and of the page bookkeeping refuse before the library sees it: tensors of another type or
+size than the kernels read and write. Without a GPU: the library is a stand-in that records which calls reach it."""
+import pytest
+import torch
+
+import nibble_b200 as nb
+
+KV, D, PAGES = 2, 64, 9
+
+
+class Library:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *args: self.calls.append(name) or 0
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    fake = Library()
+    monkeypatch.setattr(nb._abi, "lib", fake, raising=False)
+    monkeypatch.setattr(nb, "_ptr", lambda t: None if t is None else 1)
+    return fake
+
+
+@pytest.fixture
+def ctx():
+    c = object.__new__(nb.Context)
+    c.handle, c.device = 1, 0
+    return c
+
+
+def pool(dtype=nb.I8, n_pages=PAGES):
+    kv = object.__new__(nb.KVPool)
+    kv.handle, kv.n_pages, kv.n_kv_heads, kv.head_dim, kv.page_size, kv.dtype = 1, n_pages, KV, D, 16, dtype
+    return kv
+
+
+def ints(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def refused(lib, call, *args, **kw):
+    lib.calls.clear()
+    with pytest.raises(ValueError):
+        call(*args, **kw)
+    assert not lib.calls
+
+
+def rows(n=5, heads=KV, dim=D, dtype=torch.float32):
+    return torch.zeros((n, heads, dim), dtype=dtype)
+
+
+def test_kv_read(ctx, lib):
+    def read(k=None, v=None):
+        ctx.kv_read(pool(), ints(3), ints(3), ints(3), ints(3, 4), 5, k, v)
+
+    for k, v in ((rows(), rows()), (rows(), None), (None, rows()), (rows(dtype=torch.half), rows(dtype=torch.half))):
+        read(k, v)
+    assert lib.calls == ["nbl_kv_read"] * 4
+    refused(lib, read)
+    refused(lib, read, rows(), rows(dtype=torch.half))  # v_out would be written as float32
+    refused(lib, read, rows(), rows(4))
+    refused(lib, read, rows(), rows(heads=1))
+    refused(lib, read, rows(dim=32), rows(dim=32))
+    refused(lib, read, None, rows(heads=4))
+    refused(lib, read, rows().reshape(-1), None)
