@@ -112,10 +112,26 @@ def _dtype(t) -> int:
     return code
 
 
-def _same_shape(kv, q, k, v):
-    want = (q.shape[0], kv.n_kv_heads, kv.head_dim)
-    if q.dim() != 3 or q.shape[2] != kv.head_dim or k.shape != want or v.shape != want:
-        raise ValueError(f"expected q [rows, n_heads, {kv.head_dim}] and k, v [rows, {kv.n_kv_heads}, {kv.head_dim}]")
+def _new_rows(kv, q, k, v, q_out):
+    """(rows, query heads) of tokens for kv: q and q_out [rows, heads, D], k and v [rows, kv heads, D]."""
+    shape = q.shape
+    want = (shape[0], kv.n_kv_heads, kv.head_dim)
+    if len(shape) != 3 or shape[2] != kv.head_dim or q_out.shape != shape or k.shape != want or v.shape != want:
+        raise ValueError(f"expected q_in, q_out [rows, n_heads, {kv.head_dim}] and k_in, v_in [rows, {kv.n_kv_heads}, {kv.head_dim}]")
+    return shape[0], shape[1]
+
+
+def _items(first, second, third, page_table):
+    """(items, table stride): three entries an item, and a page-table row at least."""
+    n, stride = first.numel(), page_table.shape[-1]
+    if second.numel() != n or third.numel() != n or page_table.numel() < n * stride:
+        raise ValueError("expected one start, length and first position per item, and a page-table row for each")
+    return n, stride
+
+
+def _check_bias(b, heads, dim):
+    if b is not None and (_dtype(b) != F32 or b.numel() != heads * dim):
+        raise ValueError(f"expected a float32 bias of {heads} * {dim} elements")
 
 
 class KVPool:
@@ -379,13 +395,16 @@ class Context:
         in_dt = _dtype(q_in)
         if _dtype(k_in) != in_dt or _dtype(v_in) != in_dt:
             raise ValueError("q_in, k_in, v_in must share a dtype")
-        _same_shape(kv, q_in, k_in, v_in)
+        n_rows, heads = _new_rows(kv, q_in, k_in, v_in, q_out)
+        n_items, stride = _items(q_start, q_len, kv_pos0, page_table)
+        for b, h in ((bq, heads), (bk, kv.n_kv_heads), (bv, kv.n_kv_heads)):
+            _check_bias(b, h, kv.head_dim)
         if rotary.freq_factors is not None and len(rotary.freq_factors) != (rotary.rotary_dim or kv.head_dim) // 2:
             raise ValueError("freq_factors must hold rotary_dim / 2 factors")
         check(_abi.lib.nbl_rotary_kv_append(
             self.handle, kv.handle, _ptr(q_in), _ptr(k_in), _ptr(v_in), in_dt, _ptr(bq), _ptr(bk), _ptr(bv),
-            _ptr(q_out), _dtype(q_out), q_in.shape[0], _ptr(q_start), _ptr(q_len), _ptr(kv_pos0), _ptr(page_table),
-            page_table.shape[-1], q_start.shape[0], q_in.shape[1], max_q_len, C.byref(p)))
+            _ptr(q_out), _dtype(q_out), n_rows, _ptr(q_start), _ptr(q_len), _ptr(kv_pos0), _ptr(page_table),
+            stride, n_items, heads, max_q_len, C.byref(p)))
 
     def kv_read(self, kv: KVPool, start, length, kv_pos0, page_table, max_len: int, k_out=None, v_out=None):
         """Item i's positions kv_pos0[i].. as rows start[i].. of k_out / v_out [rows, n_kv_heads, D] (see nbl_kv_read)."""
@@ -396,8 +415,9 @@ class Context:
         if like.shape != want or (k_out is not None and v_out is not None and
                                   (v_out.shape != want or v_out.dtype != k_out.dtype)):
             raise ValueError(f"expected k_out and v_out [rows, {kv.n_kv_heads}, {kv.head_dim}] of one shape and dtype")
+        n_items, stride = _items(start, length, kv_pos0, page_table)
         check(_abi.lib.nbl_kv_read(self.handle, kv.handle, like.shape[0], _ptr(start), _ptr(length), _ptr(kv_pos0),
-                                   _ptr(page_table), page_table.shape[-1], start.shape[0], max_len, _ptr(k_out),
+                                   _ptr(page_table), stride, n_items, max_len, _ptr(k_out),
                                    _ptr(v_out), _dtype(like)))
 
     def kv_import(self, kv: KVPool, page_ids, codes, scales):

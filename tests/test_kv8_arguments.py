@@ -66,3 +66,38 @@ def test_kv_read(ctx, lib):
     refused(lib, read, rows(dim=32), rows(dim=32))
     refused(lib, read, None, rows(heads=4))
     refused(lib, read, rows().reshape(-1), None)
+
+
+def test_append_outputs_biases_and_items(ctx, lib):
+    spec = nb.RotarySpec(1e4, False)
+
+    def append(q_out=None, items=(3, 3, 3), table=ints(3, 4), **biases):
+        q, k = rows(heads=4), rows()
+        ctx.rotary_kv_append(pool(), q, k, k, rows(heads=4) if q_out is None else q_out, *map(ints, items), table, 5, spec, **biases)
+
+    append()
+    append(bq=torch.zeros(4 * D), bk=torch.zeros(KV, D), bv=torch.zeros(KV * D))
+    append(q_out=rows(heads=4, dtype=torch.bfloat16), table=ints(7, 4))
+    assert len(lib.calls) == 3
+    refused(lib, append, q_out=rows(4, heads=4))
+    refused(lib, append, q_out=rows(heads=3))
+    refused(lib, append, q_out=rows(heads=4).reshape(-1))
+    for name, heads in (("bq", 4), ("bk", KV), ("bv", KV)):
+        refused(lib, append, **{name: torch.zeros(heads * D, dtype=torch.bfloat16)})  # was read as float32
+        refused(lib, append, **{name: torch.zeros(heads * D - 1)})
+    refused(lib, append, items=(3, 2, 3))
+    refused(lib, append, items=(3, 3, 2))
+    refused(lib, append, items=(2, 3, 3))
+    refused(lib, append, table=ints(2, 4))
+
+
+def test_kv_read_items(ctx, lib):
+    def read(items=(3, 3, 3), table=ints(3, 4)):
+        ctx.kv_read(pool(), *map(ints, items), table, 5, rows())
+
+    read()
+    read(table=ints(4, 4))
+    assert len(lib.calls) == 2
+    refused(lib, read, (3, 2, 3))
+    refused(lib, read, (3, 3, 1))
+    refused(lib, read, table=ints(2, 4))
