@@ -134,6 +134,21 @@ def _check_bias(b, heads, dim):
         raise ValueError(f"expected a float32 bias of {heads} * {dim} elements")
 
 
+_EIGHT_BITS = (I8, E4M3)
+
+
+def _check_pages(kv, page_ids, codes, scales):
+    """Import and export: one byte a code, every page whole. (A pool of another type is refused by the library.)"""
+    if kv.dtype not in _EIGHT_BITS:
+        return
+    want = (page_ids.numel(), 2, kv.n_kv_heads, kv.page_size, kv.head_dim)
+    types = ("int8", "uint8", "float8_e4m3fn") if kv.dtype == E4M3 else ("int8", "uint8")
+    if codes.shape != want or str(codes.dtype).replace("torch.", "") not in types:
+        raise ValueError(f"expected codes {list(want)} of {' or '.join(types)}")
+    if scales.shape != want[:3] or _dtype(scales) != F32:
+        raise ValueError(f"expected float32 scales {list(want[:3])}")
+
+
 class KVPool:
     """A paged K/V pool: pool[page][2][n_kv_heads][page_size][head_dim] (fp16 or bf16), or with dtype I8 / E4M3 8-bit
     codes with a scale per (page, K/V, head), in an order of the library's own (Context.kv_import / kv_export)."""
@@ -422,10 +437,13 @@ class Context:
 
     def kv_import(self, kv: KVPool, page_ids, codes, scales):
         """codes [n, 2, n_kv_heads, 16, D] (int8 / float8_e4m3fn) and scales [n, 2, n_kv_heads] fp32 into pages page_ids."""
+        _check_pages(kv, page_ids, codes, scales)
         check(_abi.lib.nbl_kv_import(self.handle, kv.handle, _ptr(page_ids), page_ids.shape[0], _ptr(codes),
                                      _ptr(scales)))
 
     def kv_export(self, kv: KVPool, page_ids, codes, scales):
+        """Pages page_ids into codes and scales, as kv_import takes them."""
+        _check_pages(kv, page_ids, codes, scales)
         check(_abi.lib.nbl_kv_export(self.handle, kv.handle, _ptr(page_ids), page_ids.shape[0], _ptr(codes),
                                      _ptr(scales)))
 

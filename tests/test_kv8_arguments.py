@@ -101,3 +101,25 @@ def test_kv_read_items(ctx, lib):
     refused(lib, read, (3, 2, 3))
     refused(lib, read, (3, 3, 1))
     refused(lib, read, table=ints(2, 4))
+
+
+@pytest.mark.parametrize("name", ["kv_import", "kv_export"])
+def test_import_and_export_pages(ctx, lib, name):
+    def call(kind=nb.I8, n=3, codes=(3, 2, KV, 16, D), dtype=torch.int8, scales=(3, 2, KV), scale_dtype=torch.float32):
+        getattr(ctx, name)(pool(kind), ints(n), torch.zeros(codes, dtype=dtype), torch.zeros(scales, dtype=scale_dtype))
+
+    call()
+    call(dtype=torch.uint8)
+    call(nb.E4M3, dtype=torch.float8_e4m3fn)
+    call(nb.E4M3)
+    assert len(lib.calls) == 4
+    refused(lib, call, n=4)  # more pages than codes
+    refused(lib, call, codes=(3, 2, KV, 16, 32))
+    refused(lib, call, codes=(3, 2, 1, 16, D))
+    refused(lib, call, codes=(3, 1, KV, 16, D))
+    refused(lib, call, dtype=torch.half)
+    refused(lib, call, dtype=torch.float8_e4m3fn)  # floats for a pool of integers
+    refused(lib, call, nb.E4M3, dtype=torch.float8_e5m2)
+    refused(lib, call, scales=(3, 2, 1))
+    refused(lib, call, scales=(2, 2, KV))
+    refused(lib, call, scale_dtype=torch.half)
