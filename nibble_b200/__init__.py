@@ -129,6 +129,14 @@ def _items(first, second, third, page_table):
     return n, stride
 
 
+def _book(kv, page_table, seq_lens, ref_counts, first, second):
+    """(table rows, stride, list entries): a length per table row, a count per page of the pool, lists of one length."""
+    (n_rows, stride), n = page_table.shape, first.numel()
+    if seq_lens.numel() < n_rows or ref_counts.numel() < kv.n_pages or second.numel() != n:
+        raise ValueError("expected seq_lens for every table row, ref_counts for every page, and lists of one length")
+    return n_rows, stride, n
+
+
 def _check_bias(b, heads, dim):
     if b is not None and (_dtype(b) != F32 or b.numel() != heads * dim):
         raise ValueError(f"expected a float32 bias of {heads} * {dim} elements")
@@ -450,32 +458,37 @@ class Context:
     # ---- page bookkeeping on the device (int32 CUDA tensors: page_table [rows, stride], seq_lens [rows],
     # ref_counts [n_pages])
     def kv_copy_pages(self, kv: KVPool, src_pages, dst_pages):
-        check(_abi.lib.nbl_kv_copy_pages(self.handle, kv.handle, _ptr(src_pages), _ptr(dst_pages), src_pages.shape[0]))
+        n = src_pages.numel()
+        if dst_pages.numel() != n:
+            raise ValueError("src_pages and dst_pages must have one length")
+        check(_abi.lib.nbl_kv_copy_pages(self.handle, kv.handle, _ptr(src_pages), _ptr(dst_pages), n))
 
     def kv_fork(self, kv: KVPool, page_table, seq_lens, ref_counts, src_rows, dst_rows):
         """Row dst_rows[i] becomes a branch of src_rows[i]: full pages shared, the part-filled one copied."""
-        check(_abi.lib.nbl_kv_fork(self.handle, kv.handle, _ptr(page_table), page_table.shape[-1], page_table.shape[0],
-                                   _ptr(seq_lens), _ptr(ref_counts), _ptr(src_rows), _ptr(dst_rows),
-                                   src_rows.shape[0]))
+        n_rows, stride, n = _book(kv, page_table, seq_lens, ref_counts, src_rows, dst_rows)
+        check(_abi.lib.nbl_kv_fork(self.handle, kv.handle, _ptr(page_table), stride, n_rows, _ptr(seq_lens),
+                                   _ptr(ref_counts), _ptr(src_rows), _ptr(dst_rows), n))
 
     def kv_release(self, kv: KVPool, page_table, seq_lens, ref_counts, rows):
-        check(_abi.lib.nbl_kv_release(self.handle, kv.handle, _ptr(page_table), page_table.shape[-1],
-                                      page_table.shape[0], _ptr(seq_lens), _ptr(ref_counts), _ptr(rows),
-                                      rows.shape[0]))
+        n_rows, stride, n = _book(kv, page_table, seq_lens, ref_counts, rows, rows)
+        check(_abi.lib.nbl_kv_release(self.handle, kv.handle, _ptr(page_table), stride, n_rows, _ptr(seq_lens),
+                                      _ptr(ref_counts), _ptr(rows), n))
 
     def kv_extend(self, kv: KVPool, page_table, seq_lens, ref_counts, rows, new_lens):
         """Row rows[i] gets the pages that new_lens[i] tokens need, lowest free ids first, and that length."""
-        check(_abi.lib.nbl_kv_extend(self.handle, kv.handle, _ptr(page_table), page_table.shape[-1],
-                                     page_table.shape[0], _ptr(seq_lens), _ptr(ref_counts), _ptr(rows),
-                                     _ptr(new_lens), rows.shape[0]))
+        n_rows, stride, n = _book(kv, page_table, seq_lens, ref_counts, rows, new_lens)
+        check(_abi.lib.nbl_kv_extend(self.handle, kv.handle, _ptr(page_table), stride, n_rows, _ptr(seq_lens),
+                                     _ptr(ref_counts), _ptr(rows), _ptr(new_lens), n))
 
     def kv_compact(self, src: KVPool, dst: KVPool, page_table, seq_lens, table_out, ref_counts_out, n_used):
         """The rows' pages move from pool src into pool dst, numbered by first appearance; src stays as it is."""
-        if table_out.shape != page_table.shape or ref_counts_out.shape[0] < dst.n_pages:
+        n_rows, stride = page_table.shape
+        if table_out.shape != page_table.shape or ref_counts_out.numel() < dst.n_pages:
             raise ValueError("table_out must have page_table's shape and ref_counts_out one count per page of dst")
-        check(_abi.lib.nbl_kv_compact(self.handle, src.handle, dst.handle, _ptr(page_table), page_table.shape[-1],
-                                      page_table.shape[0], _ptr(seq_lens), _ptr(table_out), _ptr(ref_counts_out),
-                                      _ptr(n_used)))
+        if seq_lens.numel() < n_rows or n_used.numel() < 1:
+            raise ValueError("expected seq_lens for every table row, and one element in n_used")
+        check(_abi.lib.nbl_kv_compact(self.handle, src.handle, dst.handle, _ptr(page_table), stride, n_rows,
+                                      _ptr(seq_lens), _ptr(table_out), _ptr(ref_counts_out), _ptr(n_used)))
 
     def lse_merge_packed(self, packed, n_parts: int, rows: int, head_dim: int, out, lse=None):
         """packed [n_parts, rows * (head_dim + 1)] fp32 (per part: outputs then lse) -> out [rows, head_dim]."""

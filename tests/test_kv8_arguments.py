@@ -123,3 +123,35 @@ def test_import_and_export_pages(ctx, lib, name):
     refused(lib, call, scales=(3, 2, 1))
     refused(lib, call, scales=(2, 2, KV))
     refused(lib, call, scale_dtype=torch.half)
+
+
+@pytest.mark.parametrize("name", ["kv_fork", "kv_extend", "kv_release"])
+def test_page_bookkeeping_arrays(ctx, lib, name):
+    def call(table=(4, 6), lens=4, refs=PAGES, first=2, second=2):
+        lists = [ints(first)] if name == "kv_release" else [ints(first), ints(second)]
+        getattr(ctx, name)(pool(nb.F16), ints(*table), ints(lens), ints(refs), *lists)
+
+    call()
+    call(lens=5, refs=PAGES + 1)
+    assert len(lib.calls) == 2
+    refused(lib, call, refs=PAGES - 1)  # counts past the end were read and written
+    refused(lib, call, lens=3)
+    refused(lib, call, table=(24,))
+    if name != "kv_release":
+        refused(lib, call, second=1)
+        refused(lib, call, first=1)
+
+
+def test_copy_and_compact_arrays(ctx, lib):
+    ctx.kv_copy_pages(pool(), ints(3), ints(3))
+
+    def compact(out=(4, 6), lens=4, refs=12, used=1):
+        ctx.kv_compact(pool(), pool(n_pages=12), ints(4, 6), ints(lens), ints(*out), ints(refs), ints(used))
+
+    compact()
+    assert lib.calls == ["nbl_kv_copy_pages", "nbl_kv_compact"]
+    refused(lib, ctx.kv_copy_pages, pool(), ints(3), ints(2))
+    refused(lib, compact, out=(6, 4))
+    refused(lib, compact, lens=3)
+    refused(lib, compact, refs=11)
+    refused(lib, compact, used=0)
