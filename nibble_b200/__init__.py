@@ -99,6 +99,18 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
+_int32: dict = {}  # torch.int32 -> True
+
+
+def _ints(t) -> int:
+    """Pointer to an int32 tensor: positions, lengths, page ids (another type's elements would be read as pairs of int32)."""
+    if not _int32.get(t.dtype):
+        if str(t.dtype) != "torch.int32":
+            raise ValueError(f"expected an int32 tensor, not {t.dtype}")
+        _int32[t.dtype] = True
+    return _ptr(t)
+
+
 _codes: dict = {}  # torch dtype -> element type code
 
 
@@ -426,7 +438,7 @@ class Context:
             raise ValueError("freq_factors must hold rotary_dim / 2 factors")
         check(_abi.lib.nbl_rotary_kv_append(
             self.handle, kv.handle, _ptr(q_in), _ptr(k_in), _ptr(v_in), in_dt, _ptr(bq), _ptr(bk), _ptr(bv),
-            _ptr(q_out), _dtype(q_out), n_rows, _ptr(q_start), _ptr(q_len), _ptr(kv_pos0), _ptr(page_table),
+            _ptr(q_out), _dtype(q_out), n_rows, _ints(q_start), _ints(q_len), _ints(kv_pos0), _ints(page_table),
             stride, n_items, heads, max_q_len, C.byref(p)))
 
     def kv_read(self, kv: KVPool, start, length, kv_pos0, page_table, max_len: int, k_out=None, v_out=None):
@@ -439,20 +451,20 @@ class Context:
                                   (v_out.shape != want or v_out.dtype != k_out.dtype)):
             raise ValueError(f"expected k_out and v_out [rows, {kv.n_kv_heads}, {kv.head_dim}] of one shape and dtype")
         n_items, stride = _items(start, length, kv_pos0, page_table)
-        check(_abi.lib.nbl_kv_read(self.handle, kv.handle, like.shape[0], _ptr(start), _ptr(length), _ptr(kv_pos0),
-                                   _ptr(page_table), stride, n_items, max_len, _ptr(k_out),
+        check(_abi.lib.nbl_kv_read(self.handle, kv.handle, like.shape[0], _ints(start), _ints(length), _ints(kv_pos0),
+                                   _ints(page_table), stride, n_items, max_len, _ptr(k_out),
                                    _ptr(v_out), _dtype(like)))
 
     def kv_import(self, kv: KVPool, page_ids, codes, scales):
         """codes [n, 2, n_kv_heads, 16, D] (int8 / float8_e4m3fn) and scales [n, 2, n_kv_heads] fp32 into pages page_ids."""
         _check_pages(kv, page_ids, codes, scales)
-        check(_abi.lib.nbl_kv_import(self.handle, kv.handle, _ptr(page_ids), page_ids.shape[0], _ptr(codes),
+        check(_abi.lib.nbl_kv_import(self.handle, kv.handle, _ints(page_ids), page_ids.shape[0], _ptr(codes),
                                      _ptr(scales)))
 
     def kv_export(self, kv: KVPool, page_ids, codes, scales):
         """Pages page_ids into codes and scales, as kv_import takes them."""
         _check_pages(kv, page_ids, codes, scales)
-        check(_abi.lib.nbl_kv_export(self.handle, kv.handle, _ptr(page_ids), page_ids.shape[0], _ptr(codes),
+        check(_abi.lib.nbl_kv_export(self.handle, kv.handle, _ints(page_ids), page_ids.shape[0], _ptr(codes),
                                      _ptr(scales)))
 
     # ---- page bookkeeping on the device (int32 CUDA tensors: page_table [rows, stride], seq_lens [rows],
@@ -461,24 +473,24 @@ class Context:
         n = src_pages.numel()
         if dst_pages.numel() != n:
             raise ValueError("src_pages and dst_pages must have one length")
-        check(_abi.lib.nbl_kv_copy_pages(self.handle, kv.handle, _ptr(src_pages), _ptr(dst_pages), n))
+        check(_abi.lib.nbl_kv_copy_pages(self.handle, kv.handle, _ints(src_pages), _ints(dst_pages), n))
 
     def kv_fork(self, kv: KVPool, page_table, seq_lens, ref_counts, src_rows, dst_rows):
         """Row dst_rows[i] becomes a branch of src_rows[i]: full pages shared, the part-filled one copied."""
         n_rows, stride, n = _book(kv, page_table, seq_lens, ref_counts, src_rows, dst_rows)
-        check(_abi.lib.nbl_kv_fork(self.handle, kv.handle, _ptr(page_table), stride, n_rows, _ptr(seq_lens),
-                                   _ptr(ref_counts), _ptr(src_rows), _ptr(dst_rows), n))
+        check(_abi.lib.nbl_kv_fork(self.handle, kv.handle, _ints(page_table), stride, n_rows, _ints(seq_lens),
+                                   _ints(ref_counts), _ints(src_rows), _ints(dst_rows), n))
 
     def kv_release(self, kv: KVPool, page_table, seq_lens, ref_counts, rows):
         n_rows, stride, n = _book(kv, page_table, seq_lens, ref_counts, rows, rows)
-        check(_abi.lib.nbl_kv_release(self.handle, kv.handle, _ptr(page_table), stride, n_rows, _ptr(seq_lens),
-                                      _ptr(ref_counts), _ptr(rows), n))
+        check(_abi.lib.nbl_kv_release(self.handle, kv.handle, _ints(page_table), stride, n_rows, _ints(seq_lens),
+                                      _ints(ref_counts), _ints(rows), n))
 
     def kv_extend(self, kv: KVPool, page_table, seq_lens, ref_counts, rows, new_lens):
         """Row rows[i] gets the pages that new_lens[i] tokens need, lowest free ids first, and that length."""
         n_rows, stride, n = _book(kv, page_table, seq_lens, ref_counts, rows, new_lens)
-        check(_abi.lib.nbl_kv_extend(self.handle, kv.handle, _ptr(page_table), stride, n_rows, _ptr(seq_lens),
-                                     _ptr(ref_counts), _ptr(rows), _ptr(new_lens), n))
+        check(_abi.lib.nbl_kv_extend(self.handle, kv.handle, _ints(page_table), stride, n_rows, _ints(seq_lens),
+                                     _ints(ref_counts), _ints(rows), _ints(new_lens), n))
 
     def kv_compact(self, src: KVPool, dst: KVPool, page_table, seq_lens, table_out, ref_counts_out, n_used):
         """The rows' pages move from pool src into pool dst, numbered by first appearance; src stays as it is."""
@@ -487,8 +499,8 @@ class Context:
             raise ValueError("table_out must have page_table's shape and ref_counts_out one count per page of dst")
         if seq_lens.numel() < n_rows or n_used.numel() < 1:
             raise ValueError("expected seq_lens for every table row, and one element in n_used")
-        check(_abi.lib.nbl_kv_compact(self.handle, src.handle, dst.handle, _ptr(page_table), stride, n_rows,
-                                      _ptr(seq_lens), _ptr(table_out), _ptr(ref_counts_out), _ptr(n_used)))
+        check(_abi.lib.nbl_kv_compact(self.handle, src.handle, dst.handle, _ints(page_table), stride, n_rows,
+                                      _ints(seq_lens), _ints(table_out), _ints(ref_counts_out), _ints(n_used)))
 
     def lse_merge_packed(self, packed, n_parts: int, rows: int, head_dim: int, out, lse=None):
         """packed [n_parts, rows * (head_dim + 1)] fp32 (per part: outputs then lse) -> out [rows, head_dim]."""

@@ -155,3 +155,28 @@ def test_copy_and_compact_arrays(ctx, lib):
     refused(lib, compact, lens=3)
     refused(lib, compact, refs=11)
     refused(lib, compact, used=0)
+
+
+def test_indices_are_int32(ctx, lib):
+    """64-bit tables, lengths or lists (what a torch index is by default) are refused wherever they come."""
+    kv, x, spec = pool(), rows(), nb.RotarySpec(1e4, False)
+    codes, scales = torch.zeros((3, 2, KV, 16, D), dtype=torch.int8), torch.zeros((3, 2, KV))
+    book = (ints(4, 6), ints(4), ints(PAGES))
+    calls = [  # (call, its index arguments)
+        (lambda *i: ctx.rotary_kv_append(kv, x, x, x, x, *i, 5, spec), (ints(3), ints(3), ints(3), ints(3, 4))),
+        (lambda *i: ctx.kv_read(kv, *i, 5, x), (ints(3), ints(3), ints(3), ints(3, 4))),
+        (lambda i: ctx.kv_import(kv, i, codes, scales), (ints(3),)),
+        (lambda i: ctx.kv_export(kv, i, codes, scales), (ints(3),)),
+        (lambda *i: ctx.kv_copy_pages(kv, *i), (ints(3), ints(3))),
+        (lambda *i: ctx.kv_fork(kv, *i), (*book, ints(2), ints(2))),
+        (lambda *i: ctx.kv_extend(kv, *i), (*book, ints(2), ints(2))),
+        (lambda *i: ctx.kv_release(kv, *i), (*book, ints(2))),
+        (lambda *i: ctx.kv_compact(kv, pool(), *i), (ints(4, 6), ints(4), ints(4, 6), ints(PAGES), ints(1))),
+    ]
+    for call, args in calls:
+        call(*args)
+    assert len(lib.calls) == len(calls)
+    for call, args in calls:
+        for k in range(len(args)):
+            for dtype in (torch.int64, torch.float32):
+                refused(lib, call, *args[:k], args[k].to(dtype), *args[k + 1:])
