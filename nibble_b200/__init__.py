@@ -396,6 +396,17 @@ class Context:
 
     def attn_decode(self, kv: KVPool, q, page_table, seq_lens, max_seq_len: int, out, lse=None, n_splits: int = 0):
         """One query token per row: q/out [rows, n_heads, head_dim] fp32, page_table [rows, stride] int32."""
+        if kv.dtype in _EIGHT_BITS:
+            (rows, heads, dim), (tables, stride), f32 = q.shape, page_table.shape, q.dtype
+            if dim != kv.head_dim or _dtype(q) != F32 or out.dtype != f32 or out.numel() < rows * heads * dim:
+                raise ValueError(f"expected float32 q and out [rows, n_heads, {kv.head_dim}]")
+            if tables < rows or seq_lens.numel() < rows:
+                raise ValueError("expected a length and a page-table row for each row of q")
+            if lse is not None and (lse.dtype != f32 or lse.numel() < rows * heads):
+                raise ValueError("expected a float32 lse [rows, n_heads]")
+            check(_abi.lib.nbl_attn_decode(self.handle, kv.handle, _ptr(q), _ints(page_table), stride, _ints(seq_lens),
+                                           max_seq_len, rows, heads, _ptr(out), _ptr(lse), n_splits))
+            return
         check(_abi.lib.nbl_attn_decode(self.handle, kv.handle, _ptr(q), _ptr(page_table), page_table.shape[-1],
                                        _ptr(seq_lens), max_seq_len, q.shape[0], q.shape[1], _ptr(out), _ptr(lse),
                                        n_splits))
@@ -415,7 +426,17 @@ class Context:
             q_in_h.shape[1], C.byref(p), out_h.data_ptr(), n_chunks))
 
     def attn_prefill(self, kv: KVPool, q, q_start, q_len, kv_pos0, page_table, max_q_len: int, out):
-        """Causal prefill: q [rows, n_heads, head_dim] (pool dtype), out [rows, n_heads, head_dim] fp32/pool dtype."""
+        """Causal prefill: q [rows, n_heads, head_dim] (pool dtype), out [rows, n_heads, head_dim] fp32/pool dtype.
+        (8-bit pools: q fp32, fp16 or bf16, out fp32 or q's dtype.)"""
+        if kv.dtype in _EIGHT_BITS:
+            rows, heads, dim = q.shape
+            if dim != kv.head_dim or out.numel() < rows * heads * dim:
+                raise ValueError(f"expected q and out [rows, n_heads, {kv.head_dim}]")
+            n, stride = _items(q_start, q_len, kv_pos0, page_table)
+            check(_abi.lib.nbl_attn_prefill(self.handle, kv.handle, _ptr(q), _dtype(q), rows, _ints(q_start),
+                                            _ints(q_len), _ints(kv_pos0), _ints(page_table), stride, n, heads,
+                                            max_q_len, _ptr(out), _dtype(out)))
+            return
         check(_abi.lib.nbl_attn_prefill(self.handle, kv.handle, _ptr(q), _dtype(q), q.shape[0], _ptr(q_start),
                                         _ptr(q_len), _ptr(kv_pos0), _ptr(page_table), page_table.shape[-1],
                                         q_start.shape[0], q.shape[1], max_q_len, _ptr(out), _dtype(out)))

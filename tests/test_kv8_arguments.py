@@ -180,3 +180,46 @@ def test_indices_are_int32(ctx, lib):
         for k in range(len(args)):
             for dtype in (torch.int64, torch.float32):
                 refused(lib, call, *args[:k], args[k].to(dtype), *args[k + 1:])
+
+
+def test_decode_queries_and_rows(ctx, lib):
+    def decode(q=None, out=None, lse=None, lens=ints(5), table=ints(5, 4)):
+        ctx.attn_decode(pool(), rows(heads=4) if q is None else q, table, lens, 60, rows(heads=4) if out is None else out, lse)
+
+    decode()
+    decode(lse=torch.zeros((5, 4)), lens=ints(6), table=ints(6, 4))
+    assert len(lib.calls) == 2
+    refused(lib, decode, q=rows(heads=4, dtype=torch.half))  # was read as float32
+    refused(lib, decode, out=rows(heads=4, dtype=torch.half))
+    refused(lib, decode, out=rows(4, heads=4))
+    refused(lib, decode, q=rows(heads=4, dim=128), out=rows(heads=4, dim=128))
+    refused(lib, decode, lse=torch.zeros((5, 3)))
+    refused(lib, decode, lse=torch.zeros((5, 4), dtype=torch.half))
+    refused(lib, decode, lens=ints(4))
+    refused(lib, decode, table=ints(4, 4))
+    refused(lib, decode, lens=ints(5).long())
+    refused(lib, decode, table=ints(5, 4).long())
+
+
+def test_prefill_queries_and_items(ctx, lib):
+    def prefill(q=None, out=None, items=(3, 3, 3), table=ints(3, 4), index=torch.int32):
+        ctx.attn_prefill(pool(), rows(heads=4) if q is None else q, *(ints(n).to(index) for n in items), table, 5,
+                         rows(heads=4) if out is None else out)
+
+    prefill()
+    prefill(rows(heads=4, dtype=torch.half), rows(heads=4, dtype=torch.half))
+    assert len(lib.calls) == 2
+    refused(lib, prefill, out=rows(4, heads=4))
+    refused(lib, prefill, q=rows(heads=4, dim=32))
+    refused(lib, prefill, items=(3, 2, 3))
+    refused(lib, prefill, items=(3, 3, 2))
+    refused(lib, prefill, table=ints(2, 4))
+    refused(lib, prefill, index=torch.int64)
+    refused(lib, prefill, table=ints(3, 4).long())
+
+
+def test_attention_over_16_bit_pools_is_called_as_before(ctx, lib):
+    q = rows(heads=4)
+    ctx.attn_decode(pool(nb.F16), q, ints(5, 4), ints(5), 60, q)
+    ctx.attn_prefill(pool(nb.F16), q.half(), ints(3), ints(3), ints(3), ints(3, 4), 5, q)
+    assert lib.calls == ["nbl_attn_decode", "nbl_attn_prefill"]
