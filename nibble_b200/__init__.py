@@ -199,23 +199,28 @@ class KVPool:
         return self._tensor.view(self._tensor.shape)
 
     def close(self):
-        """Frees the pool; while tensors from tensor() are alive, once the last of them is gone."""
+        """Frees the pool; while tensors from tensor() are alive, at the context's next kv_pool(), sync() or check() after the
+        last of them is gone."""
         self.handle = self._tensor = None
         self._memory.close()
 
 
 class _PoolMemory:
-    """A pool's device memory: freed when the pool is closed and no tensor views it any more."""
+    """A pool's device memory: freed when the pool is closed and no tensor views it any more, by a call of the context's user:
+    the last view may go on any thread, at any point, where the library must not be called."""
 
     def __init__(self, ctx: "Context", handle):
-        self.ctx, self.handle, self.views, self.closing = ctx, handle, 0, False
+        self.ctx, self.handle, self.views, self.closing = ctx, handle, [], False  # a list: its changes are atomic
 
     def close(self):
         self.closing = True
-        if self.handle and not self.views:
-            handle, self.handle = self.handle, None
-            if self.ctx.handle:  # a closed context has freed its pools
-                check(_abi.lib.nbl_kv_destroy(handle))
+        if not self.views:
+            self.free()
+
+    def free(self):
+        handle, self.handle = self.handle, None
+        if handle and self.ctx.handle:  # a closed context has freed its pools
+            check(_abi.lib.nbl_kv_destroy(handle))
 
 
 class _View:
@@ -224,12 +229,13 @@ class _View:
     def __init__(self, memory: _PoolMemory, interface: dict):
         self.__cuda_array_interface__ = interface
         self.memory = memory
-        memory.views += 1
+        memory.views.append(None)
 
     def __del__(self):
-        self.memory.views -= 1
-        if self.memory.closing:
-            self.memory.close()
+        memory = self.memory
+        memory.views.pop()
+        if memory.closing and not memory.views:
+            memory.ctx._unviewed.append(memory)
 
 
 class Weight:
@@ -281,6 +287,7 @@ class Context:
         check(_abi.lib.nbl_ctx_create(device, C.byref(h)))
         self.handle = h
         self.device = device
+        self._unviewed = []  # memory of closed pools whose last view is gone
         if use_torch_stream:
             import torch
             self.set_stream(torch.cuda.current_stream(device).cuda_stream)
@@ -295,11 +302,17 @@ class Context:
         call before reserve() and before allocating the blocks."""
         check(_abi.lib.nbl_ctx_set_paged_kv(self.handle, 1 if on else 0))
 
+    def _free_unviewed(self):
+        while self._unviewed:
+            self._unviewed.pop().free()
+
     def sync(self):
+        self._free_unviewed()
         check(_abi.lib.nbl_ctx_sync(self.handle))
 
     def check(self):
         """Raises NibbleError(NBL_E_DEVICE) if a kernel flagged an out-of-range device-side index."""
+        self._free_unviewed()
         check(_abi.lib.nbl_ctx_check(self.handle))
 
     def close(self):
@@ -380,6 +393,7 @@ class Context:
     # ---- paged path
     def kv_pool(self, n_pages: int, n_kv_heads: int, head_dim: int = 64, page_size: int = 16,
                 dtype: int = F16) -> KVPool:
+        self._free_unviewed()
         return KVPool(self, n_pages, n_kv_heads, head_dim, page_size, dtype)
 
     def rope_kv_append(self, kv: KVPool, q_in, k_in, v_in, q_out, tok_row, tok_pos, page_table, n_heads: int,

@@ -1,5 +1,7 @@
 """What the Python calls of the 8-bit cache and of the page bookkeeping refuse before the library sees it: tensors of another type or
 size than the kernels read and write. Without a GPU: the library is a stand-in that records which calls reach it."""
+import threading
+
 import pytest
 import torch
 
@@ -27,7 +29,7 @@ def lib(monkeypatch):
 @pytest.fixture
 def ctx():
     c = object.__new__(nb.Context)
-    c.handle, c.device = 1, 0
+    c.handle, c.device, c._unviewed = 1, 0, []
     return c
 
 
@@ -223,3 +225,34 @@ def test_attention_over_16_bit_pools_is_called_as_before(ctx, lib):
     ctx.attn_decode(pool(nb.F16), q, ints(5, 4), ints(5), 60, q)
     ctx.attn_prefill(pool(nb.F16), q.half(), ints(3), ints(3), ints(3), ints(3, 4), 5, q)
     assert lib.calls == ["nbl_attn_decode", "nbl_attn_prefill"]
+
+
+@pytest.mark.parametrize("then", ["sync", "check"])
+def test_a_closed_pools_last_view_may_go_on_another_thread(ctx, lib, then):
+    """The library is not called from there: a context is one thread's at a time."""
+    memory = nb._PoolMemory(ctx, 7)
+    views = [nb._View(memory, {}), nb._View(memory, {})]
+    memory.close()
+    assert not lib.calls
+    t = threading.Thread(target=views.clear)
+    t.start()
+    t.join()
+    assert not views and not lib.calls
+    getattr(ctx, then)()
+    assert lib.calls == ["nbl_kv_destroy", "nbl_ctx_" + then]
+    getattr(ctx, then)()
+    memory.close()
+    assert lib.calls.count("nbl_kv_destroy") == 1
+
+
+def test_a_pool_without_views_goes_at_once(ctx, lib):
+    memory = nb._PoolMemory(ctx, 7)
+    view = nb._View(memory, {})
+    del view
+    memory.close()
+    assert lib.calls == ["nbl_kv_destroy"]
+    ctx.sync()
+    other = nb._PoolMemory(ctx, 8)
+    ctx.handle = None  # closed: its pools are gone
+    other.close()
+    assert lib.calls == ["nbl_kv_destroy", "nbl_ctx_sync"]
