@@ -193,6 +193,8 @@ class KVPool:
         import torch
         if self.dtype in (I8, E4M3):
             raise ValueError("an 8-bit pool has no plain view: use Context.kv_read, kv_export and kv_import")
+        if self.handle is None:
+            raise ValueError("the pool is closed")
         if self._tensor is None:
             t = _wrap_device_memory(self.base, self.nbytes // 2, torch.int16, self.ctx.device, self._memory)
             self._tensor = t.view(self.n_pages, 2, self.n_kv_heads, self.page_size, self.head_dim)

@@ -256,3 +256,16 @@ def test_a_pool_without_views_goes_at_once(ctx, lib):
     ctx.handle = None  # closed: its pools are gone
     other.close()
     assert lib.calls == ["nbl_kv_destroy", "nbl_ctx_sync"]
+
+
+def test_a_closed_pool_gives_no_view(ctx, lib, monkeypatch):
+    """tensor() of a closed pool would be a view of freed memory."""
+    wrapped = []
+    monkeypatch.setattr(nb, "_wrap_device_memory", lambda *a: wrapped.append(a) or torch.zeros(PAGES * 2 * KV * 16 * D, dtype=torch.int16))
+    kv = pool(nb.F16)
+    kv.ctx, kv.base, kv.nbytes, kv._memory, kv._tensor = ctx, 4096, PAGES * 2 * KV * 16 * D * 2, nb._PoolMemory(ctx, 1), None
+    assert kv.tensor().shape == (PAGES, 2, KV, 16, D)
+    kv.close()
+    with pytest.raises(ValueError, match="closed"):
+        kv.tensor()
+    assert len(wrapped) == 1
