@@ -67,6 +67,10 @@ class RotarySpec:
             object.__setattr__(self, "_made", made)
         return made
 
+    def __getstate__(self):
+        """For copies and pickles: the fields, without the C struct and its pointers."""
+        return {k: v for k, v in self.__dict__.items() if k != "_made"}
+
     def _make(self):
         if self.scaling not in _abi.ROTARY_SCALING:
             raise ValueError(f"unknown rotary scaling {self.scaling!r} (one of {', '.join(_abi.ROTARY_SCALING)})")

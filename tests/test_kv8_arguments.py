@@ -1,5 +1,7 @@
 """What the Python calls of the 8-bit cache and of the page bookkeeping refuse before the library sees it: tensors of another type or
 size than the kernels read and write. Without a GPU: the library is a stand-in that records which calls reach it."""
+import copy
+import pickle
 import threading
 
 import pytest
@@ -269,3 +271,14 @@ def test_a_closed_pool_gives_no_view(ctx, lib, monkeypatch):
     with pytest.raises(ValueError, match="closed"):
         kv.tensor()
     assert len(wrapped) == 1
+
+
+def test_a_rotary_spec_copies_and_pickles_after_its_use():
+    spec = nb.RotarySpec(5e5, True, rotary_dim=8, scaling="yarn", factor=4.0, original_ctx=64, freq_factors=(1.0, 2.0, 3.0, 8.0))
+    first = spec._c()
+    assert spec._c() is first
+    for twin in (copy.copy(spec), copy.deepcopy(spec), pickle.loads(pickle.dumps(spec))):
+        assert twin == spec and hash(twin) == hash(spec)
+        made, factors = twin._c()
+        assert made is not first[0] and list(factors) == [1.0, 2.0, 3.0, 8.0]
+        assert (made.freq_base, made.neox, made.rotary_dim, made.scaling, made.factor) == (5e5, 1, 8, nb._abi.ROTARY_SCALING["yarn"], 4.0)
