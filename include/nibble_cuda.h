@@ -257,7 +257,7 @@ NBL_API int nbl_rope_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const
  * head_dim 64, n_heads / n_kv_heads <= 8.
  * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes any group size; n_splits is then not used, the pages of all
  * rows being divided evenly over the GPU whatever their lengths. The results are the softmax over the values that the
- * codes stand for, to fp32 accuracy. */
+ * codes stand for, to fp32 accuracy; a head whose query has an infinity or NaN gets NaN in out and lse. */
 NBL_API int nbl_attn_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_t* page_table, int32_t pt_stride,
                     const int32_t* seq_lens, int32_t max_seq_len, int32_t n_rows, int32_t n_heads, float* out,
                     float* lse, int32_t n_splits);
@@ -304,7 +304,8 @@ NBL_API int nbl_attn_decode_static(nbl_ctx* ctx, const nbl_kv* kv, const float* 
  * items' out rows in out_dtype (F32 or the pool dtype). Tensor-core kernel (tcgen05): bf16/fp16 operands, fp32
  * accumulation in TMEM.
  * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes q in F32, F16 or BF16 and writes out in F32 or q's dtype;
- * the scales are applied to scores and weights in fp32, the weights of 16-bit queries are rounded to fp16. */
+ * the scales are applied to scores and weights in fp32, the weights of 16-bit queries are rounded to fp16. A head whose
+ * query has an infinity or NaN gets NaN. */
 NBL_API int nbl_attn_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype, int64_t n_q_rows,
                      const int32_t* q_start, const int32_t* q_len, const int32_t* kv_pos0, const int32_t* page_table,
                      int32_t pt_stride, int32_t n_items, int32_t n_heads, int32_t max_q_len, void* out,

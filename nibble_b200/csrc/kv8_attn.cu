@@ -37,6 +37,7 @@
 // the sake of whole pages: 217 and 199 us, and 18.4 against 16.8 for 8 items of 5 drafted tokens.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -397,7 +398,8 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       const uint32_t e = min(max(__float_as_uint(mx) >> 23, 1u), 253u);
-      const float inv = __uint_as_float((254u - e) << 23);
+      // an infinity makes the row's scores NaN, as a NaN does (its own products could be -inf, like those of masked keys)
+      const float inv = mx <= FLT_MAX ? __uint_as_float((254u - e) << 23) : NAN;
       // dim d = 64 sb + 16 t + 4 ks: k-step 4 sb + ks, lane (row % 8, t)
       const int at = ((d >> 6) * 4 + ((d >> 2) & 3)) * 32 + (row & 7) * 4 + ((d >> 4) & 3);
       uint32_t hi0, hi1, lo0 = 0, lo1 = 0;
@@ -439,7 +441,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
   auto store4 = [&](int q_start, int kvh, int rr, int d, float4 v, float L, float m) {
     const int tok = a.by_group.div(rr);
     const int64_t row = (int64_t(q_start) + tok) * a.n_heads + kvh * a.group + rr - tok * a.group;
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // 0: no keys; NaN: a query that is not finite, and so is the row
     if (a.out_dtype == NBL_F32 && a.q_vec) {
       *reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * D + d) =
           make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
       store_as(a.out, row * D + d + 2, v.z * inv, a.out_dtype);
       store_as(a.out, row * D + d + 3, v.w * inv, a.out_dtype);
     }
-    if (d == 0 && a.lse) a.lse[row] = L > 0.f ? (m + log2f(L)) * kLn2 : -INFINITY;
+    if (d == 0 && a.lse) a.lse[row] = L == 0.f ? -INFINITY : (m + log2f(L)) * kLn2;
   };
   // The unit in s_due, whose parts are all in scratch, if this CTA was the last to arrive.
   int seg_parity = 0;
@@ -467,17 +469,16 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
       float mx = -INFINITY;
 #pragma unroll 8
       for (int k = first; k <= last; ++k) mx = fmaxf(mx, __ldcg(part(k) + ROWS * D + r));
+      const float mu = mx == -INFINITY ? 0.f : mx;  // (a sum that is NaN has a maximum of -inf, and stays NaN)
       float L = 0.f;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (mx != -INFINITY) {
 #pragma unroll 4
-        for (int k = first; k <= last; ++k) {
-          const float* pb = part(k);
-          const float e = ex2(__ldcg(pb + ROWS * D + r) - mx);
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(pb + r * D + d));
-          L = fmaf(e, __ldcg(pb + ROWS * D + ROWS + r), L);
-          O.x = fmaf(e, x.x, O.x), O.y = fmaf(e, x.y, O.y), O.z = fmaf(e, x.z, O.z), O.w = fmaf(e, x.w, O.w);
-        }
+      for (int k = first; k <= last; ++k) {
+        const float* pb = part(k);
+        const float e = ex2(__ldcg(pb + ROWS * D + r) - mu);
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(pb + r * D + d));
+        L = fmaf(e, __ldcg(pb + ROWS * D + ROWS + r), L);
+        O.x = fmaf(e, x.x, O.x), O.y = fmaf(e, x.y, O.y), O.z = fmaf(e, x.z, O.z), O.w = fmaf(e, x.w, O.w);
       }
       store4(q_start, kvh, row0 + r, d, O, L, mx);
     }
@@ -715,17 +716,16 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
       float mx = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kConsumers; ++w) mx = fmaxf(mx, mrg[w * C::kMergeFloats + ROWS * D + r]);
+      const float mu = mx == -INFINITY ? 0.f : mx;
       float L = 0.f;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (mx != -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < kConsumers; ++w) {
-          const float* wb = mrg + w * C::kMergeFloats;
-          const float k = ex2(wb[ROWS * D + r] - mx);  // 0 for warps that saw no key
-          const float4 x = *reinterpret_cast<const float4*>(wb + r * D + d);
-          L = fmaf(k, wb[ROWS * D + ROWS + r], L);
-          O.x = fmaf(k, x.x, O.x), O.y = fmaf(k, x.y, O.y), O.z = fmaf(k, x.z, O.z), O.w = fmaf(k, x.w, O.w);
-        }
+      for (int w = 0; w < kConsumers; ++w) {
+        const float* wb = mrg + w * C::kMergeFloats;
+        const float k = ex2(wb[ROWS * D + r] - mu);  // 0 for warps that saw no key
+        const float4 x = *reinterpret_cast<const float4*>(wb + r * D + d);
+        L = fmaf(k, wb[ROWS * D + ROWS + r], L);
+        O.x = fmaf(k, x.x, O.x), O.y = fmaf(k, x.y, O.y), O.z = fmaf(k, x.z, O.z), O.w = fmaf(k, x.w, O.w);
       }
       if (whole) {
         store4(done.x.q_start, kvh, row0 + r, d, O, L, mx);

@@ -681,8 +681,9 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       }
       if (!ok) break;
       // ---- epilogue: O_g out of TMEM, normalised and stored; then the next work's first PV may overwrite it
-      if (m_ref == -INFINITY) l_run = 0.f;  // no key seen (a part past the row's position)
-      const float inv = l_run > 0.f ? vrefc * unit<KIND>() / l_run : 0.f;
+      // no key seen (a part past the row's position): 0; keys, but no score above -inf: a query that is not finite
+      if (m_ref == -INFINITY) l_run = wk.t0 * kBN <= qpos ? NAN : 0.f;
+      const float inv = l_run == 0.f ? 0.f : vrefc * unit<KIND>() / l_run;
       ok = warp_wait(&bars[C::kBarODone + g], h_works & 1, a.err);
       if (!ok) break;
       ++h_works;
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
         float* lse = a.part_lse + orow;
         const int64_t step = a.it.n_rows * a.n_heads;
         const int part = wk.part & (kLastPart - 1);
-        lse[part * step] = l_run > 0.f ? m_ref + log2f(l_run) : -INFINITY;
+        lse[part * step] = l_run == 0.f ? -INFINITY : m_ref + log2f(l_run);
         if (wk.part & kLastPart)
           for (int p = part + 1; p < a.n_splits; ++p) lse[p * step] = -INFINITY;  // parts that the work does not have
       }
@@ -762,14 +763,14 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const float* __r
     for (int p = 0; p < n_splits; ++p) mx = fmaxf(mx, part_lse[p * rows + row]);
     float W = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (mx != -INFINITY)
-      for (int p = 0; p < n_splits; ++p) {
-        const float w = fast_exp2(part_lse[p * rows + row] - mx);
-        const float4 x = *reinterpret_cast<const float4*>(part_o + (p * rows + row) * D + d);
-        W += w;
-        if (w > 0.f) O.x += w * x.x, O.y += w * x.y, O.z += w * x.z, O.w += w * x.w;
-      }
-    const float inv = W > 0.f ? 1.f / W : 0.f;
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    for (int p = 0; p < n_splits; ++p) {
+      const float w = fast_exp2(part_lse[p * rows + row] - mu);  // NaN: a query that is not finite, and so is the row
+      const float4 x = *reinterpret_cast<const float4*>(part_o + (p * rows + row) * D + d);
+      W += w;
+      if (w > 0.f) O.x += w * x.x, O.y += w * x.y, O.z += w * x.z, O.w += w * x.w;
+    }
+    const float inv = W == 0.f ? 0.f : 1.f / W;
     store_as(out, row * D + d, O.x * inv, out_dtype);
     store_as(out, row * D + d + 1, O.y * inv, out_dtype);
     store_as(out, row * D + d + 2, O.z * inv, out_dtype);

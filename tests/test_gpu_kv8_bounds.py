@@ -41,3 +41,72 @@ def test_prefill_item_longer_than_max_q_len_is_left_out(nbl_ctx, D, dtype, strid
     for i in (0, 1):
         check_rows(got, qf, values, table[i], starts[i], *items[i], dtype, every=13)
     kv.close()
+
+
+def spoil(q, rng, bad):
+    """A copy of q with bad in one element of some (row, head)s, and which."""
+    import torch
+    n, H, D = q.shape
+    at = rng.random((n, H)) < 0.3
+    at[0, 0] = True
+    r, h = np.nonzero(at)
+    x = q.clone()
+    x[torch.from_numpy(r), torch.from_numpy(h), torch.from_numpy(rng.integers(0, D, len(r)))] = bad
+    return x, torch.from_numpy(at).cuda()
+
+
+@pytest.mark.parametrize("bad", [NAN, float("inf"), float("-inf")])
+@pytest.mark.parametrize("kind,D", [("int8", 64), ("e4m3", 128)])
+def test_decode_of_queries_that_are_not_finite(nbl_ctx, kind, D, bad):
+    """Their heads' outputs and lse are NaN (a row without keys stays 0 and -inf); all others are the same bits as without them."""
+    import torch
+    lens, H, KV = [1, 40, 0, 900, 9000], 6, 2  # the last one's parts are joined
+    table, n_pages = make_page_tables(lens, shuffle_seed=1)
+    kv, _ = random_pool(nbl_ctx, kind, n_pages, KV, D, 3)
+    rng = np.random.default_rng(7)
+    q = dev(rng.standard_normal((5, H, D)).astype(np.float32))
+    x, at = spoil(q, rng, bad)
+    got = []
+    for t in (q, x):
+        out, lse = torch.empty_like(q), torch.empty((5, H), device="cuda")
+        nbl_ctx.attn_decode(kv, t, dev(table), ints(lens), max(lens), out, lse)
+        got.append((out, lse))
+    nbl_ctx.check()
+    (out, lse), (bad_out, bad_lse) = got
+    keys = ints(lens) > 0
+    nan = at & keys[:, None]
+    assert bad_out[nan].isnan().all() and bad_lse[nan].isnan().all()
+    assert torch.equal(bad_out[~nan], out[~nan]) and torch.equal(bad_lse[~nan], lse[~nan])
+    assert (bad_out[~keys] == 0).all() and (bad_lse[~keys] == float("-inf")).all()
+    kv.close()
+
+
+@pytest.mark.parametrize("bad", [NAN, float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("kind,D,items,stride", [
+    ("int8", 64, [(0, 5), (3001, 4)], None),           # few tokens: the warp-level kernel
+    ("e4m3", 128, [(0, 3), (40, 2)], None),
+    ("int8", 64, [(0, 300), (70, 150)], 30),           # whole works
+    ("e4m3", 64, [(0, 300), (3000, 150)], None),       # joined parts
+    ("int8", 128, [(0, 200), (3000, 130)], None),
+    ("e4m3", 128, [(0, 200), (100, 130)], 20)])
+def test_prefill_of_queries_that_are_not_finite(nbl_ctx, kind, D, items, stride, dtype, bad):
+    import torch
+    H, KV = 6, 2
+    table, n_pages = make_page_tables([p + m for p, m in items], shuffle_seed=1, stride=stride)
+    kv, _ = random_pool(nbl_ctx, kind, n_pages, KV, D, 3)
+    starts = np.cumsum([0] + [m for _, m in items])[:-1]
+    rng = np.random.default_rng(8)
+    q = dev(rng.standard_normal((sum(m for _, m in items), H, D)).astype(np.float32)).to(getattr(torch, dtype))
+    x, at = spoil(q, rng, bad)
+    got = []
+    for t in (q, x):
+        out = torch.empty_like(q)
+        nbl_ctx.attn_prefill(kv, t, ints(starts), ints([m for _, m in items]), ints([p for p, _ in items]), dev(table),
+                             max(m for _, m in items), out)
+        got.append(out)
+    nbl_ctx.check()
+    assert not got[0].isnan().any()
+    assert got[1][at].isnan().all()
+    assert torch.equal(got[1][~at], got[0][~at])
+    kv.close()
