@@ -103,16 +103,18 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
-_int32: dict = {}  # torch.int32 -> True
+_int32: set = set()  # torch.int32, once it has been seen
 
 
 def _ints(t) -> int:
     """Pointer to an int32 tensor: positions, lengths, page ids (another type's elements would be read as pairs of int32)."""
-    if not _int32.get(t.dtype):
+    if t.dtype not in _int32:
         if str(t.dtype) != "torch.int32":
             raise ValueError(f"expected an int32 tensor, not {t.dtype}")
-        _int32[t.dtype] = True
-    return _ptr(t)
+        _int32.add(t.dtype)
+    if t.is_cuda and t.is_contiguous():
+        return t.data_ptr()
+    return _ptr(t)  # says what is wrong
 
 
 _codes: dict = {}  # torch dtype -> element type code
@@ -131,18 +133,23 @@ def _dtype(t) -> int:
 def _new_rows(kv, q, k, v, q_out):
     """(rows, query heads) of tokens for kv: q and q_out [rows, heads, D], k and v [rows, kv heads, D]."""
     shape = q.shape
-    want = (shape[0], kv.n_kv_heads, kv.head_dim)
-    if len(shape) != 3 or shape[2] != kv.head_dim or q_out.shape != shape or k.shape != want or v.shape != want:
+    n, heads, dim = shape
+    if dim != kv.head_dim or q_out.shape != shape or k.shape != (n, kv.n_kv_heads, dim) or v.shape != k.shape:
         raise ValueError(f"expected q_in, q_out [rows, n_heads, {kv.head_dim}] and k_in, v_in [rows, {kv.n_kv_heads}, {kv.head_dim}]")
-    return shape[0], shape[1]
+    return n, heads
 
 
 def _items(first, second, third, page_table):
-    """(items, table stride): three entries an item, and a page-table row at least."""
-    n, stride = first.numel(), page_table.shape[-1]
+    """Pointers to an item's three entries and to the page table, which has a row for each; its stride, and the items. (One
+    function for the four: the checks of a small call cost as much as its launch.)"""
+    n, stride, dtype = first.numel(), page_table.shape[-1], first.dtype
     if second.numel() != n or third.numel() != n or page_table.numel() < n * stride:
         raise ValueError("expected one start, length and first position per item, and a page-table row for each")
-    return n, stride
+    if (dtype in _int32 and second.dtype is dtype and third.dtype is dtype and page_table.dtype is dtype and
+            first.is_cuda and second.is_cuda and third.is_cuda and page_table.is_cuda and first.is_contiguous() and
+            second.is_contiguous() and third.is_contiguous() and page_table.is_contiguous()):
+        return first.data_ptr(), second.data_ptr(), third.data_ptr(), page_table.data_ptr(), stride, n
+    return _ints(first), _ints(second), _ints(third), _ints(page_table), stride, n
 
 
 def _book(kv, page_table, seq_lens, ref_counts, first, second):
@@ -154,7 +161,7 @@ def _book(kv, page_table, seq_lens, ref_counts, first, second):
 
 
 def _check_bias(b, heads, dim):
-    if b is not None and (_dtype(b) != F32 or b.numel() != heads * dim):
+    if _dtype(b) != F32 or b.numel() != heads * dim:
         raise ValueError(f"expected a float32 bias of {heads} * {dim} elements")
 
 
@@ -452,10 +459,9 @@ class Context:
             rows, heads, dim = q.shape
             if dim != kv.head_dim or out.numel() < rows * heads * dim:
                 raise ValueError(f"expected q and out [rows, n_heads, {kv.head_dim}]")
-            n, stride = _items(q_start, q_len, kv_pos0, page_table)
-            check(_abi.lib.nbl_attn_prefill(self.handle, kv.handle, _ptr(q), _dtype(q), rows, _ints(q_start),
-                                            _ints(q_len), _ints(kv_pos0), _ints(page_table), stride, n, heads,
-                                            max_q_len, _ptr(out), _dtype(out)))
+            start, length, pos0, table, stride, n = _items(q_start, q_len, kv_pos0, page_table)
+            check(_abi.lib.nbl_attn_prefill(self.handle, kv.handle, _ptr(q), _dtype(q), rows, start, length, pos0, table,
+                                            stride, n, heads, max_q_len, _ptr(out), _dtype(out)))
             return
         check(_abi.lib.nbl_attn_prefill(self.handle, kv.handle, _ptr(q), _dtype(q), q.shape[0], _ptr(q_start),
                                         _ptr(q_len), _ptr(kv_pos0), _ptr(page_table), page_table.shape[-1],
@@ -468,33 +474,36 @@ class Context:
         [rows, n_heads, D], k_in and v_in [rows, n_kv_heads, D]) at positions kv_pos0[i].. of page-table row i, and the
         rotated queries into q_out (see nbl_rotary_kv_append)."""
         p, keep = rotary._c()
-        in_dt = _dtype(q_in)
-        if _dtype(k_in) != in_dt or _dtype(v_in) != in_dt:
+        dtype = q_in.dtype
+        if k_in.dtype is not dtype or v_in.dtype is not dtype:
             raise ValueError("q_in, k_in, v_in must share a dtype")
         n_rows, heads = _new_rows(kv, q_in, k_in, v_in, q_out)
-        n_items, stride = _items(q_start, q_len, kv_pos0, page_table)
-        for b, h in ((bq, heads), (bk, kv.n_kv_heads), (bv, kv.n_kv_heads)):
-            _check_bias(b, h, kv.head_dim)
+        start, length, pos0, table, stride, n_items = _items(q_start, q_len, kv_pos0, page_table)
+        if bq is not None:
+            _check_bias(bq, heads, kv.head_dim)
+        if bk is not None:
+            _check_bias(bk, kv.n_kv_heads, kv.head_dim)
+        if bv is not None:
+            _check_bias(bv, kv.n_kv_heads, kv.head_dim)
         if rotary.freq_factors is not None and len(rotary.freq_factors) != (rotary.rotary_dim or kv.head_dim) // 2:
             raise ValueError("freq_factors must hold rotary_dim / 2 factors")
         check(_abi.lib.nbl_rotary_kv_append(
-            self.handle, kv.handle, _ptr(q_in), _ptr(k_in), _ptr(v_in), in_dt, _ptr(bq), _ptr(bk), _ptr(bv),
-            _ptr(q_out), _dtype(q_out), n_rows, _ints(q_start), _ints(q_len), _ints(kv_pos0), _ints(page_table),
-            stride, n_items, heads, max_q_len, C.byref(p)))
+            self.handle, kv.handle, _ptr(q_in), _ptr(k_in), _ptr(v_in), _dtype(q_in), _ptr(bq), _ptr(bk), _ptr(bv),
+            _ptr(q_out), _dtype(q_out), n_rows, start, length, pos0, table, stride, n_items, heads, max_q_len, C.byref(p)))
 
     def kv_read(self, kv: KVPool, start, length, kv_pos0, page_table, max_len: int, k_out=None, v_out=None):
         """Item i's positions kv_pos0[i].. as rows start[i].. of k_out / v_out [rows, n_kv_heads, D] (see nbl_kv_read)."""
         like = k_out if k_out is not None else v_out
         if like is None:
             raise ValueError("kv_read needs k_out or v_out")
-        want = (like.shape[0], kv.n_kv_heads, kv.head_dim)
-        if like.shape != want or (k_out is not None and v_out is not None and
-                                  (v_out.shape != want or v_out.dtype != k_out.dtype)):
+        shape = like.shape
+        n_rows, heads, dim = shape
+        if heads != kv.n_kv_heads or dim != kv.head_dim or (
+                like is not v_out and v_out is not None and (v_out.shape != shape or v_out.dtype is not like.dtype)):
             raise ValueError(f"expected k_out and v_out [rows, {kv.n_kv_heads}, {kv.head_dim}] of one shape and dtype")
-        n_items, stride = _items(start, length, kv_pos0, page_table)
-        check(_abi.lib.nbl_kv_read(self.handle, kv.handle, like.shape[0], _ints(start), _ints(length), _ints(kv_pos0),
-                                   _ints(page_table), stride, n_items, max_len, _ptr(k_out),
-                                   _ptr(v_out), _dtype(like)))
+        first, n, pos0, table, stride, n_items = _items(start, length, kv_pos0, page_table)
+        check(_abi.lib.nbl_kv_read(self.handle, kv.handle, n_rows, first, n, pos0, table, stride, n_items, max_len,
+                                   _ptr(k_out), _ptr(v_out), _dtype(like)))
 
     def kv_import(self, kv: KVPool, page_ids, codes, scales):
         """codes [n, 2, n_kv_heads, 16, D] (int8 / float8_e4m3fn) and scales [n, 2, n_kv_heads] fp32 into pages page_ids."""
