@@ -257,7 +257,9 @@ NBL_API int nbl_rope_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const
  * head_dim 64, n_heads / n_kv_heads <= 8.
  * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes any group size; n_splits is then not used, the pages of all
  * rows being divided evenly over the GPU whatever their lengths. The results are the softmax over the values that the
- * codes stand for, to fp32 accuracy; a head whose query has an infinity or NaN gets NaN in out and lse. */
+ * codes stand for, to fp32 accuracy (and to 2^-38 of the largest value scale among the row's pages: where a row all but
+ * ignores pages 2^17 times as loud as those that it attends, the latter's values lose bits); a head whose query has an
+ * infinity or NaN gets NaN in out and lse. */
 NBL_API int nbl_attn_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_t* page_table, int32_t pt_stride,
                     const int32_t* seq_lens, int32_t max_seq_len, int32_t n_rows, int32_t n_heads, float* out,
                     float* lse, int32_t n_splits);

@@ -3,9 +3,11 @@
 // Mathematics. With codes c and block scales s_k, s_v: score_j = s_k (q . ck_j) / sqrt(D), out = sum_j p_j s_v cv_j /
 // sum_j p_j. The codes are exact fp16 (bf16) operands, so the tensor cores multiply codes and the scales meet scores and
 // weights in fp32: a score is raw * f_b (f_b one number per 16-key block), and the weight that multiplies the value codes
-// is p'_j = 2^(score - m + log2(s_v / vref) + 6), the same fused multiply-add with another addend. The row sum needs p
-// without s_v: per block, sum(p') * (vref / s_v) / 2^6. vref is at least twice every s_v met so far (it moves rarely,
-// with the accumulators), so p' <= 2^13 fits fp16, which holds it to 2^-12 relative: below the output's rounding.
+// is p'_j = 2^(score + log2 s_v - M + 6), the same fused multiply-add with another addend. M is the row's largest score +
+// log2 s_v (to 2^8: it moves rarely, with the accumulators), so p' <= 2^14 fits fp16, which holds it to 2^-12 relative: below
+// the output's rounding, and whatever the scales of pages that the row hardly attends (with the largest s_v met in place
+// of M, the values of a row that attends quiet pages after a loud one were lost). The row sum needs p without s_v: per block,
+// sum(p') / s_v * 2^(M - m - 6), m being the row's largest score.
 //
 // Work. Persistent CTAs walk works, a work being a 128-row query tile of two or four heads of a KV group over all of its
 // keys (or a part of them, see Walk). Warps:
@@ -48,7 +50,9 @@ constexpr int kBN = 64;                    // keys of a tile
 constexpr int kTilePages = kBN / kPage;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: p may reach 2^8 before the reference max moves
 constexpr float kPShift = 6.0f;            // p' carries 2^6
-constexpr float kMinLv = -24.0f;           // smallest log2(s_v / vref) kept: below it a block adds nothing to fp16 weights
+// Smallest log2 s_v - (M - m) kept in a block's exponents, for the sum's sake: below it p' is at most 2^(8 - 40 + 6), which
+// fp16 weights round to 0 as they would the smaller one.
+constexpr float kMinLv = -40.0f;
 
 constexpr int kRing = 4;                   // works handed from the first converting warp to the other roles
 
@@ -470,8 +474,8 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
           *reinterpret_cast<uint2*>(sV(s) + swz128(32 * k + 8 * jj + g, 2 * b + (t >> 1)) + 8 * (t & 1)) = y;
         }
       }
-      // a scale of 0 comes with codes of 0: any other scale gives the same
-      const float ks = fmaxf(sc.x, 1e-34f), vs = fmaxf(sc.y, 1e-34f);
+      // a scale of 0 comes with codes of 0: any other scale gives the same (here the smallest there is)
+      const float ks = fmaxf(sc.x, kTiny / 448.f), vs = fmaxf(sc.y, kTiny / 448.f);
       const float4 out = make_float4(ks * (unit<KIND>() * a.scale_log2), __log2f(vs), __fdividef(1.f, vs), 0.f);
       if (lane == 0) scales[s * kTilePages + b] = out;
       fence_proxy_async_smem();  // the operands, for the tensor core
@@ -592,7 +596,8 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       const int64_t orow = (int64_t(wk.row) + r) * a.n_heads + wk.head0 + g;
       const bool live = r < wk.live;
       float m_ref = -INFINITY, l_run = 0.f;
-      float lref = -INFINITY, vrefc = 0.f;  // log2 of vref, and vref / 2^6
+      float o_ref = -INFINITY;       // M
+      float lref = 0.f, vrefc = 0.f;  // M - m, and 2^(M - m - 6)
       for (int j = 0; j < n; ++j, ++h_tiles) {
         const int buf = h_tiles % SB, s = (kt0 + j) % ST;
         const uint32_t tS = tmem + C::col_s(g, buf) + lane_off;
@@ -609,7 +614,7 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
             if (kbase + c > qpos) t[c] = __float_as_uint(-INFINITY);
         }
         float4 sc[kTilePages];
-        float m_tile = -INFINITY, lmax = -INFINITY;
+        float m_tile = -INFINITY, o_tile = -INFINITY;
 #pragma unroll
         for (int b = 0; b < kTilePages; ++b) {
           sc[b] = scales[s * kTilePages + b];
@@ -621,23 +626,21 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
             mx[i] = fmax3(mx[i], __uint_as_float(x[i + 6]), __uint_as_float(x[i + 8]));
             mx[i] = fmax3(mx[i], __uint_as_float(x[i + 10]), __uint_as_float(x[i + 12]));
           }
-          m_tile = fmaxf(m_tile, fmax3(fmax3(mx[0], mx[1], __uint_as_float(x[14])), __uint_as_float(x[15]), -INFINITY) * sc[b].x);
-          lmax = fmaxf(lmax, sc[b].y);
+          const float top = fmax3(fmax3(mx[0], mx[1], __uint_as_float(x[14])), __uint_as_float(x[15]), -INFINITY) * sc[b].x;
+          m_tile = fmaxf(m_tile, top);
+          o_tile = fmaxf(o_tile, top + sc[b].y);
         }
-        const bool need_m = m_tile > m_ref + kRescaleThreshold;  // false for m_tile = -inf
-        const float m_new = need_m ? m_tile : m_ref;
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        float l_scale = need_m ? fast_exp2(m_ref - m_use) : 1.f, alpha = l_scale;  // m_ref = -inf gives 0
-        bool need = need_m;
-        if (lmax > lref) {  // the same in every row
-          const float lnew = lmax + 1.f;
-          alpha *= fast_exp2(lref - lnew);
-          need = true;
-          lref = lnew;
+        const bool need = m_tile > m_ref + kRescaleThreshold || o_tile > o_ref + kRescaleThreshold;  // false for -inf
+        float alpha = 1.f;
+        if (need) {
+          const float m_new = fmaxf(m_ref, m_tile), o_new = fmaxf(o_ref, o_tile);
+          l_run *= fast_exp2(m_ref - m_new);  // m_ref = -inf gives 0
+          alpha = fast_exp2(o_ref - o_new);
+          m_ref = m_new, o_ref = o_new;
+          lref = o_new - m_new;
           vrefc = fast_exp2(lref - kPShift);
         }
-        m_ref = m_new;
-        l_run *= l_scale;
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
         uint32_t p[kBN / 2];
 #pragma unroll
         for (int b = 0; b < kTilePages; ++b) {
@@ -654,7 +657,7 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
             p[8 * b + 2 * (u & 3) + (u >> 2)] = pack2<false>(e.x, e.y);
           }
           const float2 s2 = __fadd2_rn(sum[0], sum[1]);
-          const float w = lv < kMinLv ? 262144.f : sc[b].z * vrefc;  // 2^(24 - 6), or vref / s_v / 2^6
+          const float w = lv < kMinLv ? 17179869184.f : sc[b].z * vrefc;  // 2^(40 - 6), or 2^(M - m - 6) / s_v
           l_run = fmaf(s2.x + s2.y, w, l_run);
         }
         // P into the first columns of the S buffer (the PV MMA's A operand)

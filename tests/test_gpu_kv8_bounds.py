@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from nibble_b200.workloads import make_page_tables
-from test_gpu_kv8 import attend, dev, ints, np_of, random_pool, rows_of
+from test_gpu_kv8 import QMAX, attend, dev, export, ints, np_of, random_pool, rows_of
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -109,4 +109,55 @@ def test_prefill_of_queries_that_are_not_finite(nbl_ctx, kind, D, items, stride,
     assert not got[0].isnan().any()
     assert got[1][at].isnan().all()
     assert torch.equal(got[1][~at], got[0][~at])
+    kv.close()
+
+
+@pytest.mark.parametrize("how", ["loud_page_not_attended", "spread", "zero_pages"])
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,H,items,stride", [
+    (64, 8, [(0, 300), (70, 150)], 30),     # four heads a block, whole works
+    (64, 4, [(0, 300), (3000, 150)], None),  # two, joined parts
+    (128, 8, [(0, 200), (100, 130)], 20),
+    (128, 4, [(0, 200), (3000, 130)], None)])
+def test_prefill_of_uneven_value_scales(nbl_ctx, how, kind, D, H, items, stride):
+    """Value scales far apart among a row's pages: errors are measured by what the row attends (sum p |v|), however loud the rest.
+    loud_page_not_attended: an item's first page is 2^30 times as loud as the others and has weights near e^-96 of theirs."""
+    import torch
+    KV = 2
+    table, n_pages = make_page_tables([p + m for p, m in items], shuffle_seed=1, stride=stride)
+    kv, _ = random_pool(nbl_ctx, kind, n_pages, KV, D, 3)
+    codes, scales = export(nbl_ctx, kv)
+    rng = np.random.default_rng(11)
+    n = sum(m for _, m in items)
+    x = rng.standard_normal((n, H, D))
+    scales[:, 0] = np.float32(2.0 / QMAX[kind])
+    scales[:, 1] = np.float32(2.0 / QMAX[kind])
+    if how == "loud_page_not_attended":
+        x += 6 * (64 / D) ** 0.5  # a common sign, and keys of the other one in the first page
+        for row in table:
+            codes[row[0], 0], scales[row[0], 1] = -QMAX[kind], scales[row[0], 1] * np.float32(2.0 ** 30)
+    elif how == "spread":
+        scales[:, 1] *= np.exp2(rng.integers(-40, 41, (n_pages, KV))).astype(np.float32)
+    else:
+        for row in table:  # the leading pages, one in the middle
+            for page in (row[0], row[1], row[5]):
+                codes[page, 1], scales[page, 1] = 0, 0
+        scales[:, 1] *= np.float32(1e-20)
+    c = dev(codes).to(torch.int8 if kind == "int8" else torch.float8_e4m3fn)
+    nbl_ctx.kv_import(kv, ints(np.arange(n_pages)), c, dev(scales))
+    values = codes.astype(np.float64) * scales.astype(np.float64)[..., None, None]
+    q, qf = np_of(x.astype(np.float32), torch.float16)
+    out = torch.full((n, H, D), NAN, device="cuda")
+    starts = np.cumsum([0] + [m for _, m in items])[:-1]
+    nbl_ctx.attn_prefill(kv, q, ints(starts), ints([m for _, m in items]), ints([p for p, _ in items]), dev(table),
+                         max(m for _, m in items), out)
+    nbl_ctx.check()
+    got = out.double().cpu().numpy()
+    for i, (p, m) in enumerate(items):
+        k, v = rows_of(values, table[i], p + m)
+        for t in range(0, m, 7):
+            if how == "loud_page_not_attended" and p + t < 40:
+                continue  # rows that see little but the loud page
+            ro, _, size = attend(qf[starts[i] + t], k, v, p + t + 1)
+            assert (np.abs(got[starts[i] + t] - ro) <= 2.0 ** -11 * size + 2e-5 * size.max(-1, keepdims=True)).all(), f"item {i} row {t}"
     kv.close()
