@@ -20,18 +20,18 @@
 //
 // What each choice is for: issue slots (a page of one head, 2 KB at D = 64, is 89 clocks of HBM time per SM and takes
 // ~130 warp instructions, most of them the widening of the codes).
-// - I8 keys are widened by the byte permute alone: code + 128 in the low bits of an fp16 is (code + 128) * 2^-24, a
-//   subnormal, and the 128 * sum(q) it adds to a score is a constant of the row, taken off in the exponent's
-//   fused multiply-add. (Values would lose accuracy that way: sum(p v) is far smaller than 128 sum(p).)
+// - I8 keys are widened to the codes themselves, a byte permute and a subtraction for two of them. (As code + 128, by the
+//   permute alone, with 128 * sum(q) taken off the scores afterwards, 256 rows of 4097 tokens took 215 us in place of 222 and
+//   4 rows of 131073 194 in place of 209; but for queries of one sign that difference cancels, and the tensor cores'
+//   truncation of the larger sums left scores off by 1e-5 to 1e-4 of their size, and lse with them.)
 // - p * s_v is formed relative to the largest s_v that the warp has met (vref) and scaled by 2^14, so fp16 holds it
 //   whatever the cache's magnitudes: the accumulators are O * 2^14 / vref.
 // - A chunk's P V is accumulated from zero by the tensor cores and added to O in fp32: the tensor cores truncate, and
 //   over thousands of pages that shows (4e-6 relative at 131k tokens, 8e-7 this way). The addition is the
 //   multiply-add that rescales O anyway.
 //
-// Measured: 256 rows of 4097 tokens, 32/8 heads of 64: 217 us, 5.0 TB/s of codes and scales (77 % of the measured copy rate)
-// with other pools of that size read in between, 187 us on the same pool again and again; 4 rows of 131073, 32/8 heads of 128:
-// 195 us, 5.5 TB/s (85 %), and 176; 48 rows of 511..16384, 28/4 heads of 128: 55 us, 4.1 TB/s: the launch, the CTAs' search
+// Measured: 256 rows of 4097 tokens, 32/8 heads of 64: 222 us, 4.9 TB/s of codes and scales (75 % of the measured copy rate)
+// with other pools of that size read in between; 4 rows of 131073, 32/8 heads of 128: 209 us, 5.1 TB/s (79 %); 48 rows of 511..16384, 28/4 heads of 128: 55 us, 4.1 TB/s: the launch, the CTAs' search
 // for their stretch, the first loads and the joining of partials take about 12 us of a call that short. One row of 257 tokens:
 // 9 us, the launch and one chain of loads. Walking the KV heads of the same pages side by side in neighbouring CTAs, for
 // the sake of whole pages: 217 and 199 us, and 18.4 against 16.8 for 8 items of 5 drafted tokens.
@@ -62,7 +62,7 @@ struct Cfg {
   static constexpr int kStageBytes = kPages * kBlock;
   static constexpr int kMergeFloats = kRows * (D + 2);  // per warp: outputs, maxima, sums
   static constexpr int kQBytes = (D / 16) * 32 * 16;    // a tile's queries in operand order
-  static constexpr int kRowFloats = 2 * kRows;          // per row: factor and offset of its scores
+  static constexpr int kRowFloats = kRows;              // per row: the factor of its scores
   static constexpr int kFixed = kConsumers * kMergeFloats * 4 + kQBytes + kRowFloats * 4;
   // A whole number of stages for each attending warp: chunk k is warp k % kConsumers's, and so are all the chunks
   // of its stage, so a warp never waits on a barrier that is two phases behind.
@@ -160,21 +160,6 @@ __device__ __forceinline__ void split_half2(float2 x, uint32_t& hi, uint32_t& lo
   hi = *reinterpret_cast<const uint32_t*>(&h);
   const float2 r = __ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), x);  // exact
   lo = pack(r.x, r.y);
-}
-
-// Four key codes as two fp16 pairs times key_unit<KIND>, plus the row's constant (see the file comment).
-template <int KIND>
-__device__ __forceinline__ void widen4_key(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (KIND == NBL_I8) {
-    lo = __byte_perm(w, 0u, 0x4140);
-    hi = __byte_perm(w, 0u, 0x4342);
-  } else {
-    widen4<KIND>(w, lo, hi);
-  }
-}
-template <int KIND>
-constexpr float key_unit() {  // what a score in those units is multiplied by
-  return KIND == NBL_I8 ? 16777216.f : unit<KIND>();
 }
 
 // An item's rows and keys as the kernel takes them; pages 0 when there is nothing to do.
@@ -369,7 +354,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
   // ================= the attending warps
   // The queries of a segment's tile into shared memory in operand order -- 16 bytes for each k-step (4 dims of
   // every lane t) and lane -- each row over its largest power of two, so fp16 holds it whatever its magnitude; and
-  // per row the factor and offset that make a raw product a score: raw * factor * s_k - offset * s_k (log2 units).
+  // per row the factor that makes a raw product a score: raw * factor * s_k (log2 units).
   uint4* s_q = reinterpret_cast<uint4*>(smem + C::kOffQ);
   float* s_row = reinterpret_cast<float*>(smem + C::kOffRow);
   constexpr int kLanes = D / 4;                                               // threads of a row, 4 dims each
@@ -414,21 +399,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
         w[0] = hi0;
         w[2] = hi1;
       }
-      float sum = 0.f;
-      if constexpr (KIND == NBL_I8) {
-        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&hi0));
-        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi1));
-        const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&lo0));
-        const float2 l1 = __half22float2(*reinterpret_cast<const __half2*>(&lo1));
-        sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((l0.x + l0.y) + (l1.x + l1.y));
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      }
-      if (d == 0) {
-        const float scale = __uint_as_float(e << 23) * a.scale_log2;
-        s_row[row] = scale * key_unit<KIND>();
-        s_row[ROWS + row] = 128.f * sum * scale;
-      }
+      if (d == 0) s_row[row] = __uint_as_float(e << 23) * (a.scale_log2 * unit<KIND>());
     }
   };
   // A barrier of the attending warps.
@@ -493,12 +464,11 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
     const int row0 = tile * ROWS, n_rows_item = cc.x.q_len * a.group;
     const int n_here = min(ROWS, n_rows_item - row0);
     const int kv_min = cc.x.pos0 + a.by_group.div(row0) + 1;  // keys that every row of the tile sees
-    float row_scale[NR], row_off[NR];
+    float row_scale[NR];
     int lim[NR];  // keys the row sees
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       row_scale[n] = s_row[g + 8 * n];
-      row_off[n] = s_row[ROWS + g + 8 * n];
       lim[n] = row0 + g + 8 * n < n_rows_item ? cc.x.pos0 + a.by_group.div(row0 + g + 8 * n) + 1 : 0;
     }
     float2 o[D / 8][2];  // dims (8j + 2t, 8j + 2t + 1) of row g; of row g + 8, or of row g's remainder terms
@@ -534,10 +504,10 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
             const uint32_t wa = ks == 0 ? ka[j].x : ks == 1 ? ka[j].y : ks == 2 ? ka[j].z : ka[j].w;
             const uint32_t wb = ks == 0 ? kb[j].x : ks == 1 ? kb[j].y : ks == 2 ? kb[j].z : kb[j].w;
             uint32_t b0, b1;
-            widen4_key<KIND>(wa, b0, b1);
+            widen4<KIND>(wa, b0, b1);
             if (sb == 0 && ks == 0) mma_first(c0[j], q4, b0, b1);
             else mma(c0[j], q4, b0, b1);
-            widen4_key<KIND>(wb, b0, b1);
+            widen4<KIND>(wb, b0, b1);
             if (sb == 0 && ks == 0) mma_first(c1[j], q4, b0, b1);
             else mma(c1[j], q4, b0, b1);
           }
@@ -575,7 +545,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
         for (int j = 0; j < NP; ++j) {
           const float pm = fmaxf(fmaxf(s[n][j][0].x, s[n][j][0].y), fmaxf(s[n][j][1].x, s[n][j][1].y));
           // a page with nothing to see keeps -inf (its scale may be 0, and 0 * -inf is not a number)
-          const float x = fmaf(pm, row_scale[n] * sc[j].x, -row_off[n] * sc[j].x);
+          const float x = pm * (row_scale[n] * sc[j].x);
           mx = fmaxf(mx, !FULL && pm == -INFINITY ? -INFINITY : x);
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -587,10 +557,10 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
         float2 ps = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-          const float f = row_scale[n] * sc[j].x, off = fmaf(-row_off[n], sc[j].x, -mu);
+          const float f = row_scale[n] * sc[j].x;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float2 x = __ffma2_rn(s[n][j][c], make_float2(f, f), make_float2(off, off));
+            const float2 x = __ffma2_rn(s[n][j][c], make_float2(f, f), make_float2(-mu, -mu));
             float2 p = make_float2(ex2(x.x), ex2(x.y));
             if constexpr (!FULL) {
               if (s[n][j][c].x == -INFINITY) p.x = 0.f;

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from nibble_b200.workloads import make_page_tables
-from test_gpu_kv8 import QMAX, attend, dev, export, ints, np_of, random_pool, rows_of
+from test_gpu_kv8 import QMAX, attend, check_decode, dev, export, ints, np_of, random_pool, rows_of
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -160,4 +160,30 @@ def test_prefill_of_uneven_value_scales(nbl_ctx, how, kind, D, H, items, stride)
                 continue  # rows that see little but the loud page
             ro, _, size = attend(qf[starts[i] + t], k, v, p + t + 1)
             assert (np.abs(got[starts[i] + t] - ro) <= 2.0 ** -11 * size + 2e-5 * size.max(-1, keepdims=True)).all(), f"item {i} row {t}"
+    kv.close()
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("mean", [1.0, -4.0])
+def test_attention_of_queries_of_one_sign(nbl_ctx, kind, D, mean):
+    """Queries with a common part (a projection's bias): scores are still good to fp32 accuracy. Decode, and fp32 and 16-bit
+    queries of few tokens. |score| stays below 60, whose fp32 error is 2^-24 * 60 = 4e-6, so test_gpu_kv8's 2e-5 holds."""
+    import torch
+    lens, H, KV = [1, 33, 700, 3000], 8, 2
+    table, n_pages = make_page_tables(lens, shuffle_seed=4)
+    kv, values = random_pool(nbl_ctx, kind, n_pages, KV, D, 5, spread=0.3)
+    rng = np.random.default_rng(6)
+    q = (rng.standard_normal((len(lens), H, D)) + mean).astype(np.float32)
+    check_decode(nbl_ctx, kv, values, table, lens, H, q)
+    for dtype in ("float32", "float16"):
+        x, xf = np_of(q, getattr(torch, dtype))
+        out = torch.full((len(lens), H, D), NAN, device="cuda")
+        nbl_ctx.attn_prefill(kv, x, ints(np.arange(4)), ints([1] * 4), ints(np.array(lens) - 1), dev(table), 1, out)
+        nbl_ctx.check()
+        got = out.cpu().numpy()
+        for r, n in enumerate(lens):
+            k, v = rows_of(values, table[r], n)
+            ro, _, size = attend(xf[r], k, v, n)
+            assert (np.abs(got[r] - ro) <= (0 if dtype == "float32" else 2.0 ** -11) * size + 2e-5 * size.max(-1, keepdims=True)).all()
     kv.close()
