@@ -187,3 +187,26 @@ def test_attention_of_queries_of_one_sign(nbl_ctx, kind, D, mean):
             ro, _, size = attend(xf[r], k, v, n)
             assert (np.abs(got[r] - ro) <= (0 if dtype == "float32" else 2.0 ** -11) * size + 2e-5 * size.max(-1, keepdims=True)).all()
     kv.close()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("mean", [4.0, -16.0])
+def test_decode_scores_of_queries_of_one_sign(nbl_ctx, D, mean):
+    """A score is a sum of D products q_d k_d, whose fp32 error is a small multiple of 2^-24 of sum |q_d k_d| / sqrt(D), whatever the
+    products' signs; lse, over rows of one length and many keys, carries what the scores have in common. Allowed: 2^-21 of the
+    largest such sum (2^-22 for the two fp16 terms of q, as much for the sums)."""
+    import torch
+    lens, H, KV = [2000, 2000, 1999], 16, 4
+    table, n_pages = make_page_tables(lens, shuffle_seed=4)
+    kv, values = random_pool(nbl_ctx, "int8", n_pages, KV, D, 5, spread=0.1)
+    q = (np.random.default_rng(6).standard_normal((len(lens), H, D)) + mean).astype(np.float32)
+    out, lse = torch.empty((len(lens), H, D), device="cuda"), torch.empty((len(lens), H), device="cuda")
+    nbl_ctx.attn_decode(kv, dev(q), dev(table), ints(lens), max(lens), out, lse)
+    nbl_ctx.check()
+    got = lse.double().cpu().numpy()
+    for r, n in enumerate(lens):
+        k, v = rows_of(values, table[r], n)
+        _, want, _ = attend(q[r], k, v, n)
+        size = np.einsum("hd,jhd->hj", np.abs(q[r].astype(np.float64)), np.abs(np.repeat(k, H // KV, 1))).max(1) / np.sqrt(D)
+        assert (np.abs(got[r] - want) <= 2.0 ** -21 * size).all(), f"row {r}"
+    kv.close()
