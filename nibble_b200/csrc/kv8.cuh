@@ -203,9 +203,10 @@ inline bool kv8_few_tokens(int head_dim, int group, int max_len) {
                         : max_len <= 24 && int64_t(max_len) * group <= 72;
 }
 // kv8_prefill.cu: the same for many query tokens of 16-bit type (q and out 16-byte aligned) on the tensor cores. n_rows:
-// rows of q; split keys leave partial results in scratch.
+// rows of q; split keys leave partial results in scratch, as large as the items' rows can be.
 struct Kv8PrefillPlan {
   int n_splits = 1, n_works = 0, grid = 1;
+  int64_t part_rows = 0;  // rows that a part of the split keys has room for
   size_t scratch_bytes = 0;
 };
 Kv8PrefillPlan plan_kv8_prefill(const nbl_kv* kv, int n_items, int max_len, int64_t n_rows, int n_heads, int max_kv,

@@ -59,7 +59,7 @@ constexpr int kRing = 4;                   // works handed from the first conver
 // A work as the issuing and the softmax warps need it.
 struct alignas(16) Slot {
   int t0, n, n_g, head0;  // first tile, tiles (0: no more works), heads, the first
-  int pos, row, live;     // position and row of the tile's first query token, rows of it
+  int pos, row, live;     // position of the tile's first query token, its row of the output (or of the parts), rows of the tile
   int part;               // which part of the work; + kLastPart: the last one
 };
 constexpr int kLastPart = 1 << 16;
@@ -112,7 +112,8 @@ struct PrefillArgs {
   Kv8Items it;
   const uint8_t* pool;
   void* out;
-  float *part_o, *part_lse;  // [n_splits][rows][heads][D] and [n_splits][rows][heads] when n_splits > 1
+  float *part_o, *part_lse;  // [n_splits][part_rows][heads][D] and [n_splits][part_rows][heads] when n_splits > 1
+  int64_t part_rows;         // rows of q, or (fewer) n_items * max_len: a token's row is then item * max_len + its place
   int* err;
   int64_t n_pages;
   int out_dtype;
@@ -125,10 +126,16 @@ struct PrefillArgs {
 
 struct Work {
   int kvh, n_g, head0, qlen, pos0, qs, m0, t0, t1, n_item_pages;
+  int out_row;  // the item's first row of the output, or of the parts
   int split;  // which part of the work this is
   const int32_t* pt_row;
   bool valid, last;  // last: the work's last part
 };
+
+// An item's first row of the parts.
+__device__ __forceinline__ int part_row(const Kv8Items& it, int64_t part_rows, int item, int start) {
+  return part_rows < it.n_rows ? item * it.max_len : start;
+}
 
 // Work w (-1: none); the same in every warp. Works are numbered with the query tile (latest, so heaviest, first) slowest,
 // then the item, the KV head and the heads of the group: the works of a round are about equally long, whatever the
@@ -147,6 +154,7 @@ __device__ __forceinline__ Work decode_work(const PrefillArgs& a, int w) {
   k.qlen = a.it.len[item];
   k.pos0 = a.it.pos0[item];
   k.qs = a.it.start[item];
+  k.out_row = a.n_splits > 1 ? part_row(a.it, a.part_rows, item, k.qs) : k.qs;
   k.m0 = mt * kBM;
   k.valid = k.qlen > 0 && k.m0 < k.qlen;
   if (!k.valid) return k;
@@ -376,7 +384,7 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       if (elect_one()) {
         Slot w{};
         if (wk.valid)
-          w = Slot{wk.t0, wk.t1 - wk.t0, wk.n_g, wk.head0, wk.pos0 + wk.m0, wk.qs + wk.m0, wk.qlen - wk.m0,
+          w = Slot{wk.t0, wk.t1 - wk.t0, wk.n_g, wk.head0, wk.pos0 + wk.m0, wk.out_row + wk.m0, wk.qlen - wk.m0,
                    wk.split + (wk.last ? kLastPart : 0)};
         ring[i] = w;
         mbar_arrive(&bars[C::kBarWFull + i]);
@@ -697,7 +705,7 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       uint8_t* stage = sQ(lw & 1, g) + quarter * (32 * 128);
       const int64_t row_bytes = int64_t(a.n_heads) * D * (wide ? 4 : 2);
       uint8_t* dst = a.n_splits > 1
-                         ? reinterpret_cast<uint8_t*>(a.part_o + int64_t(wk.part & (kLastPart - 1)) * a.it.n_rows * a.n_heads * D)
+                         ? reinterpret_cast<uint8_t*>(a.part_o + int64_t(wk.part & (kLastPart - 1)) * a.part_rows * a.n_heads * D)
                          : static_cast<uint8_t*>(a.out);
       dst += (int64_t(wk.row) + quarter * 32 + (lane >> 3)) * row_bytes + int64_t(wk.head0 + g) * D * (wide ? 4 : 2) + (lane & 7) * 16;
       const int rows = wk.live - quarter * 32 - (lane >> 3);  // of this warp, from this lane's first on
@@ -734,7 +742,7 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
       if (lane == 0) mbar_arrive(&bars[C::kBarQFree + (lw & 1)]);
       if (live && a.n_splits > 1) {
         float* lse = a.part_lse + orow;
-        const int64_t step = a.it.n_rows * a.n_heads;
+        const int64_t step = a.part_rows * a.n_heads;
         const int part = wk.part & (kLastPart - 1);
         lse[part * step] = l_run == 0.f ? -INFINITY : m_ref + log2f(l_run);
         if (wk.part & kLastPart)
@@ -753,14 +761,14 @@ __global__ void __launch_bounds__(PCfg<D, HEADS>::kThreads, PCfg<D, HEADS>::kCta
 // Joins the parts of each (token, head) row: part_lse in log2 units. A thread takes 4 dims.
 template <int D>
 __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse,
-                                                                int n_splits, const Kv8Items it, int n_heads, void* out,
-                                                                int out_dtype) {
+                                                                int n_splits, int64_t part_rows, const Kv8Items it,
+                                                                int n_heads, void* out, int out_dtype) {
   const int item = blockIdx.y;
   const int start = it.start[item], len = it.len[item], pos0 = it.pos0[item];
   if (len <= 0 || !item_fits(it, start, len, pos0)) return;
-  const int64_t rows = it.n_rows * n_heads;
+  const int64_t rows = part_rows * n_heads, first = int64_t(part_row(it, part_rows, item, start)) * n_heads;
   for (int64_t u = blockIdx.x * 256ll + threadIdx.x; u < int64_t(len) * n_heads * (D / 4); u += gridDim.x * 256ll) {
-    const int64_t row = int64_t(start) * n_heads + u / (D / 4);
+    const int64_t row = first + u / (D / 4), to = int64_t(start) * n_heads + u / (D / 4);
     const int d = static_cast<int>(u % (D / 4)) * 4;
     float mx = -INFINITY;
     for (int p = 0; p < n_splits; ++p) mx = fmaxf(mx, part_lse[p * rows + row]);
@@ -774,10 +782,10 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const float* __r
       if (w > 0.f) O.x += w * x.x, O.y += w * x.y, O.z += w * x.z, O.w += w * x.w;
     }
     const float inv = W == 0.f ? 0.f : 1.f / W;
-    store_as(out, row * D + d, O.x * inv, out_dtype);
-    store_as(out, row * D + d + 1, O.y * inv, out_dtype);
-    store_as(out, row * D + d + 2, O.z * inv, out_dtype);
-    store_as(out, row * D + d + 3, O.w * inv, out_dtype);
+    store_as(out, to * D + d, O.x * inv, out_dtype);
+    store_as(out, to * D + d + 1, O.y * inv, out_dtype);
+    store_as(out, to * D + d + 2, O.z * inv, out_dtype);
+    store_as(out, to * D + d + 3, O.w * inv, out_dtype);
   }
 }
 
@@ -836,8 +844,9 @@ Kv8PrefillPlan plan_kv8_prefill(const nbl_kv* kv, int n_items, int max_len, int6
     p.n_splits = static_cast<int>(std::min({(slots + works - 1) / works + 1, max_tiles / kMinShare + 2, int64_t(64)}));
     p.grid = static_cast<int>(slots);
   }
+  p.part_rows = std::min(n_rows, int64_t(n_items) * max_len);
   if (p.n_splits > 1)
-    p.scratch_bytes = size_t(p.n_splits) * size_t(n_rows) * size_t(n_heads) * (kv->cfg.head_dim + 1) * sizeof(float);
+    p.scratch_bytes = size_t(p.n_splits) * size_t(p.part_rows) * size_t(n_heads) * (kv->cfg.head_dim + 1) * sizeof(float);
   return p;
 }
 
@@ -856,7 +865,8 @@ void launch_kv8_prefill(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items
   a.pool = static_cast<const uint8_t*>(kv->pool);
   a.out = out;
   a.part_o = static_cast<float*>(scratch);
-  a.part_lse = a.part_o + int64_t(plan.n_splits) * items.n_rows * n_heads * d;
+  a.part_rows = plan.part_rows;
+  a.part_lse = a.part_o + int64_t(plan.n_splits) * plan.part_rows * n_heads * d;
   a.err = err;
   a.n_pages = c.n_pages;
   a.out_dtype = out_dtype;
@@ -880,9 +890,11 @@ void launch_kv8_prefill(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items
     const int64_t units = int64_t(items.max_len) * n_heads * (d / 4);
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, 1184)), static_cast<unsigned>(items.n_items));
     if (d == 64)
-      kv8_prefill_merge_kernel<64><<<grid, 256, 0, st>>>(a.part_o, a.part_lse, plan.n_splits, items, n_heads, out, out_dtype);
+      kv8_prefill_merge_kernel<64><<<grid, 256, 0, st>>>(a.part_o, a.part_lse, plan.n_splits, plan.part_rows, items, n_heads, out,
+                                                         out_dtype);
     else
-      kv8_prefill_merge_kernel<128><<<grid, 256, 0, st>>>(a.part_o, a.part_lse, plan.n_splits, items, n_heads, out, out_dtype);
+      kv8_prefill_merge_kernel<128><<<grid, 256, 0, st>>>(a.part_o, a.part_lse, plan.n_splits, plan.part_rows, items, n_heads, out,
+                                                         out_dtype);
     check_cuda(cudaGetLastError(), "kv8 prefill merge launch");
   }
 }

@@ -210,3 +210,33 @@ def test_decode_scores_of_queries_of_one_sign(nbl_ctx, D, mean):
         size = np.einsum("hd,jhd->hj", np.abs(q[r].astype(np.float64)), np.abs(np.repeat(k, H // KV, 1))).max(1) / np.sqrt(D)
         assert (np.abs(got[r] - want) <= 2.0 ** -21 * size).all(), f"row {r}"
     kv.close()
+
+
+@pytest.mark.parametrize("items", [[(4000, 128)], [(3000, 70), (0, 130), (2900, 100)]])
+def test_split_prefill_inside_a_large_buffer(nbl_ctx, items):
+    """Few tokens of a long buffer of activations: the scratch goes by the tokens that the call can have."""
+    import torch
+    import nibble_b200 as nb
+    H, KV, D, n = 8, 2, 128, 32768
+    table, n_pages = make_page_tables([p + m for p, m in items], shuffle_seed=1)
+    ctx = nb.Context(0)  # no scratch yet
+    try:
+        kv, values = random_pool(ctx, "int8", n_pages, KV, D, 3, spread=0.5)
+        starts = [n - 1000 * (i + 1) for i in range(len(items))]
+        q, qf = np_of(np.random.default_rng(2).standard_normal((n, H, D)).astype(np.float32), torch.float16)
+        out = torch.full((n, H, D), NAN, device="cuda", dtype=torch.float16)
+        args = (ints(starts), ints([m for _, m in items]), ints([p for p, _ in items]), dev(table), max(m for _, m in items), out)
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        ctx.attn_prefill(kv, q, *args)
+        ctx.check()
+        assert before - torch.cuda.mem_get_info()[0] < 64 << 20
+        got = out.float().cpu().numpy()
+        written = np.zeros(n, bool)
+        for i, (p, m) in enumerate(items):
+            check_rows(got, qf, values, table[i], starts[i], p, m, "float16", every=9)
+            written[starts[i]:starts[i] + m] = True
+        assert np.isnan(got[~written]).all() and not np.isnan(got[written]).any()
+        kv.close()
+    finally:
+        ctx.close()
