@@ -300,7 +300,7 @@ void kv8_attention(nbl_ctx* ctx, const nbl_kv* kv, const nbl::Kv8Items& it, cons
                        nbl::split_counts(ctx, plan.grid), ctx->d_err);
 }
 
-// nbl_attn_decode on an 8-bit pool (pointers and context checked).
+// nbl_attn_decode on an 8-bit pool (context checked; with no rows there are no arrays).
 void kv8_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_t* page_table, int32_t pt_stride,
                 const int32_t* seq_lens, int32_t max_seq_len, int32_t n_rows, int32_t n_heads, float* out, float* lse,
                 int32_t n_splits) {
@@ -309,6 +309,7 @@ void kv8_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_t* p
   require(int64_t(pt_stride) * kv->cfg.page_size <= INT32_MAX && int64_t(max_seq_len) <= int64_t(pt_stride) * kv->cfg.page_size,
           "attn_decode: max_seq_len exceeds pt_stride * page_size");
   if (n_rows == 0) return;
+  require(q && page_table && seq_lens && out, "attn_decode: NULL argument");
   nbl::Kv8Items it;
   it.pos0 = seq_lens;
   it.page_table = page_table;
@@ -319,7 +320,7 @@ void kv8_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_t* p
   kv8_attention(ctx, kv, it, q, NBL_F32, n_heads, out, NBL_F32, lse, max_seq_len);
 }
 
-// nbl_attn_prefill on an 8-bit pool (pointers and context checked).
+// nbl_attn_prefill on an 8-bit pool (context checked; with no items or rows there are no arrays).
 void kv8_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype, int64_t n_q_rows,
                  const int32_t* q_start, const int32_t* q_len, const int32_t* kv_pos0, const int32_t* page_table,
                  int32_t pt_stride, int32_t n_items, int32_t n_heads, int32_t max_q_len, void* out, int32_t out_dtype) {
@@ -329,6 +330,7 @@ void kv8_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype,
   require(int64_t(pt_stride) * kv->cfg.page_size <= INT32_MAX, "attn_prefill: pt_stride too large");
   require(n_heads > 0 && n_heads % kv->cfg.n_kv_heads == 0, "attn_prefill: n_heads must be a multiple of n_kv_heads");
   if (n_items == 0 || max_q_len == 0 || n_q_rows == 0) return;
+  require(q && q_start && q_len && kv_pos0 && page_table && out, "attn_prefill: NULL argument");
   nbl::Kv8Items it;
   it.start = q_start;
   it.len = q_len;
@@ -723,13 +725,16 @@ int nbl_attn_decode(nbl_ctx* ctx, const nbl_kv* kv, const float* q, const int32_
                     const int32_t* seq_lens, int32_t max_seq_len, int32_t n_rows, int32_t n_heads, float* out,
                     float* lse, int32_t n_splits) {
   return guarded([&] {
-    require(ctx && kv && q && page_table && seq_lens && out, "attn_decode: NULL argument");
-    nbl::route_flush_queries(ctx);
-    require(kv->ctx == ctx, "attn_decode: pool belongs to another context");
+    require(ctx && kv, "attn_decode: NULL argument");
     if (nbl::is_kv8(kv->cfg.dtype)) {
+      nbl::route_flush_queries(ctx);
+      require(kv->ctx == ctx, "attn_decode: pool belongs to another context");
       kv8_decode(ctx, kv, q, page_table, pt_stride, seq_lens, max_seq_len, n_rows, n_heads, out, lse, n_splits);
       return;
     }
+    require(q && page_table && seq_lens && out, "attn_decode: NULL argument");
+    nbl::route_flush_queries(ctx);
+    require(kv->ctx == ctx, "attn_decode: pool belongs to another context");
     require(kv->cfg.dtype == NBL_F16, "attn_decode: the decode kernel reads an NBL_F16, NBL_I8 or NBL_E4M3 pool");
     require(n_rows >= 0 && pt_stride > 0 && max_seq_len >= 0 && n_splits >= 0, "attn_decode: negative size");
     require(n_heads > 0 && n_heads % kv->cfg.n_kv_heads == 0 && n_heads / kv->cfg.n_kv_heads <= 8,
@@ -860,14 +865,17 @@ int nbl_attn_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dt
                      int32_t pt_stride, int32_t n_items, int32_t n_heads, int32_t max_q_len, void* out,
                      int32_t out_dtype) {
   return guarded([&] {
-    require(ctx && kv && q && q_start && q_len && kv_pos0 && page_table && out, "attn_prefill: NULL argument");
-    nbl::route_flush_queries(ctx);
-    require(kv->ctx == ctx, "attn_prefill: pool belongs to another context");
+    require(ctx && kv, "attn_prefill: NULL argument");
     if (nbl::is_kv8(kv->cfg.dtype)) {
+      nbl::route_flush_queries(ctx);
+      require(kv->ctx == ctx, "attn_prefill: pool belongs to another context");
       kv8_prefill(ctx, kv, q, q_dtype, n_q_rows, q_start, q_len, kv_pos0, page_table, pt_stride, n_items, n_heads,
                   max_q_len, out, out_dtype);
       return;
     }
+    require(q && q_start && q_len && kv_pos0 && page_table && out, "attn_prefill: NULL argument");
+    nbl::route_flush_queries(ctx);
+    require(kv->ctx == ctx, "attn_prefill: pool belongs to another context");
     require(q_dtype == kv->cfg.dtype, "attn_prefill: q must have the pool's dtype");
     require(out_dtype == NBL_F32 || out_dtype == kv->cfg.dtype, "attn_prefill: out must be F32 or the pool dtype");
     require(n_items >= 0 && pt_stride > 0 && max_q_len >= 0 && n_q_rows >= 0, "attn_prefill: negative size");

@@ -28,6 +28,12 @@ void require(bool ok, const char* what, const char* msg) {
   if (!ok) nbl::fail(NBL_E_INVALID, std::string(what) + ": " + msg);
 }
 
+// The arrays of a call that has work: an empty one's pointer may be NULL.
+template <class... P>
+void require_arrays(const char* what, const P*... p) {
+  require((... && (p != nullptr)), what, "NULL argument");
+}
+
 void use(nbl_ctx* ctx) {
   nbl::check_cuda(cudaSetDevice(ctx->device), "cudaSetDevice");
   nbl::route_flush_queries(ctx);
@@ -195,14 +201,14 @@ int nbl_rotary_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const void*
                          int32_t n_heads, int32_t max_q_len, const nbl_rotary_params* rotary) {
   return guarded([&] {
     const char* what = "rotary_kv_append";
-    require(ctx && kv && q_in && k_in && v_in && q_out && q_start && q_len && kv_pos0 && page_table && rotary,
-            what, "NULL argument");
+    require(ctx && kv && rotary, what, "NULL argument");
     require_kv8(ctx, kv, what);
     require(is_float(in_dtype) && is_float(q_out_dtype), what, "bad dtype");
     require(n_heads > 0 && n_heads % kv->cfg.n_kv_heads == 0, what, "n_heads must be a multiple of n_kv_heads");
     const auto it = items_of(kv, n_rows, q_start, q_len, kv_pos0, page_table, pt_stride, n_items, max_q_len, what);
     check_rotary(*rotary, kv->cfg.head_dim, what);
     if (n_items == 0 || max_q_len == 0 || n_rows == 0) return;
+    require_arrays(what, q_in, k_in, v_in, q_out, q_start, q_len, kv_pos0, page_table);
     use(ctx);
     nbl::Kv8Append a;
     a.q_in = q_in;
@@ -229,11 +235,12 @@ int nbl_kv_read(nbl_ctx* ctx, const nbl_kv* kv, int64_t n_rows, const int32_t* s
                 void* k_out, void* v_out, int32_t out_dtype) {
   return guarded([&] {
     const char* what = "kv_read";
-    require(ctx && kv && start && len && kv_pos0 && page_table && (k_out || v_out), what, "NULL argument");
+    require(ctx && kv, what, "NULL argument");
     require_kv8(ctx, kv, what);
     require(is_float(out_dtype), what, "bad dtype");
     const auto it = items_of(kv, n_rows, start, len, kv_pos0, page_table, pt_stride, n_items, max_len, what);
     if (n_items == 0 || max_len == 0 || n_rows == 0) return;
+    require_arrays(what, start, len, kv_pos0, page_table, k_out ? k_out : v_out);
     use(ctx);
     nbl::launch_kv8_read(ctx->stream, kv, it, k_out, v_out, out_dtype, ctx->d_err);
   });
@@ -241,10 +248,11 @@ int nbl_kv_read(nbl_ctx* ctx, const nbl_kv* kv, int64_t n_rows, const int32_t* s
 
 int nbl_kv_import(nbl_ctx* ctx, nbl_kv* kv, const int32_t* page_ids, int64_t n, const void* codes, const float* scales) {
   return guarded([&] {
-    require(ctx && kv && page_ids && codes && scales, "kv_import", "NULL argument");
+    require(ctx && kv, "kv_import", "NULL argument");
     require_kv8(ctx, kv, "kv_import");
     require(n >= 0 && n <= INT32_MAX, "kv_import", "bad page count");
     if (n == 0) return;
+    require_arrays("kv_import", page_ids, codes, scales);
     use(ctx);
     nbl::launch_kv8_import(ctx->stream, kv, page_ids, n, codes, scales, ctx->d_err);
   });
@@ -252,10 +260,11 @@ int nbl_kv_import(nbl_ctx* ctx, nbl_kv* kv, const int32_t* page_ids, int64_t n, 
 
 int nbl_kv_export(nbl_ctx* ctx, const nbl_kv* kv, const int32_t* page_ids, int64_t n, void* codes, float* scales) {
   return guarded([&] {
-    require(ctx && kv && page_ids && codes && scales, "kv_export", "NULL argument");
+    require(ctx && kv, "kv_export", "NULL argument");
     require_kv8(ctx, kv, "kv_export");
     require(n >= 0 && n <= INT32_MAX, "kv_export", "bad page count");
     if (n == 0) return;
+    require_arrays("kv_export", page_ids, codes, scales);
     use(ctx);
     nbl::launch_kv8_export(ctx->stream, kv, page_ids, n, codes, scales, ctx->d_err);
   });
@@ -263,10 +272,11 @@ int nbl_kv_export(nbl_ctx* ctx, const nbl_kv* kv, const int32_t* page_ids, int64
 
 int nbl_kv_copy_pages(nbl_ctx* ctx, nbl_kv* kv, const int32_t* src_pages, const int32_t* dst_pages, int32_t n) {
   return guarded([&] {
-    require(ctx && kv && src_pages && dst_pages, "kv_copy_pages", "NULL argument");
+    require(ctx && kv, "kv_copy_pages", "NULL argument");
     require_pool(ctx, kv, "kv_copy_pages");
     require(n >= 0, "kv_copy_pages", "negative size");
     if (n == 0) return;
+    require_arrays("kv_copy_pages", src_pages, dst_pages);
     use(ctx);
     nbl::launch_copy_pages(ctx->stream, kv, src_pages, dst_pages, n, ctx->d_err, ctx->num_sms);
   });
@@ -275,11 +285,12 @@ int nbl_kv_copy_pages(nbl_ctx* ctx, nbl_kv* kv, const int32_t* src_pages, const 
 int nbl_kv_fork(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride, int32_t n_rows, int32_t* seq_lens,
                 int32_t* ref_counts, const int32_t* src_rows, const int32_t* dst_rows, int32_t n) {
   return guarded([&] {
-    require(ctx && kv && page_table && seq_lens && ref_counts && src_rows && dst_rows, "kv_fork", "NULL argument");
+    require(ctx && kv, "kv_fork", "NULL argument");
     require_pool(ctx, kv, "kv_fork");
     const auto b = book_of(kv, page_table, pt_stride, n_rows, seq_lens, ref_counts, "kv_fork");
     require(n >= 0 && n <= n_rows, "kv_fork", "n must be 0..n_rows");
     if (n == 0) return;
+    require_arrays("kv_fork", page_table, seq_lens, ref_counts, src_rows, dst_rows);
     use(ctx);
     nbl::ensure_scratch(ctx, nbl::kv_book_scratch(n, kv->cfg.n_pages));
     nbl::launch_kv_fork(ctx->stream, kv, b, src_rows, dst_rows, n, ctx->scratch, nbl::split_counts(ctx, 1), ctx->d_err);
@@ -289,11 +300,12 @@ int nbl_kv_fork(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride
 int nbl_kv_release(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride, int32_t n_rows, int32_t* seq_lens,
                    int32_t* ref_counts, const int32_t* rows, int32_t n) {
   return guarded([&] {
-    require(ctx && kv && page_table && seq_lens && ref_counts && rows, "kv_release", "NULL argument");
+    require(ctx && kv, "kv_release", "NULL argument");
     require_pool(ctx, kv, "kv_release");
     const auto b = book_of(kv, page_table, pt_stride, n_rows, seq_lens, ref_counts, "kv_release");
     require(n >= 0, "kv_release", "negative size");
     if (n == 0) return;
+    require_arrays("kv_release", page_table, seq_lens, ref_counts, rows);
     use(ctx);
     nbl::launch_kv_release(ctx->stream, b, rows, n, ctx->d_err);
   });
@@ -302,11 +314,12 @@ int nbl_kv_release(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_str
 int nbl_kv_extend(nbl_ctx* ctx, nbl_kv* kv, int32_t* page_table, int32_t pt_stride, int32_t n_rows, int32_t* seq_lens,
                   int32_t* ref_counts, const int32_t* rows, const int32_t* new_lens, int32_t n) {
   return guarded([&] {
-    require(ctx && kv && page_table && seq_lens && ref_counts && rows && new_lens, "kv_extend", "NULL argument");
+    require(ctx && kv, "kv_extend", "NULL argument");
     require_pool(ctx, kv, "kv_extend");
     const auto b = book_of(kv, page_table, pt_stride, n_rows, seq_lens, ref_counts, "kv_extend");
     require(n >= 0 && n <= n_rows, "kv_extend", "n must be 0..n_rows");
     if (n == 0) return;
+    require_arrays("kv_extend", page_table, seq_lens, ref_counts, rows, new_lens);
     use(ctx);
     nbl::ensure_scratch(ctx, nbl::kv_book_scratch(n, kv->cfg.n_pages));
     nbl::launch_kv_extend(ctx->stream, b, rows, new_lens, n, ctx->scratch, ctx->d_err);
@@ -317,15 +330,14 @@ int nbl_kv_compact(nbl_ctx* ctx, const nbl_kv* src, nbl_kv* dst, const int32_t* 
                    int32_t n_rows, const int32_t* seq_lens, int32_t* table_out, int32_t* ref_counts_out,
                    int32_t* n_used) {
   return guarded([&] {
-    require(ctx && src && dst && page_table && seq_lens && table_out && ref_counts_out && n_used,
-            "kv_compact", "NULL argument");
+    require(ctx && src && dst && ref_counts_out && n_used, "kv_compact", "NULL argument");
     require_pool(ctx, src, "kv_compact");
     require_pool(ctx, dst, "kv_compact");
     const auto &s = src->cfg, &d = dst->cfg;
     require(src != dst && s.dtype == d.dtype && s.head_dim == d.head_dim && s.n_kv_heads == d.n_kv_heads &&
                 s.page_size == d.page_size,
             "kv_compact", "the pools must be two of the same dtype, head_dim, n_kv_heads and page_size");
-    require(page_table != table_out, "kv_compact", "table_out must not be page_table");
+    require(n_rows == 0 || page_table != table_out, "kv_compact", "table_out must not be page_table");
     const auto b = book_of(src, const_cast<int32_t*>(page_table), pt_stride, n_rows, const_cast<int32_t*>(seq_lens),
                            nullptr, "kv_compact");
     require(int64_t(n_rows) * pt_stride <= INT32_MAX, "kv_compact", "n_rows * pt_stride exceeds 2^31");
@@ -335,6 +347,7 @@ int nbl_kv_compact(nbl_ctx* ctx, const nbl_kv* src, nbl_kv* dst, const int32_t* 
       nbl::check_cuda(cudaMemsetAsync(ref_counts_out, 0, size_t(d.n_pages) * sizeof(int32_t), ctx->stream), "kv_compact");
       return;
     }
+    require_arrays("kv_compact", page_table, seq_lens, table_out);
     nbl::ensure_scratch(ctx, nbl::kv_compact_scratch(n_rows, s.n_pages));
     nbl::launch_kv_compact(ctx->stream, src, dst, b, table_out, ref_counts_out, n_used, ctx->scratch, ctx->d_err,
                            ctx->num_sms);

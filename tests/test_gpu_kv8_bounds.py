@@ -240,3 +240,52 @@ def test_split_prefill_inside_a_large_buffer(nbl_ctx, items):
         kv.close()
     finally:
         ctx.close()
+
+
+def test_empty_calls_are_no_work(nbl_ctx):
+    """No rows, no items, no pages, empty lists: nothing is refused, nothing changes."""
+    import torch
+    import nibble_b200 as nb
+    lens = [40, 17]
+    table, n_pages = make_page_tables(lens, shuffle_seed=1)
+    kv, _ = random_pool(nbl_ctx, "int8", n_pages, 2, 64, 3)
+    before = export(nbl_ctx, kv)
+    book = dev(table), ints(lens), ints(np.ones(n_pages))
+    kept = [t.clone() for t in book]
+    none, no_rows = ints([]), ints(np.zeros((0, table.shape[1])))
+
+    def empty(heads, dtype=torch.float32):
+        return torch.zeros((0, heads, 64), device="cuda", dtype=dtype)
+
+    assert none.data_ptr() == 0
+    nbl_ctx.rotary_kv_append(kv, empty(4), empty(2), empty(2), empty(4), none, none, none, no_rows, 0, nb.RotarySpec(1e4, True))
+    nbl_ctx.rotary_kv_append(kv, empty(4), empty(2), empty(2), empty(4), none, none, none, no_rows, 7, nb.RotarySpec(1e4, True))
+    nbl_ctx.kv_read(kv, none, none, none, no_rows, 7, empty(2), empty(2))
+    nbl_ctx.attn_decode(kv, empty(4), no_rows, none, 0, empty(4), torch.zeros((0, 4), device="cuda"))
+    for dtype in (torch.float32, torch.half):
+        nbl_ctx.attn_prefill(kv, empty(4, dtype), none, none, none, no_rows, 7, empty(4, dtype))
+    for call in (nbl_ctx.kv_import, nbl_ctx.kv_export):
+        call(kv, none, torch.zeros((0, 2, 2, 16, 64), device="cuda", dtype=torch.int8), torch.zeros((0, 2, 2), device="cuda"))
+    nbl_ctx.kv_copy_pages(kv, none, none)
+    nbl_ctx.kv_fork(kv, *book, none, none)
+    nbl_ctx.kv_extend(kv, *book, none, none)
+    nbl_ctx.kv_release(kv, *book, none)
+    # items without tokens among the rows
+    out = torch.full((3, 4, 64), NAN, device="cuda")
+    q, k = torch.ones((3, 4, 64), device="cuda"), torch.ones((3, 2, 64), device="cuda")
+    zero, start = ints([0, 0]), ints([0, 3])
+    nbl_ctx.rotary_kv_append(kv, q, k, k, out, start, zero, zero, dev(table), 3, nb.RotarySpec(1e4, True))
+    nbl_ctx.attn_prefill(kv, q, start, zero, zero, dev(table), 3, out)
+    nbl_ctx.kv_read(kv, start, zero, zero, dev(table), 3, out[:, :2].contiguous())
+    nbl_ctx.check()
+    assert out.isnan().all()
+    assert all(torch.equal(a, b) for a, b in zip(book, kept))
+    assert all(np.array_equal(a, b) for a, b in zip(export(nbl_ctx, kv), before))
+    # a table without rows
+    small = nbl_ctx.kv_pool(3, 2, dtype=nb.I8)
+    refs, used = ints([5, 5, 5]), ints([9])
+    nbl_ctx.kv_compact(kv, small, no_rows, none, no_rows.clone(), refs, used)
+    nbl_ctx.check()
+    assert refs.tolist() == [0, 0, 0] and used.item() == 0
+    kv.close()
+    small.close()
