@@ -106,6 +106,7 @@ struct AttnArgs {
   int64_t n_pages;
   int q_dtype, out_dtype;
   int n_heads, n_kv_heads, group;
+  int tile0, n_tiles;  // the items' query tiles of this launch
   FastDiv by_group, by_kv_heads;
   int q_vec;         // q allows 4-element loads
   float scale_log2;  // log2(e) / sqrt(D)
@@ -187,7 +188,8 @@ __device__ __forceinline__ Item load_item(const AttnArgs& a, int i) {
     x.q_start = i, x.q_len = 1, x.pos0 = len - 1;
     x.pages = (len + kPage - 1) / kPage;
   }
-  x.subs = a.n_kv_heads * ((x.q_len * a.group + ROWS - 1) / ROWS);  // ROWS: 8 or 16
+  x.subs = a.n_kv_heads * min(max((x.q_len * a.group + ROWS - 1) / ROWS - a.tile0, 0), a.n_tiles);  // ROWS: 8 or 16
+  if (x.subs == 0) x.pages = 0;
   return x;
 }
 
@@ -360,7 +362,8 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
   constexpr int kLanes = D / 4;                                               // threads of a row, 4 dims each
   constexpr int kQSteps = (ROWS * kLanes + kConsumers * 32 - 1) / (kConsumers * 32);
   auto read_queries = [&](const Cursor& c, float (&x)[kQSteps][4]) {
-    const int tile = a.by_kv_heads.div(c.sub), kvh = c.sub - tile * a.n_kv_heads, n_rows_item = c.x.q_len * a.group;
+    const int t_sub = a.by_kv_heads.div(c.sub), kvh = c.sub - t_sub * a.n_kv_heads, tile = a.tile0 + t_sub;
+    const int n_rows_item = c.x.q_len * a.group;
 #pragma unroll
     for (int i = 0; i < kQSteps; ++i) {
       const int u = i * kConsumers * 32 + threadIdx.x;
@@ -460,7 +463,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
   float* mrg = reinterpret_cast<float*>(smem + C::kOffMerge);
 
   for (;;) {  // segments
-    const int tile = a.by_kv_heads.div(cc.sub), kvh = cc.sub - tile * a.n_kv_heads;
+    const int t_sub = a.by_kv_heads.div(cc.sub), kvh = cc.sub - t_sub * a.n_kv_heads, tile = a.tile0 + t_sub;
     const int row0 = tile * ROWS, n_rows_item = cc.x.q_len * a.group;
     const int n_here = min(ROWS, n_rows_item - row0);
     const int kv_min = cc.x.pos0 + a.by_group.div(row0) + 1;  // keys that every row of the tile sees
@@ -771,10 +774,9 @@ Kv8AttnPlan plan_kv8_attn(const nbl_kv* kv, int n_items, int max_len, int n_head
   return with_cfg(kv->cfg.head_dim, q_dtype == NBL_F32, [&](auto cfg) {
     using C = decltype(cfg);
     Kv8AttnPlan p;
-    const int64_t tiles = (int64_t(max_len) * (n_heads / kv->cfg.n_kv_heads) + C::kRows - 1) / C::kRows;
+    p.seg_cost = C::kSegCost;
+    const int64_t tiles = p.tiles = (int64_t(max_len) * (n_heads / kv->cfg.n_kv_heads) + C::kRows - 1) / C::kRows;
     const int64_t max_pages = std::max(1, (max_kv + kPage - 1) / kPage);
-    if (double(n_items) * kv->cfg.n_kv_heads * double(tiles) * (double(max_pages) + C::kSegCost) > 2.0e9)
-      fail(NBL_E_INVALID, "attention: over 2^31 pages of all rows, heads and query tiles in one call");
     // one wave of CTAs, or one for each kSegCost + 1 of the most that the call can cost
     const double bound = double(n_items) * kv->cfg.n_kv_heads * double(tiles) * (double(max_pages) + C::kSegCost) / (C::kSegCost + 1);
     const int slots = num_sms * C::kCtas;
@@ -808,12 +810,32 @@ void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, c
   const uintptr_t bits = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out);
   a.q_vec = (bits & 15u) == 0;
   a.scale_log2 = 1.4426950408889634f / std::sqrt(static_cast<float>(c.head_dim));
-  if (c.head_dim == 64) {
-    if (c.dtype == NBL_I8) launch_q<64, NBL_I8>(st, a, plan.grid);
-    else launch_q<64, NBL_E4M3>(st, a, plan.grid);
-  } else {
-    if (c.dtype == NBL_I8) launch_q<128, NBL_I8>(st, a, plan.grid);
-    else launch_q<128, NBL_E4M3>(st, a, plan.grid);
+  // The kernel counts the pages of all units in 32 bits: a launch takes as many items and query tiles as that allows, were
+  // every item as long as its page-table row (one launch but for many fp32 queries or very wide tables).
+  const int64_t cost = int64_t(c.n_kv_heads) * (items.pt_stride + plan.seg_cost), most = 2000000000;
+  if (cost > most) fail(NBL_E_INVALID, "attention: over 2^31 pages of all heads in a page-table row");
+  const int64_t tiles = std::min(plan.tiles, most / cost), n = std::min<int64_t>(items.n_items, most / (cost * tiles));
+  for (int64_t i = 0; i < items.n_items; i += n) {
+    a.it.n_items = static_cast<int>(std::min(n, items.n_items - i));
+    a.it.page_table = items.page_table + i * items.pt_stride;
+    a.it.pos0 = items.pos0 + i;
+    if (items.len) {
+      a.it.start = items.start + i, a.it.len = items.len + i;
+    } else {
+      const int64_t row = int64_t(n_heads) * c.head_dim;
+      a.q = static_cast<const float*>(q) + i * row, a.out = static_cast<float*>(out) + i * row;
+      if (lse) a.lse = lse + i * n_heads;
+    }
+    for (int64_t t = 0; t < plan.tiles; t += tiles) {
+      a.tile0 = static_cast<int>(t), a.n_tiles = static_cast<int>(tiles);
+      if (c.head_dim == 64) {
+        if (c.dtype == NBL_I8) launch_q<64, NBL_I8>(st, a, plan.grid);
+        else launch_q<64, NBL_E4M3>(st, a, plan.grid);
+      } else {
+        if (c.dtype == NBL_I8) launch_q<128, NBL_I8>(st, a, plan.grid);
+        else launch_q<128, NBL_E4M3>(st, a, plan.grid);
+      }
+    }
   }
   check_cuda(cudaGetLastError(), "kv8 attention launch");
 }

@@ -289,3 +289,24 @@ def test_empty_calls_are_no_work(nbl_ctx):
     assert refs.tolist() == [0, 0, 0] and used.item() == 0
     kv.close()
     small.close()
+
+
+@pytest.mark.parametrize("width,items", [(170_000, [(3, 1000), (0, 40), (500, 900)]), (4_000_000, [(70, 1000)])])
+def test_prefill_with_a_wide_page_table(nbl_ctx, width, items):
+    """A table row's width is no work: fp32 queries whose tiles times the width pass 2^31 are attended in several launches."""
+    import torch
+    H, KV, D = 32, 8, 64
+    narrow, n_pages = make_page_tables([p + m for p, m in items], shuffle_seed=1)
+    table = np.full((len(items), width), -1, np.int32)
+    table[:, :narrow.shape[1]] = narrow
+    kv, values = random_pool(nbl_ctx, "int8", n_pages, KV, D, 3, spread=0.5)
+    starts = np.cumsum([0] + [m for _, m in items])[:-1]
+    q, qf = np_of(np.random.default_rng(1).standard_normal((sum(m for _, m in items), H, D)).astype(np.float32), torch.float32)
+    out = torch.full_like(q, NAN)
+    nbl_ctx.attn_prefill(kv, q, ints(starts), ints([m for _, m in items]), ints([p for p, _ in items]), dev(table), 1000, out)
+    nbl_ctx.check()
+    got = out.cpu().numpy()
+    assert not np.isnan(got).any()
+    for i, (p, m) in enumerate(items):
+        check_rows(got, qf, values, table[i], starts[i], p, m, "float32", every=29)
+    kv.close()
