@@ -338,9 +338,10 @@ void kv8_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype,
   it.page_table = page_table;
   it.pt_stride = pt_stride;
   it.n_items = n_items;
+  const int max_kv = pt_stride * kv->cfg.page_size;
+  max_q_len = static_cast<int32_t>(std::min<int64_t>({max_q_len, n_q_rows, max_kv}));  // a longer item is out of bounds
   it.max_len = max_q_len;
   it.n_rows = n_q_rows;
-  const int max_kv = pt_stride * kv->cfg.page_size;
   const bool aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
   const bool few = nbl::kv8_few_tokens(kv->cfg.head_dim, n_heads / kv->cfg.n_kv_heads, max_q_len);
   if (q_dtype == NBL_F32 || !aligned || few || n_items > 65535 || n_q_rows * n_heads >= (int64_t(1) << 31)) {

@@ -310,3 +310,20 @@ def test_prefill_with_a_wide_page_table(nbl_ctx, width, items):
     for i, (p, m) in enumerate(items):
         check_rows(got, qf, values, table[i], starts[i], p, m, "float32", every=29)
     kv.close()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("most", [150, 10_000, 2 ** 31 - 1])
+def test_prefill_with_a_loose_max_q_len(nbl_ctx, dtype, most):
+    """max_q_len only bounds the items: any larger one gives the same."""
+    import torch
+    items, H, KV, D = [(900, 150), (0, 60)], 4, 2, 64
+    table, n_pages = make_page_tables([p + m for p, m in items], shuffle_seed=1)
+    kv, values = random_pool(nbl_ctx, "e4m3", n_pages, KV, D, 3, spread=0.5)
+    q, qf = np_of(np.random.default_rng(1).standard_normal((210, H, D)).astype(np.float32), getattr(torch, dtype))
+    out = torch.full_like(q, NAN)
+    nbl_ctx.attn_prefill(kv, q, ints([0, 150]), ints([150, 60]), ints([900, 0]), dev(table), most, out)
+    nbl_ctx.check()
+    for i, (p, m) in enumerate(items):
+        check_rows(out.float().cpu().numpy(), qf, values, table[i], (0, 150)[i], p, m, dtype, every=11)
+    kv.close()
