@@ -256,7 +256,8 @@ NBL_API int nbl_rope_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const
  * from the sizes); more than one uses context scratch sized by nbl_reserve (grown on demand otherwise).
  * head_dim 64, n_heads / n_kv_heads <= 8.
  * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes any group size; n_splits is then not used, the pages of all
- * rows being divided evenly over the GPU whatever their lengths. The results are the softmax over the values that the
+ * rows being divided evenly over the GPU whatever their lengths, and a call allocates nothing (its scratch comes with the
+ * context's first 8-bit pool), so it may be captured into a CUDA graph. The results are the softmax over the values that the
  * codes stand for, to fp32 accuracy (and to 2^-38 of the largest value scale among the row's pages: where a row all but
  * ignores pages 2^17 times as loud as those that it attends, the latter's values lose bits); a head whose query has an
  * infinity or NaN gets NaN in out and lse. */

@@ -290,14 +290,13 @@ void qblock_matmul(nbl_ctx* ctx, const nbl_weight* w, float* y, const float* x, 
   nbl::launch_qblock_matmul(ctx->stream, w->w, y, x, n, ctx->qblock_act, ctx->num_sms);
 }
 
-// Attention over an 8-bit pool: plans the grid, grows the scratch and launches.
+// Attention over an 8-bit pool by the warp-level kernel. Its scratch has one size and place, so a call allocates nothing and
+// a captured one stays good.
 void kv8_attention(nbl_ctx* ctx, const nbl_kv* kv, const nbl::Kv8Items& it, const void* q, int q_dtype, int n_heads,
                    void* out, int out_dtype, float* lse, int max_kv) {
   use_device(ctx);
   const auto plan = nbl::plan_kv8_attn(kv, it.n_items, it.max_len, n_heads, max_kv, q_dtype, ctx->num_sms);
-  ensure_scratch(ctx, plan.scratch_bytes);
-  nbl::launch_kv8_attn(ctx->stream, kv, it, q, q_dtype, n_heads, out, out_dtype, lse, plan, ctx->scratch,
-                       nbl::split_counts(ctx, plan.grid), ctx->d_err);
+  nbl::launch_kv8_attn(ctx->stream, kv, it, q, q_dtype, n_heads, out, out_dtype, lse, plan, ctx->kv8_scratch, ctx->d_err);
 }
 
 // nbl_attn_decode on an 8-bit pool (context checked; with no rows there are no arrays).
@@ -427,6 +426,7 @@ int nbl_ctx_destroy(nbl_ctx* ctx) {
     for (auto& t : ctx->rope_tables) cudaFree(t.dev);
     for (auto& t : ctx->rotary_tables) cudaFree(t.dev);
     if (ctx->scratch) cudaFree(ctx->scratch);
+    if (ctx->kv8_scratch) cudaFree(ctx->kv8_scratch);
     if (ctx->split_counts) cudaFree(ctx->split_counts);
     if (ctx->io) cudaFree(ctx->io);
     for (cudaEvent_t e : ctx->events) cudaEventDestroy(e);
@@ -655,6 +655,14 @@ int nbl_kv_create(nbl_ctx* ctx, const nbl_kv_config* cfg, nbl_kv** out) {
       kv->pool = device_alloc(kv->bytes, "kv pool");
       nbl::check_cuda(cudaMemsetAsync(kv->pool, 0, kv->bytes, ctx->stream), "kv pool zero-fill");
       if (kv8) {  // read with bulk copies: no tensor map
+        if (!ctx->kv8_scratch) {
+          const size_t bytes = nbl::kv8_attn_scratch(ctx->num_sms);
+          void* scratch = device_alloc(bytes, "8-bit attention scratch");
+          const cudaError_t e = cudaMemsetAsync(scratch, 0, bytes, ctx->stream);
+          if (e != cudaSuccess) cudaFree(scratch);
+          nbl::check_cuda(e, "8-bit attention scratch");
+          ctx->kv8_scratch = scratch;
+        }
         nbl::launch_kv8_clear(ctx->stream, kv);
         nbl::check_cuda(cudaStreamSynchronize(ctx->stream), "kv pool zero-fill");
         ctx->kvs.push_back(kv);

@@ -181,19 +181,19 @@ void launch_kv8_export(cudaStream_t st, const nbl_kv* kv, const int32_t* page_id
 void launch_rotary_table(cudaStream_t st, float2* tab, int64_t n_pos, const double* freq, int n_pairs, double mul);
 
 struct Kv8AttnPlan {
-  int grid = 1;              // CTAs, and arrival counters
+  int grid = 1;              // CTAs
   int64_t tiles = 1;         // query tiles of the longest item
   int seg_cost = 0;          // what a unit costs besides its pages, in pages
-  size_t scratch_bytes = 0;  // parts of units that span CTAs
 };
 // max_kv: longest key range. q_dtype decides the row tile (8 rows of fp32 queries, whose two fp16 terms fill the 16 rows
 // of the instruction, or 16 rows of 16-bit queries).
 Kv8AttnPlan plan_kv8_attn(const nbl_kv* kv, int n_items, int max_len, int n_heads, int max_kv, int q_dtype,
                           int num_sms);
+// What any launch needs of scratch: arrival counters (0 between launches), then parts of units that span CTAs.
+size_t kv8_attn_scratch(int num_sms);
 // items.len == NULL: one fp32 query row per item at position pos0[i] - 1 (pos0 = sequence lengths, 0 = no keys).
 void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, const void* q, int q_dtype, int n_heads,
-                     void* out, int out_dtype, float* lse, const Kv8AttnPlan& plan, void* scratch, unsigned* counts,
-                     int* err);
+                     void* out, int out_dtype, float* lse, const Kv8AttnPlan& plan, void* scratch, int* err);
 
 // Whether the warp-level kernel takes query stretches of max_len tokens (else the tcgen05 one): its time grows with the rows
 // (tokens x heads of a group) that share each key, the other's stays until they pass 128 tokens. Measured, warp-level against

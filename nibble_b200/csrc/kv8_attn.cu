@@ -769,6 +769,23 @@ auto with_cfg(int d, bool hilo, F&& f) {
 
 }  // namespace
 
+namespace {
+constexpr size_t kCountBytes = 4096;  // of the counters
+}
+
+size_t kv8_attn_scratch(int num_sms) {
+  size_t most = 0;
+  for (int d : {64, 128})
+    for (bool hilo : {false, true})
+      with_cfg(d, hilo, [&](auto cfg) {
+        using C = decltype(cfg);
+        const size_t ctas = size_t(num_sms) * C::kCtas;
+        if (ctas * sizeof(unsigned) > kCountBytes) fail(NBL_E_UNSUPPORTED, "8-bit attention: more SMs than its counters are for");
+        most = std::max(most, ctas * 2 * C::kMergeFloats * sizeof(float));
+      });
+  return kCountBytes + most;
+}
+
 Kv8AttnPlan plan_kv8_attn(const nbl_kv* kv, int n_items, int max_len, int n_heads, int max_kv, int q_dtype,
                           int num_sms) {
   return with_cfg(kv->cfg.head_dim, q_dtype == NBL_F32, [&](auto cfg) {
@@ -781,14 +798,12 @@ Kv8AttnPlan plan_kv8_attn(const nbl_kv* kv, int n_items, int max_len, int n_head
     const double bound = double(n_items) * kv->cfg.n_kv_heads * double(tiles) * (double(max_pages) + C::kSegCost) / (C::kSegCost + 1);
     const int slots = num_sms * C::kCtas;
     p.grid = bound >= slots ? slots : std::max(1, static_cast<int>(std::ceil(bound)));
-    p.scratch_bytes = size_t(p.grid) * 2 * C::kMergeFloats * sizeof(float);
     return p;
   });
 }
 
 void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, const void* q, int q_dtype, int n_heads,
-                     void* out, int out_dtype, float* lse, const Kv8AttnPlan& plan, void* scratch, unsigned* counts,
-                     int* err) {
+                     void* out, int out_dtype, float* lse, const Kv8AttnPlan& plan, void* scratch, int* err) {
   const auto& c = kv->cfg;
   AttnArgs a{};
   a.it = items;
@@ -796,8 +811,8 @@ void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, c
   a.out = out;
   a.lse = lse;
   a.pool = static_cast<const uint8_t*>(kv->pool);
-  a.part = static_cast<float*>(scratch);
-  a.counts = counts;
+  a.counts = static_cast<unsigned*>(scratch);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + kCountBytes);
   a.err = err;
   a.n_pages = c.n_pages;
   a.q_dtype = q_dtype;

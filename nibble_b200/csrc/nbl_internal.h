@@ -67,6 +67,7 @@ struct nbl_ctx {
   int64_t reserved_ctx = 0, reserved_heads = 0;
   std::vector<nbl::RopeTable> rope_tables;
   std::vector<nbl::RotaryTable> rotary_tables;
+  void* kv8_scratch = nullptr;                 // arrival counters and parts of kv8_attn.cu: made with the first 8-bit pool, never moved
   std::vector<nbl_kv*> kvs;
   // nbl_decode_step_host: staging for the step's inputs/outputs and the two copy streams with their events
   void* io = nullptr;

@@ -327,3 +327,43 @@ def test_prefill_with_a_loose_max_q_len(nbl_ctx, dtype, most):
     for i, (p, m) in enumerate(items):
         check_rows(out.float().cpu().numpy(), qf, values, table[i], (0, 150)[i], p, m, dtype, every=11)
     kv.close()
+
+
+def test_decode_is_captured_at_its_first_call_and_outlives_scratch_growth(nbl_ctx):
+    """A graph of the decode: nothing is allocated at its first call, and a later call that grows the context's scratch leaves
+    what the graph uses where it is."""
+    import torch
+    import nibble_b200 as nb
+    ctx = nb.Context(0)
+    try:
+        lens, H, KV, D = [9000, 3, 0, 4100], 8, 2, 128
+        table, n_pages = make_page_tables(lens, shuffle_seed=1)
+        kv, values = random_pool(ctx, "int8", n_pages, KV, D, 3)
+        qs = np.random.default_rng(2).standard_normal((3, 4, H, D)).astype(np.float32)
+        q, t, n = dev(qs[0]), dev(table), ints(lens)
+        out, lse = torch.zeros((4, H, D), device="cuda"), torch.zeros((4, H), device="cuda")
+        torch.cuda.synchronize()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=side):
+            ctx.set_stream(side.cuda_stream)
+            ctx.attn_decode(kv, q, t, n, max(lens), out, lse)
+        ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        x = torch.randn((300, H, D), device="cuda").half()  # few works over many keys: parts in the context's scratch
+        free = torch.cuda.mem_get_info()[0]
+        ctx.attn_prefill(kv, x, ints([0]), ints([300]), ints([8700]), t, 300, torch.empty_like(x))
+        ctx.check()
+        assert torch.cuda.mem_get_info()[0] < free
+        for k in (1, 2):
+            q.copy_(dev(qs[k]))
+            graph.replay()
+            ctx.check()
+            for r, m in enumerate(lens):
+                keys, vals = rows_of(values, table[r], m)
+                ro, rl, size = attend(qs[k][r], keys, vals, m)
+                assert (np.abs(out[r].cpu().numpy() - ro) <= 2e-5 * size.max(-1, keepdims=True)).all()
+                got = lse[r].cpu().numpy()
+                assert np.isneginf(got).all() if m == 0 else np.abs(got - rl).max() <= 2e-5 * max(1.0, np.abs(rl).max())
+        del graph
+        kv.close()
+    finally:
+        ctx.close()
