@@ -325,7 +325,10 @@ NBL_API int nbl_attn_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int3
  * when the scale grows the old codes are rounded again to it (at most half a step of the new scale each time).
  * Magnitudes below 1e-30 in a whole page are stored as 0; an infinity or NaN is stored saturated or as 0 and flagged
  * (nbl_ctx_check). A page may be written by one item only in a call, and the items' rows do not overlap. An item with
- * rows, positions or a length out of bounds is left out and flagged. */
+ * rows, positions or a length out of bounds is left out and flagged.
+ * The first call with other rotary parameters, or with a wider table than before, makes their cos / sin table (8 bytes for
+ * each position of a table row and rotated pair) and waits for it, so make one before a stream capture. The context keeps
+ * the tables of the 16 parameter sets used last, each as wide as it was needed; a captured call goes with its table. */
 NBL_API int nbl_rotary_kv_append(nbl_ctx* ctx, nbl_kv* kv, const void* q_in, const void* k_in, const void* v_in,
                                  int32_t in_dtype, const float* bq, const float* bk, const float* bv, void* q_out,
                                  int32_t q_out_dtype, int64_t n_rows, const int32_t* q_start, const int32_t* q_len,

@@ -139,11 +139,17 @@ bool same_rotary(const nbl::RotaryTable& t, const nbl_rotary_params& rp, int n) 
          std::equal(t.factors.begin(), t.factors.end(), rp.freq_factors);
 }
 
-// The device cos/sin table of these parameters for positions [0, n_pos), made on first use and kept by the context.
+// The device cos/sin table of these parameters for positions [0, n_pos), made on first use. The context keeps the
+// kRotaryTables used last (a caller may change the scaling factor with every call).
 const nbl::RotaryTable& rotary_table(nbl_ctx* ctx, const nbl_rotary_params& rp, int n, int64_t n_pos) {
-  for (const auto& t : ctx->rotary_tables)
-    if (same_rotary(t, rp, n) && t.n_pos >= n_pos) return t;
+  ++ctx->rotary_uses;
+  for (auto& t : ctx->rotary_tables)
+    if (same_rotary(t, rp, n) && t.n_pos >= n_pos) {
+      t.used = ctx->rotary_uses;
+      return t;
+    }
   nbl::RotaryTable t;
+  t.used = ctx->rotary_uses;
   t.params = rp;
   t.params.freq_factors = nullptr;
   if (rp.freq_factors) t.factors.assign(rp.freq_factors, rp.freq_factors + n / 2);
@@ -166,12 +172,15 @@ const nbl::RotaryTable& rotary_table(nbl_ctx* ctx, const nbl_rotary_params& rp, 
     throw;
   }
   cudaFree(dev_freq);
-  for (auto it = ctx->rotary_tables.begin(); it != ctx->rotary_tables.end(); ++it)
-    if (same_rotary(*it, rp, n)) {  // a shorter table of the same parameters (its readers are done: the stream is idle)
-      cudaFree(it->dev);
-      ctx->rotary_tables.erase(it);
-      break;
-    }
+  // A shorter table of the same parameters goes, or the one not used for longest (its readers are done: the stream is idle).
+  auto& all = ctx->rotary_tables;
+  auto gone = std::find_if(all.begin(), all.end(), [&](const auto& o) { return same_rotary(o, rp, n); });
+  if (gone == all.end() && all.size() >= nbl::kRotaryTables)
+    gone = std::min_element(all.begin(), all.end(), [](const auto& x, const auto& y) { return x.used < y.used; });
+  if (gone != all.end()) {
+    cudaFree(gone->dev);
+    all.erase(gone);
+  }
   ctx->rotary_tables.push_back(std::move(t));
   return ctx->rotary_tables.back();
 }

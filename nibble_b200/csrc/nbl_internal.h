@@ -44,7 +44,9 @@ struct RotaryTable {
   int n = 0;
   int64_t n_pos = 0;
   float2* dev = nullptr;
+  uint64_t used = 0;            // the context's rotary_uses at its last use
 };
+constexpr size_t kRotaryTables = 16;  // that a context keeps
 
 }  // namespace nbl
 
@@ -67,6 +69,7 @@ struct nbl_ctx {
   int64_t reserved_ctx = 0, reserved_heads = 0;
   std::vector<nbl::RopeTable> rope_tables;
   std::vector<nbl::RotaryTable> rotary_tables;
+  uint64_t rotary_uses = 0;
   void* kv8_scratch = nullptr;                 // arrival counters and parts of kv8_attn.cu: made with the first 8-bit pool, never moved
   std::vector<nbl_kv*> kvs;
   // nbl_decode_step_host: staging for the step's inputs/outputs and the two copy streams with their events

@@ -367,3 +367,35 @@ def test_decode_is_captured_at_its_first_call_and_outlives_scratch_growth(nbl_ct
         kv.close()
     finally:
         ctx.close()
+
+
+def test_rotary_tables_of_many_parameters_do_not_pile_up(nbl_ctx):
+    """A scaling factor that changes with every call: old tables go, and one that is made again gives the same bits."""
+    import torch
+    import nibble_b200 as nb
+    ctx = nb.Context(0)
+    try:
+        kv = ctx.kv_pool(4, 1, 64, dtype=nb.I8)
+        width = 16384  # a table of 262144 positions x 32 pairs x 8 bytes: 64 MB
+        table = torch.full((1, width), -1, device="cuda", dtype=torch.int32)
+        table[0, :4] = ints([0, 1, 2, 3])
+        q, k = torch.randn((40, 2, 64), device="cuda"), torch.randn((40, 1, 64), device="cuda")
+
+        def rotated(factor):
+            out = torch.empty_like(q)
+            ctx.rotary_kv_append(kv, q, k, k, out, ints([0]), ints([40]), ints([7]), table, 40,
+                                 nb.RotarySpec(1e4, True, scaling="linear", factor=factor))
+            return out
+
+        first = rotated(1.0)
+        ctx.check()
+        free = torch.cuda.mem_get_info()[0]
+        outs = [rotated(1.0 + i / 8) for i in range(40)]
+        ctx.check()
+        assert free - torch.cuda.mem_get_info()[0] < 18 * (width * 16 * 32 * 8)
+        assert torch.equal(outs[0], first) and torch.equal(rotated(1.0), first) and torch.equal(rotated(5.75), outs[38])
+        assert not torch.equal(outs[1], first)
+        ctx.check()
+        kv.close()
+    finally:
+        ctx.close()
