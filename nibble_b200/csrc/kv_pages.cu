@@ -40,19 +40,20 @@ __device__ __forceinline__ void release_row(const PageBook& b, int32_t row, int*
 }
 
 // Sum over the block's threads of the values before this one (exclusive), and the total; every thread calls it.
-__device__ __forceinline__ int block_scan(int v, int& total) {
-  __shared__ int part[32];
+template <class T>
+__device__ __forceinline__ T block_scan(T v, T& total) {
+  __shared__ T part[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int inc = v;
+  T inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, inc, o);
+    const T x = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += x;
   }
   __syncthreads();  // part may still be read by an earlier call
   if (lane == 31) part[warp] = inc;
   __syncthreads();
-  int before = 0;
+  T before = 0;
   total = 0;
   for (int w = 0; w < warps; ++w) {
     if (w < warp) before += part[w];
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(kThreads) kv_fork_kernel(const PageBook b, con
   for (int i0 = 0; i0 < n; i0 += kThreads) {
     const int k = i0 + threadIdx.x;
     int add;
-    block_scan(k < n && __ldcg(&want[k].src_page) >= 0, add);
+    block_scan<int>(k < n && __ldcg(&want[k].src_page) >= 0, add);
     total += add;
   }
   const int found = collect_free(b, total, list);
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(kThreads) kv_fork_kernel(const PageBook b, con
     const int k = i0 + threadIdx.x;
     const bool wants = k < n && __ldcg(&want[k].src_page) >= 0;
     int add;
-    const int at = before + block_scan(wants, add);
+    const int at = before + block_scan<int>(wants, add);
     if (wants) {
       const int32_t row = __ldcg(&want[k].row), slot = __ldcg(&want[k].slot);
       if (at < found) {
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(kExtendThreads) kv_extend_kernel(const PageBoo
   __syncthreads();
   for (int i0 = 0; i0 < n; i0 += kExtendThreads) {
     const int i = i0 + threadIdx.x;
-    int need = 0;
+    int64_t need = 0;  // (the rows of one step may want more than 2^31 together)
     if (i < n) {
       const int32_t row = rows[i], to = new_lens[i];
       bool ok = row >= 0 && row < b.n_rows;
@@ -234,8 +235,8 @@ __global__ void __launch_bounds__(kExtendThreads) kv_extend_kernel(const PageBoo
         else need = (to + kPage - 1) / kPage - (len + kPage - 1) / kPage;
       }
     }
-    int add;
-    const int at = block_scan(need, add);
+    int64_t add;
+    const int64_t at = block_scan(need, add);
     if (i < n) before[i] = total + at;
     __syncthreads();
     if (threadIdx.x == 0) total += add;
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) compact_rank_kernel(const PageBook b
     const int32_t e = j < held ? b.table[at] : -1;
     const bool lead = page_ok(b, e) && __ldcg(&first[e]) == static_cast<unsigned>(at);
     int add;
-    const int id = before + block_scan(lead, add);
+    const int id = before + block_scan<int>(lead, add);
     if (lead) {
       new_id[e] = id;
       source[id] = e;

@@ -399,3 +399,21 @@ def test_rotary_tables_of_many_parameters_do_not_pile_up(nbl_ctx):
         kv.close()
     finally:
         ctx.close()
+
+
+def test_extend_by_more_pages_than_32_bits_count(nbl_ctx):
+    """Rows that want 2^31 pages together: there are not so many, so no row gets any."""
+    import torch
+    import nibble_b200 as nb
+    kv = nbl_ctx.kv_pool(64, 1)
+    width, rows = 2 ** 27 - 1, 17
+    table = torch.full((rows, width), -1, device="cuda", dtype=torch.int32)  # 9 GB
+    lens, refs = ints([0] * rows), ints([0] * 64)
+    nbl_ctx.kv_extend(kv, table, lens, refs, ints(range(rows)), ints([width * 16] * rows))
+    with pytest.raises(nb.NibbleError, match="no free page"):
+        nbl_ctx.check()
+    assert lens.tolist() == [0] * rows and refs.tolist() == [0] * 64 and (table[:, :64] == -1).all()
+    nbl_ctx.kv_extend(kv, table, lens, refs, ints([3]), ints([33]))
+    nbl_ctx.check()
+    assert table[3, :4].tolist() == [0, 1, 2, -1] and lens[3].item() == 33
+    kv.close()
