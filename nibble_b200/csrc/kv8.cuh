@@ -114,15 +114,25 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-// The same with an L2 eviction-priority hint.
-__device__ __forceinline__ void bulk_load_hint(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar,
-                                               uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-          smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
-}
+// Quotient and remainder of 0 <= n < 2^31 by a call's constant, without a division (Granlund and Montgomery, "Division by
+// invariant integers using multiplication", 1994): with 2^l >= d, the quotient is (n + floor(n m / 2^32)) >> l for
+// m = floor(2^32 (2^l - d) / d) + 1.
+struct Divisor {
+  uint32_t d = 1, m = 1, l = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t by) : d(by) {
+    while ((uint64_t(1) << l) < d) ++l;
+    m = static_cast<uint32_t>((uint64_t(1) << 32) * ((uint64_t(1) << l) - d) / d + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), m) + static_cast<uint32_t>(n)) >> l);
+  }
+  __device__ __forceinline__ int split(int& n) const {  // n becomes the quotient; returns the remainder
+    const int q = div(n), r = n - q * static_cast<int>(d);
+    n = q;
+    return r;
+  }
+};
 
 // An element of a float type as fp32, and back (one rounding).
 __device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {

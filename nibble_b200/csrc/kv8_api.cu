@@ -287,7 +287,7 @@ int nbl_kv_copy_pages(nbl_ctx* ctx, nbl_kv* kv, const int32_t* src_pages, const 
     if (n == 0) return;
     require_arrays("kv_copy_pages", src_pages, dst_pages);
     use(ctx);
-    nbl::launch_copy_pages(ctx->stream, kv, src_pages, dst_pages, n, ctx->d_err, ctx->num_sms);
+    nbl::launch_copy_pages(ctx->stream, kv, src_pages, dst_pages, n, ctx->d_err);
   });
 }
 

@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "kv8.cuh"
+#include "softmax_tile.cuh"
 
 namespace nbl {
 namespace {
@@ -80,20 +81,6 @@ struct Cfg {
   static_assert(kOffQ % 16 == 0 && kOffBar % 8 == 0 && kStages >= kConsumers, "layout");
 };
 
-// n / d for 0 <= n < 2^31 by a multiplication (the divisors are a call's constants): with 2^l >= d, the quotient is
-// (n + floor(n m / 2^32)) >> l for m = floor(2^32 (2^l - d) / d) + 1.
-struct FastDiv {
-  uint32_t d = 1, m = 1, l = 0;
-  FastDiv() = default;
-  explicit FastDiv(uint32_t div) : d(div) {
-    while ((uint64_t(1) << l) < d) ++l;
-    m = static_cast<uint32_t>((uint64_t(1) << 32) * ((uint64_t(1) << l) - d) / d + 1);
-  }
-  __device__ __forceinline__ int div(int n) const {
-    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), m) + static_cast<uint32_t>(n)) >> l);
-  }
-};
-
 struct AttnArgs {
   Kv8Items it;
   const void* q;
@@ -107,7 +94,7 @@ struct AttnArgs {
   int q_dtype, out_dtype;
   int n_heads, n_kv_heads, group;
   int tile0, n_tiles;  // the items' query tiles of this launch
-  FastDiv by_group, by_kv_heads;
+  Divisor by_group, by_kv_heads;
   int q_vec;         // q allows 4-element loads
   float scale_log2;  // log2(e) / sqrt(D)
 };
@@ -122,12 +109,6 @@ __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4],
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Four consecutive elements of q as fp32.
@@ -152,15 +133,11 @@ __device__ __forceinline__ void load4q(const AttnArgs& a, int64_t i, float (&v)[
   }
 }
 
-__device__ __forceinline__ uint32_t pack(float x, float y) {
-  const __half2 h = __floats2half2_rn(x, y);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ void split_half2(float2 x, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(x.x, x.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   const float2 r = __ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), x);  // exact
-  lo = pack(r.x, r.y);
+  lo = pack2<false>(r.x, r.y);
 }
 
 // An item's rows and keys as the kernel takes them; pages 0 when there is nothing to do.
@@ -396,8 +373,8 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
         split_half2(make_float2(x[2] * inv, x[3] * inv), hi1, lo1);
         s_q[at] = make_uint4(hi0, lo0, hi1, lo1);
       } else {
-        hi0 = pack(x[0] * inv, x[1] * inv);
-        hi1 = pack(x[2] * inv, x[3] * inv);
+        hi0 = pack2<false>(x[0] * inv, x[1] * inv);
+        hi1 = pack2<false>(x[2] * inv, x[3] * inv);
         uint32_t* w = reinterpret_cast<uint32_t*>(&s_q[at]) + (row >> 3);
         w[0] = hi0;
         w[2] = hi1;
@@ -449,7 +426,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
 #pragma unroll 4
       for (int k = first; k <= last; ++k) {
         const float* pb = part(k);
-        const float e = ex2(__ldcg(pb + ROWS * D + r) - mu);
+        const float e = fast_exp2(__ldcg(pb + ROWS * D + r) - mu);
         const float4 x = __ldcg(reinterpret_cast<const float4*>(pb + r * D + d));
         L = fmaf(e, __ldcg(pb + ROWS * D + ROWS + r), L);
         O.x = fmaf(e, x.x, O.x), O.y = fmaf(e, x.y, O.y), O.z = fmaf(e, x.z, O.z), O.w = fmaf(e, x.w, O.w);
@@ -555,7 +532,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float mn = fmaxf(m_run[n], mx);
         const float mu = mn == -INFINITY ? 0.f : mn;
-        al[n] = ex2(m_run[n] - mu);
+        al[n] = fast_exp2(m_run[n] - mu);
         m_run[n] = mn;
         float2 ps = make_float2(0.f, 0.f);
 #pragma unroll
@@ -564,7 +541,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const float2 x = __ffma2_rn(s[n][j][c], make_float2(f, f), make_float2(-mu, -mu));
-            float2 p = make_float2(ex2(x.x), ex2(x.y));
+            float2 p = make_float2(fast_exp2(x.x), fast_exp2(x.y));
             if constexpr (!FULL) {
               if (s[n][j][c].x == -INFINITY) p.x = 0.f;
               if (s[n][j][c].y == -INFINITY) p.y = 0.f;
@@ -596,8 +573,8 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
             split_half2(x, pa[j][2 * c], pa[j][2 * c + 1]);
           } else {
             const float2 y = __fmul2_rn(s[NR - 1][j][c], r);
-            pa[j][2 * c] = pack(x.x, x.y);
-            pa[j][2 * c + 1] = pack(y.x, y.y);
+            pa[j][2 * c] = pack2<false>(x.x, x.y);
+            pa[j][2 * c + 1] = pack2<false>(y.x, y.y);
           }
         }
       }
@@ -695,7 +672,7 @@ __global__ void __launch_bounds__(Cfg<D, HILO>::kThreads, Cfg<D, HILO>::kCtas) k
 #pragma unroll
       for (int w = 0; w < kConsumers; ++w) {
         const float* wb = mrg + w * C::kMergeFloats;
-        const float k = ex2(wb[ROWS * D + r] - mu);  // 0 for warps that saw no key
+        const float k = fast_exp2(wb[ROWS * D + r] - mu);  // 0 for warps that saw no key
         const float4 x = *reinterpret_cast<const float4*>(wb + r * D + d);
         L = fmaf(k, wb[ROWS * D + ROWS + r], L);
         O.x = fmaf(k, x.x, O.x), O.y = fmaf(k, x.y, O.y), O.z = fmaf(k, x.z, O.z), O.w = fmaf(k, x.w, O.w);
@@ -820,8 +797,8 @@ void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, c
   a.n_heads = n_heads;
   a.n_kv_heads = c.n_kv_heads;
   a.group = n_heads / c.n_kv_heads;
-  a.by_group = FastDiv(static_cast<uint32_t>(a.group));
-  a.by_kv_heads = FastDiv(static_cast<uint32_t>(c.n_kv_heads));
+  a.by_group = Divisor(static_cast<uint32_t>(a.group));
+  a.by_kv_heads = Divisor(static_cast<uint32_t>(c.n_kv_heads));
   const uintptr_t bits = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out);
   a.q_vec = (bits & 15u) == 0;
   a.scale_log2 = 1.4426950408889634f / std::sqrt(static_cast<float>(c.head_dim));

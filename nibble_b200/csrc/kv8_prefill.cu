@@ -92,22 +92,6 @@ struct PCfg {
   __host__ __device__ static constexpr uint32_t col_o(int g) { return NH * SB * kBN + g * D; }
 };
 
-// n / d and n % d of n < 2^31 without a division: q = (high word of n m + n) >> l with l = ceil(log2 d) and
-// m = floor(2^32 (2^l - d) / d) + 1.
-struct Divisor {
-  uint32_t d = 1, m = 1, l = 0;
-  Divisor() = default;
-  explicit Divisor(uint32_t d) : d(d) {
-    while ((uint64_t(1) << l) < d) ++l;
-    m = static_cast<uint32_t>(((uint64_t(1) << l) - d << 32) / d) + 1;
-  }
-  __device__ __forceinline__ int split(int& n) const {  // n becomes the quotient; returns the remainder
-    const uint32_t x = static_cast<uint32_t>(n), q = (__umulhi(x, m) + x) >> l;
-    n = static_cast<int>(q);
-    return static_cast<int>(x - q * d);
-  }
-};
-
 struct PrefillArgs {
   Kv8Items it;
   const uint8_t* pool;

@@ -402,9 +402,7 @@ unsigned copy_pieces(int64_t page_bytes) {
 
 int64_t kv_page_bytes(const nbl_kv* kv) { return static_cast<int64_t>(kv->bytes / static_cast<size_t>(kv->cfg.n_pages)); }
 
-void launch_copy_pages(cudaStream_t st, const nbl_kv* kv, const int32_t* src, const int32_t* dst, int n, int* err,
-                       int num_sms) {
-  (void)num_sms;
+void launch_copy_pages(cudaStream_t st, const nbl_kv* kv, const int32_t* src, const int32_t* dst, int n, int* err) {
   const int64_t pb = kv_page_bytes(kv);
   kv_copy_pages_kernel<<<dim3(static_cast<unsigned>(n), copy_pieces(pb)), kThreads, 0, st>>>(
       static_cast<uint8_t*>(kv->pool), pb, kv->cfg.n_pages, src, dst, err);

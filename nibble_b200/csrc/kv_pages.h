@@ -17,8 +17,7 @@ struct PageBook {
 };
 
 int64_t kv_page_bytes(const nbl_kv* kv);
-void launch_copy_pages(cudaStream_t st, const nbl_kv* kv, const int32_t* src, const int32_t* dst, int n, int* err,
-                       int num_sms);
+void launch_copy_pages(cudaStream_t st, const nbl_kv* kv, const int32_t* src, const int32_t* dst, int n, int* err);
 // scratch: at least kv_book_scratch(n, n_pages) bytes; count: one arrival counter, 0 between launches.
 size_t kv_book_scratch(int n, int64_t n_pages);
 void launch_kv_fork(cudaStream_t st, const nbl_kv* kv, const PageBook& b, const int32_t* src_rows,

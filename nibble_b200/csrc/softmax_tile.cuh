@@ -1,5 +1,5 @@
-// Device helpers shared by the tcgen05 attention kernels (prefill.cu, kv8_prefill.cu): Q tile loads, TMEM row loads,
-// exponentials and row maxima of a softmax whose thread owns a query row.
+// Device helpers shared by the attention kernels (prefill.cu, kv8_prefill.cu, kv8_attn.cu): Q tile loads, TMEM row loads,
+// exponentials, packing, and row maxima of a softmax whose thread owns a query row.
 #pragma once
 #include "nbl_device.cuh"
 
