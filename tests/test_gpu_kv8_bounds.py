@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 
 from nibble_b200.workloads import make_page_tables
-from test_gpu_kv8 import QMAX, attend, check_decode, dev, export, ints, np_of, random_pool, rows_of
+from test_gpu_kv8 import (QMAX, PlainCache, append_both, attend, check_decode, dev, export, ints, np_of, random_pool,
+                          rows_of)
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -416,4 +417,64 @@ def test_extend_by_more_pages_than_32_bits_count(nbl_ctx):
     nbl_ctx.kv_extend(kv, table, lens, refs, ints([3]), ints([33]))
     nbl_ctx.check()
     assert table[3, :4].tolist() == [0, 1, 2, -1] and lens[3].item() == 33
+    kv.close()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("offset", [1, 2, 4])
+def test_attention_off_alignment(nbl_ctx, dtype, D, offset):
+    """q and out that begin off a 16-byte boundary: many query tokens, and the decode."""
+    import torch
+    items, H, KV = [(700, 100), (0, 33)], 6, 2
+    table, n_pages = make_page_tables([p + m for p, m in items], shuffle_seed=1)
+    kv, values = random_pool(nbl_ctx, "int8", n_pages, KV, D, 3, spread=0.5)
+    dt = getattr(torch, dtype)
+    q, qf = np_of(np.random.default_rng(1).standard_normal((133, H, D)).astype(np.float32), dt)
+
+    def moved(t):
+        flat = torch.full((t.numel() + offset,), NAN, device="cuda", dtype=t.dtype)
+        flat[offset:] = t.reshape(-1)
+        return flat[offset:].view(t.shape)
+
+    out = moved(torch.full_like(q, NAN))
+    nbl_ctx.attn_prefill(kv, moved(q), ints([0, 100]), ints([100, 33]), ints([700, 0]), dev(table), 100, out)
+    nbl_ctx.check()
+    for i, (p, m) in enumerate(items):
+        check_rows(out.float().cpu().numpy(), qf, values, table[i], (0, 100)[i], p, m, dtype, every=7)
+    if dtype == "float32":
+        got = moved(torch.full_like(q[:2], NAN))
+        nbl_ctx.attn_decode(kv, moved(q[:2]), dev(table), ints([800, 33]), 800, got)
+        nbl_ctx.check()
+        for r, n in enumerate((800, 33)):
+            k, v = rows_of(values, table[r], n)
+            ro, _, size = attend(qf[r], k, v, n)
+            assert (np.abs(got[r].cpu().numpy() - ro) <= 2e-5 * size.max(-1, keepdims=True)).all()
+    kv.close()
+
+
+@pytest.mark.parametrize("count", [256, 257, 400])
+def test_append_and_read_of_many_items(nbl_ctx, count):
+    """More items than a warp of every block adds up (and as many): page u is then page u % most of item u / most."""
+    import torch
+    import nibble_b200 as nb
+    rng = np.random.default_rng(count)
+    items = [(int(rng.integers(0, 40)), int(rng.integers(0, 35))) for _ in range(count)]
+    table, n_pages = make_page_tables([p + m for p, m in items], shuffle_seed=5)
+    kv = nbl_ctx.kv_pool(n_pages, 1, dtype=nb.I8)
+    plain = PlainCache("int8", n_pages, 1, 64)
+    q, want = append_both(nbl_ctx, kv, plain, table, items, 2, nb.RotarySpec(1e4, True), torch.float16, rng)
+    nbl_ctx.check()
+    codes, scales = export(nbl_ctx, kv)
+    assert np.array_equal(scales, plain.scales) and np.array_equal(codes, plain.codes)
+    assert (np.abs(q.float().cpu().numpy() - want) <= np.abs(want).max(-1, keepdims=True) * 4 * 2.0 ** -24 + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all()
+    starts = np.cumsum([0] + [m for _, m in items])[:-1]
+    n = sum(m for _, m in items)
+    k, v = (torch.full((n, 1, 64), NAN, device="cuda") for _ in range(2))
+    nbl_ctx.kv_read(kv, ints(starts), ints([m for _, m in items]), ints([p for p, _ in items]), dev(table), 34, k, v)
+    nbl_ctx.check()
+    values = codes.astype(np.float64) * scales.astype(np.float64)[..., None, None]
+    for i, (p, m) in enumerate(items):
+        for got, ref in zip((k, v), rows_of(values, table[i], p + m)):
+            assert np.array_equal(got[starts[i]:starts[i] + m].cpu().numpy(), ref[p:p + m].astype(np.float32))
     kv.close()
