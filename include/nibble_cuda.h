@@ -128,7 +128,8 @@ NBL_API int nbl_ctx_create(int device, nbl_ctx** out);
  * blocks, cpu_backend.cpp:70-72). */
 NBL_API int nbl_ctx_destroy(nbl_ctx* ctx);
 /* Runs later launches on `stream` (a cudaStream_t; NULL is CUDA's default stream). A new context runs on a
- * stream of its own until this is called. */
+ * stream of its own until this is called. The context's calls share its scratch: what runs on the stream before has to be done, or
+ * ordered before what follows (cudaStreamWaitEvent), when the next call is made on another. */
 NBL_API int nbl_ctx_set_stream(nbl_ctx* ctx, void* stream);
 /* Returns the context to its own stream. */
 NBL_API int nbl_ctx_use_own_stream(nbl_ctx* ctx);

@@ -17,7 +17,7 @@
 //             the subnormal codes), so codes 0 and 1 stand at those bits of the word's two halves, and codes 2 and 3 at the
 //             bits between (sign at bit 14, the rest at 6..0): one mask gives the first pair, two shifts and two
 //             masks the second. (The conversion instruction runs at a quarter of that rate: decode of 256 rows of 4097
-//             tokens took 262 us with it, as against 207 us for NBL_I8.)
+//             tokens took 262 us with it, when NBL_I8 took 207.)
 // Every code and scale in a pool is finite: the append saturates and the import refuses, so a masked token's weight
 // of 0 always gives 0.
 #pragma once
@@ -207,9 +207,9 @@ void launch_kv8_attn(cudaStream_t st, const nbl_kv* kv, const Kv8Items& items, c
 
 // Whether the warp-level kernel takes query stretches of max_len tokens (else the tcgen05 one): its time grows with the rows
 // (tokens x heads of a group) that share each key, the other's stays until they pass 128 tokens. Measured, warp-level against
-// tcgen05, 8 items at 4000 keys, heads of 64: 32/4 heads 27 / 37 / 60 us for 8 / 16 / 32 tokens against 68 / 68 / 72, 8/8
-// heads 39 for 64 tokens against 76. Heads of 128: one item at 16k, 32/8 heads, 41 / 50 / 75 for 8 / 16 / 32 against 54 / 54 /
-// 55; 8 items at 4000, 8/8 heads, 77 for 64 against 49.
+// tcgen05, 8 items at 4000 keys, heads of 64: 32/4 heads 27 / 38 / 61 us for 8 / 16 / 32 tokens against 68 / 68 / 72, 8/8
+// heads 41 for 64 tokens against 76. Heads of 128: one item at 16k, 32/8 heads, 45 / 52 / 75 for 8 / 16 / 32 against 54 / 54 /
+// 59; 8 items at 4000, 8/8 heads, 77 for 64 against 49.
 inline bool kv8_few_tokens(int head_dim, int group, int max_len) {
   return head_dim == 64 ? max_len <= 64 && int64_t(max_len) * group <= 288
                         : max_len <= 24 && int64_t(max_len) * group <= 72;

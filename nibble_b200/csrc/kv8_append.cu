@@ -8,8 +8,8 @@
 // places after the last token are set to 0. Products use the fp32 reciprocal of s; all of it is IEEE fp32, each step
 // rounded once, so the codes do not depend on how the work is spread over threads.
 //
-// Measured, append and read back of the same tokens: 24 prompts of 97..2047 tokens, 32/4 heads of 64, bf16: 49 us, 3.8 TB/s;
-// 8191 tokens, 28/4 heads of 128, fp16, scaled positions: 55 us, 3.1 TB/s; 64 single tokens of 32/8 heads, fp32: 17 us, the
+// Measured, append and read back of the same tokens: 24 prompts of 97..2047 tokens, 32/4 heads of 64, bf16: 51 us, 3.6 TB/s;
+// 8191 tokens, 28/4 heads of 128, fp16, scaled positions: 56 us, 3.0 TB/s; 64 single tokens of 32/8 heads, fp32: 17 us, the
 // two calls' time on the host. What the longer ones lose to the copy rate goes to issue slots (68 % busy: rotation, rounding,
 // byte exchange) and to the latency of short CTAs (one page of one head: 2-4 KB in, the block's maximum, 1-2 KB out).
 #include <algorithm>

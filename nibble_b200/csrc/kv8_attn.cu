@@ -31,10 +31,12 @@
 //   multiply-add that rescales O anyway.
 //
 // Measured: 256 rows of 4097 tokens, 32/8 heads of 64: 222 us, 4.9 TB/s of codes and scales (75 % of the measured copy rate)
-// with other pools of that size read in between; 4 rows of 131073, 32/8 heads of 128: 209 us, 5.1 TB/s (79 %); 48 rows of 511..16384, 28/4 heads of 128: 55 us, 4.1 TB/s: the launch, the CTAs' search
-// for their stretch, the first loads and the joining of partials take about 12 us of a call that short. One row of 257 tokens:
-// 9 us, the launch and one chain of loads. Walking the KV heads of the same pages side by side in neighbouring CTAs, for
-// the sake of whole pages: 217 and 199 us, and 18.4 against 16.8 for 8 items of 5 drafted tokens.
+// with other pools of that size read in between; 4 rows of 131073, 32/8 heads of 128: 209 us, 5.1 TB/s (79 %). Counters of smaller
+// calls of both: issue slots 47 % and 39 % busy, 3.6 and 2.8 warps resident a scheduler and 0.8 and 0.6 of them ready: the
+// latency of few warps. 48 rows of 511..16384, 28/4 heads of 128: 55 us, 4.1 TB/s: the launch, the CTAs' search for their
+// stretch, the first loads and the joining of partials take about 12 us of a call that short. One row of 257 tokens: 8 us, the
+// launch and one chain of loads. Walking the KV heads of the same pages side by side in neighbouring CTAs, for the sake of
+// whole pages: 217 us where it took 217, 199 where it took 195, and 18.4 against 16.8 for 8 items of 5 drafted tokens.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>

@@ -21,13 +21,13 @@
 //   last    MMA issuer: S_g = Q_g K^T, O_g += P_g V with P read from TMEM.
 // D = 64, groups of three heads or more: four heads a CTA (TMEM is then full: S and P share 64 columns a head), so a
 // converted tile serves four heads; three converting warps (with two, which also kept the pace of 4200 cycles a tile, 4
-// prompts of 2048 tokens at 32/4 heads took 138 us, with three 125; a fourth would leave the others too few registers).
+// prompts of 2048 tokens at 32/4 heads took 138 us, with three 126; a fourth would leave the others too few registers).
 // Smaller groups: two heads, two CTAs per SM. D = 128: two heads fill TMEM with S double-buffered, the next tile's S is
 // computed during a tile's softmax; four converting warps.
 // What bounds it: at D = 64 the chain S -> max -> exponentials -> P -> P V of a head (the SFU, 16 exponentials a clock, is
 // busy 50 % of the time, the tensor cores 25 %); at D = 128 the tensor cores' reading of Q and K from shared memory for
 // 64-key tiles (48 cycles an instruction where the product takes 32) beside the same chain. Measured: 4 prompts of 2048
-// tokens, 32/4 heads of 64: 125 us; one of 8192: 408 us, 670 TFLOP/s; at D = 128 540 us, 1000 TFLOP/s.
+// tokens, 32/4 heads of 64: 126 us; one of 8192: 409 us, 670 TFLOP/s; at 32/8 heads of 128 572 us, 960 TFLOP/s.
 // Taking the weights against the last tiles' maximum while this tile's is found (to shorten the chain) spilled registers:
 // 208 us. Polynomials for one exponential in 8, 4, 3: 145, 147, 151 us where none took 138. With the works found, and Q
 // fetched, by the issuing warp and the softmax warps each for itself, starting on a work took 4000 cycles, as long as a tile.
