@@ -832,6 +832,12 @@ def decode_ragged(args, world, rank, local, steps, warmup):
 
 
 # ---------------------------------------------------------------- CPU baseline: nibble's own CpuBackend
+def no_reference():
+    """Why nibble's own CPU backend cannot run here, as a record; None where it can."""
+    import oracle
+    return None if oracle.have_ref() else {"unavailable": "nibble's CPU backend is not built: its sources are not there"}
+
+
 def cpu_baseline(seconds=10.0, n_bufs=48):
     """CpuBackend::attention (AVX2/AVX-VNNI tier, ThreadPool of all host threads) on config-2 rows: one call per
     (sequence, layer) with q [1, 32, 64] and the row's 4097-token cache widened to fp32 [4097, 8, 64]. Enough
@@ -930,7 +936,8 @@ def main():
     if args.impl == "reference":
         if int(os.environ.get("RANK", "0")) != 0:
             return
-        print(json.dumps(reference_arm(args)), flush=True)
+        none = no_reference()
+        print(json.dumps({"impl": "reference", **none} if none else reference_arm(args)), flush=True)
         return
 
     world, rank, local = dist_setup(args.gpus)
@@ -965,10 +972,7 @@ def main():
                 "vs_baseline": None, "data": "synthetic (seeded N(0,1))"})
     res["gpu_launches"] = res.pop("gpu_launches_per_step", 2) * args.steps
     if rank == 0 and world == 1 and args.cpu_seconds > 0 and args.workload == "decode_batched":
-        try:
-            res["cpu_baseline"] = cpu_baseline(args.cpu_seconds)
-        except OSError as e:  # nibble's own backend could not be compiled: its sources are not there
-            res["cpu_baseline"] = {"unavailable": str(e)}
+        res["cpu_baseline"] = no_reference() or cpu_baseline(args.cpu_seconds)
     if world > 1:
         import torch.distributed as dist
         dist.barrier()
