@@ -131,10 +131,10 @@ def _dtype(t) -> int:
 
 
 def _new_rows(kv, q, k, v, q_out):
-    """(rows, query heads) of tokens for kv: q and q_out [rows, heads, D], k and v [rows, kv heads, D]."""
+    """(rows, query heads) of tokens for kv: q [rows, heads, D], q_out as many elements, k and v [rows, kv heads, D]."""
     shape = q.shape
     n, heads, dim = shape
-    if dim != kv.head_dim or q_out.shape != shape or k.shape != (n, kv.n_kv_heads, dim) or v.shape != k.shape:
+    if dim != kv.head_dim or q_out.numel() != n * heads * dim or k.shape != (n, kv.n_kv_heads, dim) or v.shape != k.shape:
         raise ValueError(f"expected q_in, q_out [rows, n_heads, {kv.head_dim}] and k_in, v_in [rows, {kv.n_kv_heads}, {kv.head_dim}]")
     return n, heads
 
@@ -174,9 +174,9 @@ def _check_pages(kv, page_ids, codes, scales):
         return
     want = (page_ids.numel(), 2, kv.n_kv_heads, kv.page_size, kv.head_dim)
     types = ("int8", "uint8", "float8_e4m3fn") if kv.dtype == E4M3 else ("int8", "uint8")
-    if codes.shape != want or str(codes.dtype).replace("torch.", "") not in types:
+    if codes.numel() != want[0] * 2 * want[2] * want[3] * want[4] or str(codes.dtype).replace("torch.", "") not in types:
         raise ValueError(f"expected codes {list(want)} of {' or '.join(types)}")
-    if scales.shape != want[:3] or _dtype(scales) != F32:
+    if scales.numel() != want[0] * 2 * want[2] or _dtype(scales) != F32:
         raise ValueError(f"expected float32 scales {list(want[:3])}")
 
 
@@ -424,10 +424,10 @@ class Context:
     def attn_decode(self, kv: KVPool, q, page_table, seq_lens, max_seq_len: int, out, lse=None, n_splits: int = 0):
         """One query token per row: q/out [rows, n_heads, head_dim] fp32, page_table [rows, stride] int32."""
         if kv.dtype in _EIGHT_BITS:
-            (rows, heads, dim), (tables, stride), f32 = q.shape, page_table.shape, q.dtype
+            (rows, heads, dim), stride, f32 = q.shape, page_table.shape[-1], q.dtype
             if dim != kv.head_dim or _dtype(q) != F32 or out.dtype != f32 or out.numel() < rows * heads * dim:
                 raise ValueError(f"expected float32 q and out [rows, n_heads, {kv.head_dim}]")
-            if tables < rows or seq_lens.numel() < rows:
+            if page_table.numel() < rows * stride or seq_lens.numel() < rows:
                 raise ValueError("expected a length and a page-table row for each row of q")
             if lse is not None and (lse.dtype != f32 or lse.numel() < rows * heads):
                 raise ValueError("expected a float32 lse [rows, n_heads]")
@@ -496,11 +496,10 @@ class Context:
         like = k_out if k_out is not None else v_out
         if like is None:
             raise ValueError("kv_read needs k_out or v_out")
-        shape = like.shape
-        n_rows, heads, dim = shape
-        if heads != kv.n_kv_heads or dim != kv.head_dim or (
-                like is not v_out and v_out is not None and (v_out.shape != shape or v_out.dtype is not like.dtype)):
-            raise ValueError(f"expected k_out and v_out [rows, {kv.n_kv_heads}, {kv.head_dim}] of one shape and dtype")
+        n_rows, size = like.shape[0], like.numel()
+        if size != n_rows * kv.n_kv_heads * kv.head_dim or (
+                like is not v_out and v_out is not None and (v_out.numel() != size or v_out.dtype is not like.dtype)):
+            raise ValueError(f"expected k_out and v_out [rows, {kv.n_kv_heads}, {kv.head_dim}] of one size and dtype")
         first, n, pos0, table, stride, n_items = _items(start, length, kv_pos0, page_table)
         check(_abi.lib.nbl_kv_read(self.handle, kv.handle, n_rows, first, n, pos0, table, stride, n_items, max_len,
                                    _ptr(k_out), _ptr(v_out), _dtype(like)))

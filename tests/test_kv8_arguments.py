@@ -62,7 +62,8 @@ def test_kv_read(ctx, lib):
 
     for k, v in ((rows(), rows()), (rows(), None), (None, rows()), (rows(dtype=torch.half), rows(dtype=torch.half))):
         read(k, v)
-    assert lib.calls == ["nbl_kv_read"] * 4
+    read(rows().reshape(5, -1), rows())
+    assert lib.calls == ["nbl_kv_read"] * 5
     refused(lib, read)
     refused(lib, read, rows(), rows(dtype=torch.half))  # v_out would be written as float32
     refused(lib, read, rows(), rows(4))
@@ -82,10 +83,10 @@ def test_append_outputs_biases_and_items(ctx, lib):
     append()
     append(bq=torch.zeros(4 * D), bk=torch.zeros(KV, D), bv=torch.zeros(KV * D))
     append(q_out=rows(heads=4, dtype=torch.bfloat16), table=ints(7, 4))
-    assert len(lib.calls) == 3
+    append(q_out=rows(heads=4).reshape(5, -1))
+    assert len(lib.calls) == 4
     refused(lib, append, q_out=rows(4, heads=4))
     refused(lib, append, q_out=rows(heads=3))
-    refused(lib, append, q_out=rows(heads=4).reshape(-1))
     for name, heads in (("bq", 4), ("bk", KV), ("bv", KV)):
         refused(lib, append, **{name: torch.zeros(heads * D, dtype=torch.bfloat16)})  # was read as float32
         refused(lib, append, **{name: torch.zeros(heads * D - 1)})
@@ -116,7 +117,8 @@ def test_import_and_export_pages(ctx, lib, name):
     call(dtype=torch.uint8)
     call(nb.E4M3, dtype=torch.float8_e4m3fn)
     call(nb.E4M3)
-    assert len(lib.calls) == 4
+    call(codes=(3, 2, KV, 16 * D), scales=(3, 2 * KV))  # (flat)
+    assert len(lib.calls) == 5
     refused(lib, call, n=4)  # more pages than codes
     refused(lib, call, codes=(3, 2, KV, 16, 32))
     refused(lib, call, codes=(3, 2, 1, 16, D))
@@ -192,7 +194,8 @@ def test_decode_queries_and_rows(ctx, lib):
 
     decode()
     decode(lse=torch.zeros((5, 4)), lens=ints(6), table=ints(6, 4))
-    assert len(lib.calls) == 2
+    decode(q=rows(1, heads=4), lens=ints(1), table=ints(4))  # a single row's table
+    assert len(lib.calls) == 3
     refused(lib, decode, q=rows(heads=4, dtype=torch.half))  # was read as float32
     refused(lib, decode, out=rows(heads=4, dtype=torch.half))
     refused(lib, decode, out=rows(4, heads=4))
