@@ -309,7 +309,8 @@ NBL_API int nbl_attn_decode_static(nbl_ctx* ctx, const nbl_kv* kv, const float* 
  * accumulation in TMEM.
  * An 8-bit pool (NBL_I8, NBL_E4M3; head_dim 64 or 128) takes q in F32, F16 or BF16 and writes out in F32 or q's dtype;
  * the scales are applied to scores and weights in fp32, the weights of 16-bit queries are rounded to fp16. A head whose
- * query has an infinity or NaN gets NaN. */
+ * query has an infinity or NaN gets NaN. (fp32 queries, and few tokens, are attended by the decode's kernel, within its bound
+ * for value scales far apart.) */
 NBL_API int nbl_attn_prefill(nbl_ctx* ctx, const nbl_kv* kv, const void* q, int32_t q_dtype, int64_t n_q_rows,
                      const int32_t* q_start, const int32_t* q_len, const int32_t* kv_pos0, const int32_t* page_table,
                      int32_t pt_stride, int32_t n_items, int32_t n_heads, int32_t max_q_len, void* out,
